@@ -1,0 +1,583 @@
+// Attention for training, head_dim 64: a forward pass that keeps the row statistics and the backward pass that recomputes the
+// probabilities from them (include/dbir.h, dbir_attn_desc).  With c = scale, per (batch, head) and over the visible keys j of row i:
+//   s_ij = c q_i . k_j       lse_i = log sum_j exp(s_ij)      p_ij = exp(s_ij - lse_i)      o_i = sum_j p_ij v_j
+//   D_i = do_i . o_i         dv_j = sum_i p_ij do_i           dp_ij = do_i . v_j            ds_ij = p_ij (dp_ij - D_i)
+//   dq_i = c sum_j ds_ij k_j                                  dk_j = c sum_i ds_ij q_i      (dk, dv: also over the heads of a group)
+// Nothing of size Lq x Lk leaves the registers.  The backward pass is two kernels, one that owns keys (dk, dv) and one that owns
+// queries (dq), each with its sums in registers: 7 products a pair of tiles where one kernel would need 5, but then no atomics (the
+// result is the same in every run) and no Lq x 64 partial sum for every block of keys in memory.
+//
+// Every product is v_mfma_f32_32x32x16 (A: row = lane & 31, k = 8 (lane >> 5) + j; B: column = lane & 31, same k; C: column =
+// lane & 31, row = (r & 3) + 8 (r >> 2) + 4 (lane >> 5)).  The score tile is computed so that the index the second product sums over
+// is the ROW of C: registers 8 s .. 8 s + 7 then are a B operand of k-step s whose k runs in the order 16 s + 4 (lane >> 5) + (j & 3) +
+// 8 (j >> 2), and the A operand follows that order by reading the row-major tile through two transposing LDS reads of four rows.
+#include <math.h>
+
+#include "common.h"
+
+namespace {
+
+constexpr int HD = 64;             // head dimension
+constexpr int TILE = 64;           // rows of a tile in LDS
+constexpr int TILE_BYTES = TILE * HD * 2;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+struct Args {
+  const u16 *q, *k, *v, *o_in, *dout;
+  u16 *o, *dq, *dk, *dv;
+  long long qs[3], ks[3], vs[3], os[3], gs[3], dqs[3], dks[3], dvs[3];  // batch, row, head strides in elements
+  float* lse;             // [B, H, Lq]
+  const int *q_len, *kv_len;
+  float *nl2, *nd;        // [B * H, Lqp]: -lse * log2(e) and -D, -inf and 0 behind the last row
+  float *gmax, *vmax;     // f16: per 64 rows the largest row norm of dout / v
+  int B, H, Hkv, Lq, Lk, causal, Lqp;
+  float scale;
+};
+
+typedef __attribute__((address_space(3))) void* lds_ptr;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((address_space(3))) s16x4* lds_tr;
+
+// A tile is 64 rows of 128 bytes whose 16-byte chunks are permuted by the row: eight consecutive rows put one chunk into eight
+// different places (row reads, 16 bytes a lane) and four consecutive rows put a pair of chunks into disjoint places (transposing reads).
+__device__ __forceinline__ int swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+
+// workgroups are dealt to the 8 XCDs in turn: give each XCD a contiguous range of work so that a head's rows stay in one L2
+__device__ __forceinline__ int xcd_range(int w, int n) {
+  const int x = w & 7, i = w >> 3, per = n >> 3, rest = n & 7;
+  return x * per + (x < rest ? x : rest) + i;
+}
+
+// 64 rows [row0, row0 + 64) of a head into LDS, straight from memory; rows at or behind `n` arrive as zeros (the descriptor ends there)
+__device__ __forceinline__ void stage_tile(char* tile, const u16* base, long long ld, int row0, int n, int wave, int lane) {
+  const int left = n - row0, rows = left < 0 ? 0 : (left > TILE ? TILE : left);
+  const __amdgpu_buffer_rsrc_t srd = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<u16*>(base + (long long)row0 * ld), 0, rows ? (int)((rows - 1) * ld * 2 + HD * 2) : 0, 0x00020000);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int piece = wave + 4 * i, row = piece * 8 + (lane >> 3);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(srd, (lds_ptr)(tile + piece * 1024), 16,
+                                             (int)(row * ld * 2) + (((lane & 7) ^ swz(lane >> 3)) << 4), 0, 0, 0);
+  }
+}
+
+// operand whose rows (lane & 31) are rows row0 + .. of the tile and whose k is the head dimension, step ks
+template <typename T>
+__device__ __forceinline__ typename T::vec8 rows_frag(const char* tile, int row0, int ks, int lane) {
+  const int row = lane & 31, hi = lane >> 5;
+  return *reinterpret_cast<const typename T::vec8*>(tile + (row0 + row) * 128 + (((ks * 2 + hi) ^ swz(row)) << 4));
+}
+// operand whose rows (lane & 31) are head dimensions n0 + .. and whose k is 16 rows of the tile from k0 on, in the order of C's registers
+template <typename T>
+__device__ __forceinline__ typename T::vec8 cols_frag(const char* tile, int k0, int n0, int lane) {
+  const int hi = lane >> 5, g = (lane >> 4) & 1, i = lane & 15;
+  const int row = 4 * hi + (i >> 2), chunk = (n0 >> 3) + 2 * g + ((i & 3) >> 1);
+  const char* p = tile + (k0 + row) * 128 + ((chunk ^ swz(row)) << 4) + (i & 1) * 8;
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr)p), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr)(p + 8 * 128));
+  typedef __attribute__((ext_vector_type(8))) short s16x8;
+  const s16x8 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  return __builtin_bit_cast(typename T::vec8, v);
+}
+// one row's operand straight from memory (zeros where the row does not exist)
+template <typename T>
+__device__ __forceinline__ void load_rows(typename T::vec8* f, const u16* row, bool ok, int hi) {
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) {
+    const uint4 v = ok ? *reinterpret_cast<const uint4*>(row + ks * 16 + hi * 8) : make_uint4(0, 0, 0, 0);
+    f[ks] = __builtin_bit_cast(typename T::vec8, v);
+  }
+}
+template <typename T>
+__device__ __forceinline__ typename T::vec8 pack_frag(const f32x16& s, int half) {
+  float f[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = s[8 * half + j];
+  return __builtin_bit_cast(typename T::vec8, pack8<T>(f));
+}
+__device__ __forceinline__ f32x16 splat(float v) {
+  f32x16 r;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r[i] = v;
+  return r;
+}
+// lane's column of a transposed 64 x 32 result: 16 runs of four head dimensions, 8 bytes each
+template <typename T>
+__device__ __forceinline__ void store_cols(u16* row, const f32x16* acc, float mul, int hi) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      uint2 pk;
+      pk.x = T::pack2(acc[t][4 * g] * mul, acc[t][4 * g + 1] * mul);
+      pk.y = T::pack2(acc[t][4 * g + 2] * mul, acc[t][4 * g + 3] * mul);
+      *reinterpret_cast<uint2*>(row + t * 32 + 8 * g + 4 * hi) = pk;
+    }
+}
+__device__ __forceinline__ int row_of(int r, int hi) { return (r & 3) + 8 * (r >> 2) + 4 * hi; }
+__device__ __forceinline__ int clamp_len(const int* len, int b, int most) {
+  const int n = len ? len[b] : most;
+  return n < 0 ? 0 : (n > most ? most : n);
+}
+__device__ __forceinline__ void tile_ready() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------------------------------------------------------- forward
+// 128 queries a workgroup, 32 a wave; keys in tiles of 64, double buffered.
+template <typename T>
+__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Args a) {
+  __shared__ __attribute__((aligned(16))) char lds[4 * TILE_BYTES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
+  const int nqb = (a.Lq + 127) >> 7, w = xcd_range(blockIdx.x, gridDim.x);
+  const int bh = w / nqb, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
+  const int qb = a.causal ? nqb - 1 - w % nqb : w % nqb;   // (long rows first)
+  const int nk = clamp_len(a.kv_len, b, a.Lk), nq = clamp_len(a.q_len, b, a.Lq), off = a.Lk - a.Lq;
+  const int w0 = qb * 128 + wave * 32, row = w0 + (lane & 31);
+  const bool q_ok = row < nq;
+  int kend = qb * 128 < nq ? nk : 0;
+  if (a.causal) kend = min(kend, min(qb * 128 + 128, nq) + off);
+  const int full = a.causal ? min(nk, w0 + off + 1) : nk;                   // keys that every row of this wave sees
+  const int mine = a.causal ? min(nk, row + off + 1) : nk;                  // keys that this lane's row sees
+  const int wend = a.causal ? min(nk, w0 + 32 + off) : nk;                  // keys that some row of this wave sees
+  const u16* kp = a.k + b * a.ks[0] + hk * a.ks[2];
+  const u16* vp = a.v + b * a.vs[0] + hk * a.vs[2];
+  typename T::vec8 qf[4];
+  load_rows<T>(qf, a.q + b * a.qs[0] + (long long)(q_ok ? row : 0) * a.qs[1] + h * a.qs[2], q_ok, hi);
+  const float c = a.scale * LOG2E;
+  f32x16 acc[2] = {splat(0.f), splat(0.f)};
+  float m = -INFINITY, l = 0.f;   // running maximum (times c) and sum
+  const int nt = kend > 0 ? (kend + TILE - 1) / TILE : 0;
+  if (nt) {
+    stage_tile(lds, kp, a.ks[1], 0, nk, wave, lane);
+    stage_tile(lds + TILE_BYTES, vp, a.vs[1], 0, nk, wave, lane);
+  }
+  for (int t = 0; t < nt; ++t) {
+    const int key0 = t * TILE;
+    const char *kt = lds + (t & 1) * 2 * TILE_BYTES, *vt = kt + TILE_BYTES;
+    tile_ready();
+    if (t + 1 < nt) {
+      char* nxt = lds + ((t + 1) & 1) * 2 * TILE_BYTES;
+      stage_tile(nxt, kp, a.ks[1], key0 + TILE, nk, wave, lane);
+      stage_tile(nxt + TILE_BYTES, vp, a.vs[1], key0 + TILE, nk, wave, lane);
+    }
+    if (key0 >= wend) continue;
+    f32x16 s[2] = {splat(0.f), splat(0.f)};
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) s[kb] = T::mfma32(rows_frag<T>(kt, kb * 32, ks, lane), qf[ks], s[kb]);
+    if (key0 + TILE > full) {
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (key0 + kb * 32 + row_of(r, hi) >= mine) s[kb][r] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
+    const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(m - mu);
+    m = mn;
+    float sum = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], c, -mu));
+        sum += s[kb][r];
+      }
+    l = l * al + sum + __shfl_xor(sum, 32, 64);
+#pragma unroll
+    for (int d = 0; d < 2; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[d][r] *= al;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const typename T::vec8 pf = pack_frag<T>(s[kb], hf);
+#pragma unroll
+        for (int d = 0; d < 2; ++d) acc[d] = T::mfma32(cols_frag<T>(vt, kb * 32 + hf * 16, d * 32, lane), pf, acc[d]);
+      }
+  }
+  if (row < a.Lq) {
+    const bool some = q_ok && l != 0.f;   // (a NaN stays one)
+    store_cols<T>(a.o + b * a.os[0] + (long long)row * a.os[1] + h * a.os[2], acc, some ? 1.f / l : 0.f, hi);
+    if (hi == 0) a.lse[(long long)bh * a.Lq + row] = some ? (m + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- backward
+// D and the negated statistics of 64 rows, 8 lanes a row; f16 also the largest norms (scale_exp below).
+template <typename T>
+__global__ __launch_bounds__(256) void attn_bwd_rows_kernel(const Args a, int nqb, int f16) {
+  __shared__ float mx[4];
+  const int tid = threadIdx.x, bh = blockIdx.y, sub = tid & 7, blk = blockIdx.x;
+  float top = 0.f;
+  if (blk < nqb) {
+    const int b = bh / a.H, h = bh % a.H, nq = clamp_len(a.q_len, b, a.Lq);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = blk * 64 + i * 32 + (tid >> 3);
+      float d = 0.f, n = 0.f;
+      const float lse = row < nq ? a.lse[(long long)bh * a.Lq + row] : -INFINITY;
+      if (row < nq) {
+        float x[8], y[8];
+        unpack8<T>(*reinterpret_cast<const uint4*>(a.dout + b * a.gs[0] + (long long)row * a.gs[1] + h * a.gs[2] + sub * 8), x);
+        unpack8<T>(*reinterpret_cast<const uint4*>(a.o_in + b * a.os[0] + (long long)row * a.os[1] + h * a.os[2] + sub * 8), y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          d += x[e] * y[e];
+          n += x[e] * x[e];
+        }
+      }
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) {
+        d += __shfl_xor(d, o, 64);
+        n += __shfl_xor(n, o, 64);
+      }
+      top = fmaxf(top, n);
+      if (sub == 0) {
+        const bool some = lse != -INFINITY;   // an empty row has no probabilities
+        a.nl2[(long long)bh * a.Lqp + row] = some ? -lse * LOG2E : -INFINITY;
+        a.nd[(long long)bh * a.Lqp + row] = some ? -d : 0.f;
+      }
+    }
+  } else {
+    if (bh >= a.B * a.Hkv) return;
+    const int b = bh / a.Hkv, h = bh % a.Hkv, nk = clamp_len(a.kv_len, b, a.Lk);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int row = (blk - nqb) * 64 + i * 32 + (tid >> 3);
+      float n = 0.f;
+      if (row < nk) {
+        float x[8];
+        unpack8<T>(*reinterpret_cast<const uint4*>(a.v + b * a.vs[0] + (long long)row * a.vs[1] + h * a.vs[2] + sub * 8), x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) n += x[e] * x[e];
+      }
+#pragma unroll
+      for (int o = 4; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
+      top = fmaxf(top, n);
+    }
+  }
+  if (!f16) return;
+  top = wave_max(top);
+  if ((tid & 63) == 0) mx[tid >> 6] = top;
+  __syncthreads();
+  if (tid == 0) {
+    top = sqrtf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+    if (blk < nqb) a.gmax[(long long)bh * nqb + blk] = top;
+    else a.vmax[(long long)bh * (gridDim.x - nqb) + blk - nqb] = top;
+  }
+}
+
+// f16: p and ds are operands of 11 bits between 2^-14 and 65504, and ds may be far below (4096 keys, a gradient of 1e-3: 1e-6) or, with
+// a loss scale, above.  Both are formed times 2^e, which the result is divided by: |ds| <= 2 max|do| max|v| must stay under 2^15,
+// p under 2^14.  A power of two rounds nothing.  bf16 has the exponents of f32: e = 0.
+template <typename T>
+__device__ __forceinline__ float scale_exp(const Args& a, int b, int hk, int nqb, int nkb, int tid, float* red);
+template <>
+__device__ __forceinline__ float scale_exp<BF16>(const Args&, int, int, int, int, int, float*) { return 0.f; }
+template <>
+__device__ __forceinline__ float scale_exp<F16>(const Args& a, int b, int hk, int nqb, int nkb, int tid, float* red) {
+  const int grp = a.H / a.Hkv;
+  const float* g = a.gmax + (long long)(b * a.H + hk * grp) * nqb;   // the group's heads are adjacent
+  const float* v = a.vmax + (long long)(b * a.Hkv + hk) * nkb;
+  float x = 0.f, y = 0.f;
+  for (int i = tid; i < grp * nqb; i += 256) x = fmaxf(x, g[i]);
+  for (int i = tid; i < nkb; i += 256) y = fmaxf(y, v[i]);
+  x = wave_max(x);
+  y = wave_max(y);
+  if ((tid & 63) == 0) {
+    red[tid >> 6] = x;
+    red[4 + (tid >> 6)] = y;
+  }
+  __syncthreads();
+  x = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])) * fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
+  const int ex = (int)((__builtin_bit_cast(uint32_t, x) >> 23) & 255) - 126;   // x < 2^ex
+  const int e = 14 - ex;
+  return ex > 100 ? 0.f : (float)(e > 14 ? 14 : e);
+}
+
+// dk, dv: 128 keys a workgroup, 32 a wave (their k, v operands and sums stay in registers); queries in tiles of 64, double buffered,
+// over all heads that share these keys.
+template <typename T>
+__global__ __launch_bounds__(256, 2) void attn_bwd_kv_kernel(const Args a) {
+  __shared__ __attribute__((aligned(16))) char lds[2 * (2 * TILE_BYTES + 512)];
+  __shared__ float red[8];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
+  const int nkb = (a.Lk + 127) >> 7, w = xcd_range(blockIdx.x, gridDim.x);
+  const int bh = w / nkb, b = bh / a.Hkv, hk = bh % a.Hkv, grp = a.H / a.Hkv, k0 = (w % nkb) * 128;
+  const int nk = clamp_len(a.kv_len, b, a.Lk), nq = clamp_len(a.q_len, b, a.Lq), off = a.Lk - a.Lq;
+  const int key = k0 + wave * 32 + (lane & 31);
+  const bool k_ok = key < nk;
+  typename T::vec8 kf[4], vf[4];
+  load_rows<T>(kf, a.k + b * a.ks[0] + (long long)(k_ok ? key : 0) * a.ks[1] + hk * a.ks[2], k_ok, hi);
+  load_rows<T>(vf, a.v + b * a.vs[0] + (long long)(k_ok ? key : 0) * a.vs[1] + hk * a.vs[2], k_ok, hi);
+  const float c = a.scale * LOG2E, e = scale_exp<T>(a, b, hk, a.Lqp / 64, (a.Lk + 63) >> 6, tid, red);
+  const int qt0 = a.causal ? max(0, k0 - off) / TILE : 0, qt1 = k0 < nk ? (nq + TILE - 1) / TILE : 0, nt = max(0, qt1 - qt0);
+  f32x16 dk[2] = {splat(0.f), splat(0.f)}, dv[2] = {splat(0.f), splat(0.f)};
+  auto stage = [&](int it) {
+    const int h = hk * grp + it / nt, q0 = (qt0 + it % nt) * TILE;
+    char* p = lds + (it & 1) * (2 * TILE_BYTES + 512);
+    stage_tile(p, a.q + b * a.qs[0] + h * a.qs[2], a.qs[1], q0, nq, wave, lane);
+    stage_tile(p + TILE_BYTES, a.dout + b * a.gs[0] + h * a.gs[2], a.gs[1], q0, nq, wave, lane);
+    if (wave < 2) {
+      const float* st = (wave ? a.nd : a.nl2) + (long long)(b * a.H + h) * a.Lqp + q0;
+      const __amdgpu_buffer_rsrc_t srd = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(st), 0, 256, 0x00020000);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(srd, (lds_ptr)(p + 2 * TILE_BYTES + wave * 256), 4, lane * 4, 0, 0, 0);
+    }
+  };
+  if (nt) stage(0);
+  for (int it = 0; it < nt * grp; ++it) {
+    const char *qt = lds + (it & 1) * (2 * TILE_BYTES + 512), *gt = qt + TILE_BYTES;
+    const float* st = reinterpret_cast<const float*>(gt + TILE_BYTES);
+    tile_ready();
+    if (it + 1 < nt * grp) stage(it + 1);
+    const int q0 = (qt0 + it % nt) * TILE;
+#pragma unroll
+    for (int sb = 0; sb < 2; ++sb) {
+      if (a.causal && q0 + sb * 32 + 31 + off < k0 + wave * 32) continue;   // no row of these sees a key of this wave
+      f32x16 s = splat(e / c), dp;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(st + 64 + sb * 32 + 8 * g + 4 * hi);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) dp[4 * g + r] = v[r];
+      }
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        s = T::mfma32(rows_frag<T>(qt, sb * 32, ks, lane), kf[ks], s);
+        dp = T::mfma32(rows_frag<T>(gt, sb * 32, ks, lane), vf[ks], dp);
+      }
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 v = *reinterpret_cast<const f32x4*>(st + sb * 32 + 8 * g + 4 * hi);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[4 * g + r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + r], c, v[r]));
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) dp[r] *= s[r];
+      if (a.causal && q0 + sb * 32 + off < k0 + wave * 32 + 31) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (q0 + sb * 32 + row_of(r, hi) + off < key) s[r] = dp[r] = 0.f;
+      }
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const typename T::vec8 pf = pack_frag<T>(s, hf), df = pack_frag<T>(dp, hf);
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+          dv[d] = T::mfma32(cols_frag<T>(gt, sb * 32 + hf * 16, d * 32, lane), pf, dv[d]);
+          dk[d] = T::mfma32(cols_frag<T>(qt, sb * 32 + hf * 16, d * 32, lane), df, dk[d]);
+        }
+      }
+    }
+  }
+  if (key < a.Lk) {
+    const float un = k_ok ? __builtin_amdgcn_exp2f(-e) : 0.f;
+    if (!k_ok)
+      for (int d = 0; d < 2; ++d) dk[d] = dv[d] = splat(0.f);   // (whatever the sums of a key that nobody sees are)
+    store_cols<T>(a.dk + b * a.dks[0] + (long long)key * a.dks[1] + hk * a.dks[2], dk, un * a.scale, hi);
+    store_cols<T>(a.dv + b * a.dvs[0] + (long long)key * a.dvs[1] + hk * a.dvs[2], dv, un, hi);
+  }
+}
+
+// dq: 128 queries a workgroup, 32 a wave; keys in tiles of 64, double buffered.  D = do . o comes from the ROUNDED o, and where one key has
+// most of a row, dp - D is far below D.  The exact D makes sum_j ds_ij zero, so the sum of the ds that are formed with the rounded one is its error:
+// it corrects D for the dk kernel, and rows of up to two tiles (few keys: where it matters most) are gone through once more with the corrected one.
+template <typename T>
+__global__ __launch_bounds__(256, 2) void attn_bwd_q_kernel(const Args a) {
+  __shared__ __attribute__((aligned(16))) char lds[4 * TILE_BYTES];
+  __shared__ float red[8];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
+  const int nqb = (a.Lq + 127) >> 7, w = xcd_range(blockIdx.x, gridDim.x);
+  const int bh = w / nqb, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
+  const int qb = a.causal ? nqb - 1 - w % nqb : w % nqb;
+  const int nk = clamp_len(a.kv_len, b, a.Lk), nq = clamp_len(a.q_len, b, a.Lq), off = a.Lk - a.Lq;
+  const int w0 = qb * 128 + wave * 32, row = w0 + (lane & 31);
+  const bool q_ok = row < nq;
+  int kend = qb * 128 < nq ? nk : 0;
+  if (a.causal) kend = min(kend, min(qb * 128 + 128, nq) + off);
+  const int full = a.causal ? min(nk, w0 + off + 1) : nk, mine = a.causal ? min(nk, row + off + 1) : nk;
+  const int wend = a.causal ? min(nk, w0 + 32 + off) : nk;
+  const u16* kp = a.k + b * a.ks[0] + hk * a.ks[2];
+  const u16* vp = a.v + b * a.vs[0] + hk * a.vs[2];
+  typename T::vec8 qf[4], gf[4];
+  load_rows<T>(qf, a.q + b * a.qs[0] + (long long)(q_ok ? row : 0) * a.qs[1] + h * a.qs[2], q_ok, hi);
+  load_rows<T>(gf, a.dout + b * a.gs[0] + (long long)(q_ok ? row : 0) * a.gs[1] + h * a.gs[2], q_ok, hi);
+  const float c = a.scale * LOG2E, e = scale_exp<T>(a, b, hk, a.Lqp / 64, (a.Lk + 63) >> 6, tid, red), un = __builtin_amdgcn_exp2f(-e);
+  const float nl2 = q_ok ? a.nl2[(long long)bh * a.Lqp + row] + e : -INFINITY;
+  float nd = q_ok ? a.nd[(long long)bh * a.Lqp + row] : 0.f, sum = 0.f;
+  f32x16 acc[2] = {splat(0.f), splat(0.f)};
+  const int nt = kend > 0 ? (kend + TILE - 1) / TILE : 0;
+  auto stage = [&](int t) {
+    char* p = lds + (t & 1) * 2 * TILE_BYTES;
+    stage_tile(p, kp, a.ks[1], t * TILE, nk, wave, lane);
+    stage_tile(p + TILE_BYTES, vp, a.vs[1], t * TILE, nk, wave, lane);
+  };
+  auto ds_of = [&](const char* kt, int key0, int kb) {   // 2^e ds of 32 keys (rows) and the wave's 32 queries
+    f32x16 s = splat(0.f), dp = splat(nd);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      s = T::mfma32(rows_frag<T>(kt, kb * 32, ks, lane), qf[ks], s);
+      dp = T::mfma32(rows_frag<T>(kt + TILE_BYTES, kb * 32, ks, lane), gf[ks], dp);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dp[r] *= __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, nl2));
+    if (key0 + kb * 32 + 32 > full) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (key0 + kb * 32 + row_of(r, hi) >= mine) dp[r] = 0.f;
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum += dp[r];
+    return dp;
+  };
+  if (nt) stage(0);
+  const bool few = nt <= 2;
+  if (few) {
+    if (nt == 2) stage(1);
+    tile_ready();
+    for (int t = 0; t < nt; ++t)
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+        if (t * TILE + kb * 32 < wend) ds_of(lds + t * 2 * TILE_BYTES, t * TILE, kb);
+    nd -= (sum + __shfl_xor(sum, 32, 64)) * un;
+  }
+  for (int t = 0; t < nt; ++t) {
+    const int key0 = t * TILE;
+    const char* kt = lds + (t & 1) * 2 * TILE_BYTES;
+    if (!few) {
+      tile_ready();
+      if (t + 1 < nt) stage(t + 1);
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      if (key0 + kb * 32 >= wend) continue;
+      const f32x16 ds = ds_of(kt, key0, kb);
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const typename T::vec8 df = pack_frag<T>(ds, hf);
+#pragma unroll
+        for (int d = 0; d < 2; ++d) acc[d] = T::mfma32(cols_frag<T>(kt, kb * 32 + hf * 16, d * 32, lane), df, acc[d]);
+      }
+    }
+  }
+  if (!few) nd -= (sum + __shfl_xor(sum, 32, 64)) * un;
+  if (q_ok && hi == 0) a.nd[(long long)bh * a.Lqp + row] = nd;
+  if (row < a.Lq) {
+    if (!q_ok) acc[0] = acc[1] = splat(0.f);
+    store_cols<T>(a.dq + b * a.dqs[0] + (long long)row * a.dqs[1] + h * a.dqs[2], acc, q_ok ? un * a.scale : 0.f, hi);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- host
+bool good_layout(const void* p, const long long* s, int rows) {   // batch, row, head strides
+  return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s[0] >= 0 && s[1] >= 0 && s[2] >= 0 && s[0] % 8 == 0 && s[1] % 8 == 0 &&
+         s[2] % 8 == 0 && (rows == 1 || s[1] >= HD) && s[1] < (1 << 23);
+}
+#define CHECK_LAYOUT(P, S, ROWS)                                                                                              \
+  DBIR_CHECK_ARG(good_layout(d->P, d->S, ROWS),                                                                               \
+                 "%s: " #P " must be 16-byte aligned with strides that are multiples of 8 elements, rows at least 64 apart and " \
+                 "less than 2^23", name)
+
+int check_desc(const dbir_attn_desc* d, const char* name) {
+  DBIR_CHECK_ARG(d, "%s: null descriptor", name);
+  DBIR_CHECK_ARG(d->dtype == DBIR_F16 || d->dtype == DBIR_BF16, "%s: bad dtype %d", name, d->dtype);
+  DBIR_CHECK_ARG(d->B > 0 && d->H > 0 && d->Hkv > 0 && d->Lq > 0 && d->Lk > 0 && d->H % d->Hkv == 0,
+                 "%s: bad sizes B %d H %d Hkv %d Lq %d Lk %d", name, d->B, d->H, d->Hkv, d->Lq, d->Lk);
+  DBIR_CHECK_ARG(d->Lq <= (1 << 30) && d->Lk <= (1 << 30), "%s: more than 2^30 rows", name);
+  DBIR_CHECK_ARG((long long)d->B * d->H <= 65535 && (long long)cdiv(d->Lq, 128) * d->B * d->H < 2147483647LL &&
+                     (long long)cdiv(d->Lk, 128) * d->B * d->Hkv < 2147483647LL, "%s: grid too large", name);
+  DBIR_CHECK_ARG(d->scale > 0.f && d->scale < INFINITY, "%s: scale must be positive and finite", name);
+  DBIR_CHECK_ARG(d->lse, "%s: null lse", name);
+  CHECK_LAYOUT(q, q_stride, d->Lq);
+  CHECK_LAYOUT(k, k_stride, d->Lk);
+  CHECK_LAYOUT(v, v_stride, d->Lk);
+  CHECK_LAYOUT(out, out_stride, d->Lq);
+  return DBIR_OK;
+}
+
+Args to_args(const dbir_attn_desc* d) {
+  Args a;
+  memset(&a, 0, sizeof(a));
+  a.q = (const u16*)d->q; a.k = (const u16*)d->k; a.v = (const u16*)d->v; a.o = (u16*)d->out; a.o_in = (const u16*)d->out;
+  a.dout = (const u16*)d->dout; a.dq = (u16*)d->dq; a.dk = (u16*)d->dk; a.dv = (u16*)d->dv;
+  const long long* from[8] = {d->q_stride, d->k_stride, d->v_stride, d->out_stride, d->dout_stride, d->dq_stride, d->dk_stride, d->dv_stride};
+  long long* to[8] = {a.qs, a.ks, a.vs, a.os, a.gs, a.dqs, a.dks, a.dvs};
+  for (int i = 0; i < 8; ++i)
+    for (int j = 0; j < 3; ++j) to[i][j] = from[i][j];
+  a.lse = d->lse; a.q_len = d->q_len; a.kv_len = d->kv_len;
+  a.B = d->B; a.H = d->H; a.Hkv = d->Hkv; a.Lq = d->Lq; a.Lk = d->Lk; a.causal = d->causal; a.scale = d->scale;
+  a.Lqp = (d->Lq + 63) / 64 * 64;
+  return a;
+}
+
+// floats of the backward pass's workspace: nl2 | nd | gmax | vmax
+long long bwd_ws_floats(const dbir_attn_desc* d) {
+  const long long lqp = ((long long)d->Lq + 63) / 64 * 64, bh = (long long)d->B * d->H;
+  return bh * lqp * 2 + (d->dtype == DBIR_F16 ? bh * (lqp / 64) + (long long)d->B * d->Hkv * ((d->Lk + 63) / 64) : 0);
+}
+
+}  // namespace
+
+extern "C" int dbir_attention_fwd_ws(const dbir_attn_desc* d, long long* bytes) {
+  DBIR_CHECK_ARG(d && bytes, "dbir_attention_fwd_ws: bad arguments");
+  *bytes = 0;
+  return DBIR_OK;
+}
+
+extern "C" int dbir_attention_bwd_ws(const dbir_attn_desc* d, long long* bytes) {
+  DBIR_CHECK_ARG(d && bytes && d->B > 0 && d->H > 0 && d->Hkv > 0 && d->Lq > 0 && d->Lk > 0, "dbir_attention_bwd_ws: bad arguments");
+  *bytes = bwd_ws_floats(d) * 4;
+  return DBIR_OK;
+}
+
+extern "C" int dbir_attention_fwd(const dbir_attn_desc* d, void* stream) {
+  if (int rc = check_desc(d, "dbir_attention_fwd")) return rc;
+  const Args a = to_args(d);
+  const dim3 grid((unsigned)(cdiv(d->Lq, 128) * d->B * d->H));
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (d->dtype == DBIR_F16) hipLaunchKernelGGL(attn_fwd_kernel<F16>, grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(attn_fwd_kernel<BF16>, grid, dim3(256), 0, s, a);
+  DBIR_CHECK_LAUNCH("dbir_attention_fwd");
+  return DBIR_OK;
+}
+
+extern "C" int dbir_attention_bwd(const dbir_attn_desc* d, void* stream) {
+  const char* name = "dbir_attention_bwd";
+  if (int rc = check_desc(d, name)) return rc;
+  CHECK_LAYOUT(dout, dout_stride, d->Lq);
+  CHECK_LAYOUT(dq, dq_stride, d->Lq);
+  CHECK_LAYOUT(dk, dk_stride, d->Lk);
+  CHECK_LAYOUT(dv, dv_stride, d->Lk);
+  DBIR_CHECK_ARG(d->ws && d->ws_bytes >= bwd_ws_floats(d) * 4 && (reinterpret_cast<uintptr_t>(d->ws) & 15) == 0,
+                 "%s: the workspace must hold %lld bytes, 16-byte aligned", name, bwd_ws_floats(d) * 4);
+  Args a = to_args(d);
+  const long long bh = (long long)d->B * d->H;
+  const int f16 = d->dtype == DBIR_F16, nqb = a.Lqp / 64, nkb = cdiv(d->Lk, 64);
+  a.nl2 = reinterpret_cast<float*>(d->ws);
+  a.nd = a.nl2 + bh * a.Lqp;
+  a.gmax = a.nd + bh * a.Lqp;
+  a.vmax = a.gmax + bh * nqb;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const dim3 g0((unsigned)(nqb + (f16 ? nkb : 0)), (unsigned)bh), g1((unsigned)(cdiv(d->Lk, 128) * d->B * d->Hkv)),
+      g2((unsigned)(cdiv(d->Lq, 128) * d->B * d->H));
+  if (f16) {
+    hipLaunchKernelGGL(attn_bwd_rows_kernel<F16>, g0, dim3(256), 0, s, a, nqb, 1);
+    hipLaunchKernelGGL(attn_bwd_q_kernel<F16>, g2, dim3(256), 0, s, a);
+    hipLaunchKernelGGL(attn_bwd_kv_kernel<F16>, g1, dim3(256), 0, s, a);
+  } else {
+    hipLaunchKernelGGL(attn_bwd_rows_kernel<BF16>, g0, dim3(256), 0, s, a, nqb, 0);
+    hipLaunchKernelGGL(attn_bwd_q_kernel<BF16>, g2, dim3(256), 0, s, a);
+    hipLaunchKernelGGL(attn_bwd_kv_kernel<BF16>, g1, dim3(256), 0, s, a);
+  }
+  DBIR_CHECK_LAUNCH(name);
+  return DBIR_OK;
+}

@@ -6,7 +6,7 @@ HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
 # no packed f32 instructions: some of their forms have given wrong results on these devices now and then, without an error
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops"
 if [ -n "$DBIR_DIAG" ]; then FLAGS="$FLAGS -DDBIR_DIAG"; fi
-SRCS="api gemm gemm_glds gemm_halo gemm_pers gemm_8p gemm_rs attention norm elementwise swin clip xformer xformer2 plan"
+SRCS="api gemm gemm_glds gemm_halo gemm_pers gemm_8p gemm_rs attention norm elementwise swin clip xformer xformer2 plan attention_train norm_train embedding"
 mkdir -p build
 # objects built with a different flag set (e.g. a DBIR_DIAG build) must not be linked into this one
 if [ "$(cat build/.flags 2>/dev/null)" != "$FLAGS" ]; then rm -f build/*.o; echo "$FLAGS" > build/.flags; fi

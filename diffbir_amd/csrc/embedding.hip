@@ -1,0 +1,386 @@
+// Token embedding for training (include/dbir.h, dbir_embedding_fwd / _bwd): x[i] = scale table[t_i] + pos[i mod L] and its gradient
+//   dtable[v] = scale sum_{i: t_i = v} dy[i]      dpos[l] = sum_b dy[b L + l]
+// in f32, without atomics on floating values: the positions are sorted by token (stable, so every sum has one order), each table row
+// then sums its own run of positions.  A run may be most of the batch (the padding token): whole pieces of RUN sorted positions that
+// lie in one run are summed by workgroups of their own first.  Rows of the table that no token names are written as zeros in the same
+// pass, so the gradient is written once and needs no clearing.  Bytes bound all of it: dy once, the rows of dtable once.
+#include "common.h"
+
+namespace {
+
+struct F32T {
+  typedef float elem;
+  static __device__ __forceinline__ float load(const float* p) { return *p; }
+  static __device__ __forceinline__ void load4(const float* p, float* f) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
+  }
+  static __device__ __forceinline__ void store(float* p, float v) { *p = v; }
+  static __device__ __forceinline__ void store4(float* p, const float* f) { *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]); }
+};
+template <typename T>
+struct H16T {
+  typedef u16 elem;
+  static __device__ __forceinline__ float load(const u16* p) { return T::to_f32(*p); }
+  static __device__ __forceinline__ void load4(const u16* p, float* f) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    f[0] = T::to_f32((u16)v.x); f[1] = T::to_f32((u16)(v.x >> 16)); f[2] = T::to_f32((u16)v.y); f[3] = T::to_f32((u16)(v.y >> 16));
+  }
+  static __device__ __forceinline__ void store(u16* p, float v) { *p = T::from_f32(v); }
+  static __device__ __forceinline__ void store4(u16* p, const float* f) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(T::pack2(f[0], f[1]), T::pack2(f[2], f[3]));
+  }
+};
+typedef H16T<F16> F16T;
+typedef H16T<BF16> BF16T;
+
+constexpr int RUN = 64;          // sorted positions of a piece that is summed ahead
+constexpr int RANK_MAX = 4096;   // up to here the sort is one launch that counts for every token how many go before it
+
+__device__ __forceinline__ uint32_t clamp_token(long long t, int vocab) { return (uint32_t)(t < 0 ? 0 : (t >= vocab ? vocab - 1 : t)); }
+
+// ------------------------------------------------------------------------------------------------------------- forward
+// lpr lanes (a power of two) a row, V elements a lane and step
+template <typename TT, typename TO, int V>
+__global__ __launch_bounds__(256) void embed_fwd_kernel(const typename TT::elem* __restrict__ table, long long ldt, const long long* __restrict__ tokens,
+                                                        const float* __restrict__ pos, long long ldp, typename TO::elem* __restrict__ out, long long ldo,
+                                                        float scale, int n, int L, int W, int vocab, int lpr_log) {
+  const long long id = (long long)blockIdx.x * 256 + threadIdx.x, row = id >> lpr_log;
+  if (row >= n) return;
+  const int lpr = 1 << lpr_log;
+  const typename TT::elem* t = table + (long long)clamp_token(tokens[row], vocab) * ldt;
+  const float* p = pos ? pos + (row % L) * ldp : nullptr;
+  for (int c = ((int)id & (lpr - 1)) * V; c < W; c += lpr * V) {
+    if constexpr (V == 4) {
+      float f[4], q[4] = {0.f, 0.f, 0.f, 0.f};
+      TT::load4(t + c, f);
+      if (p) F32T::load4(p + c, q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[e] = __builtin_fmaf(f[e], scale, q[e]);
+      TO::store4(out + row * ldo + c, f);
+    } else {
+      TO::store(out + row * ldo + c, __builtin_fmaf(TT::load(t + c), scale, p ? p[c] : 0.f));
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------- sort
+// rank of each token among all: 64 tokens a workgroup, each wave compares them with a quarter of the tokens
+__global__ __launch_bounds__(256) void embed_rank_kernel(const long long* __restrict__ tokens, int n, int vocab, uint32_t* __restrict__ skey,
+                                                         int* __restrict__ spos) {
+  __shared__ __attribute__((aligned(16))) uint32_t keys[1024];
+  __shared__ int part[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.x * 64 + lane;
+  const uint32_t mine = i < n ? clamp_token(tokens[i], vocab) : 0;
+  int before = 0;
+  for (int base = 0; base < n; base += 1024) {
+    __syncthreads();
+    for (int j = threadIdx.x; j < 1024; j += 256) keys[j] = base + j < n ? clamp_token(tokens[base + j], vocab) : 0xffffffffu;
+    __syncthreads();
+    for (int j = wave * 256; j < wave * 256 + 256; j += 4) {
+      const uint4 k = *reinterpret_cast<const uint4*>(&keys[j]);
+      const int at = base + j;
+      before += (k.x < mine || (k.x == mine && at < i)) + (k.y < mine || (k.y == mine && at + 1 < i)) +
+                (k.z < mine || (k.z == mine && at + 2 < i)) + (k.w < mine || (k.w == mine && at + 3 < i));
+    }
+  }
+  part[wave][lane] = before;
+  __syncthreads();
+  if (wave == 0 && i < n) {
+    const int r = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+    skey[r] = mine;
+    spos[r] = i;
+  }
+}
+
+// One pass of a stable radix sort over 8 bits: a wave counts / places one segment of `seg` items (a multiple of 64), at most 256 segments.
+__global__ __launch_bounds__(256) void embed_count_kernel(const long long* __restrict__ tokens, const uint32_t* __restrict__ key, int n, int vocab,
+                                                          int shift, int seg, int nseg, int* __restrict__ hist) {
+  __shared__ int cnt[4][256];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sg = blockIdx.x * 4 + wave;
+  for (int d = threadIdx.x; d < 1024; d += 256) cnt[d >> 8][d & 255] = 0;
+  __syncthreads();
+  const long long e = min((long long)n, (long long)(sg + 1) * seg);
+  for (long long i = (long long)sg * seg + lane; i < e; i += 64) {
+    const uint32_t k = tokens ? clamp_token(tokens[i], vocab) : key[i];
+    atomicAdd(&cnt[wave][(k >> shift) & 255], 1);
+  }
+  __syncthreads();
+  if (sg < nseg)
+    for (int d = lane; d < 256; d += 64) hist[sg * 256 + d] = cnt[wave][d];
+}
+
+__global__ __launch_bounds__(256) void embed_place_kernel(const long long* __restrict__ tokens, const uint32_t* __restrict__ key, const int* __restrict__ pos,
+                                                          int n, int vocab, int shift, int seg, int nseg, const int* __restrict__ hist,
+                                                          uint32_t* __restrict__ okey, int* __restrict__ opos) {
+  __shared__ int at[4][256], tot[256];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, sg = blockIdx.x * 4 + wave;
+  int run = 0;
+  for (int s = 0; s < nseg; ++s) {
+    if ((s >> 2) == (int)blockIdx.x) at[s & 3][tid] = run;   // this digit's items in the segments before s
+    run += hist[s * 256 + tid];
+  }
+  tot[tid] = run;
+  __syncthreads();
+  for (int o = 1; o < 256; o <<= 1) {   // inclusive sums over the digits
+    const int v = tid >= o ? tot[tid - o] : 0;
+    __syncthreads();
+    tot[tid] += v;
+    __syncthreads();
+  }
+  const int less = tot[tid] - run;
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+    if (blockIdx.x * 4 + s < nseg) at[s][tid] += less;
+  __syncthreads();
+  volatile int* mine = at[wave];
+  const long long e = min((long long)n, (long long)(sg + 1) * seg);
+  for (long long i0 = (long long)sg * seg; i0 < e; i0 += 64) {
+    const long long i = i0 + lane;
+    const bool ok = i < e;
+    const uint32_t k = ok ? (tokens ? clamp_token(tokens[i], vocab) : key[i]) : 0;
+    const int d = (k >> shift) & 255;
+    unsigned long long same = __ballot(ok);
+#pragma unroll
+    for (int bit = 0; bit < 8; ++bit) {
+      const unsigned long long m = __ballot((d >> bit) & 1);
+      same &= ((d >> bit) & 1) ? m : ~m;
+    }
+    if (ok) {
+      const int r = __popcll(same & ((1ull << lane) - 1)), to = mine[d] + r;
+      __builtin_amdgcn_wave_barrier();
+      if (r == 0) mine[d] = to + __popcll(same);   // the first of a digit moves it on for the next 64
+      __builtin_amdgcn_wave_barrier();
+      okey[to] = k;
+      opos[to] = tokens ? (int)i : pos[i];
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------- sums
+// A lane's four columns of a block of 256: adjacent where rows are aligned for it, else 64 apart.
+template <int V>
+__device__ __forceinline__ int col_of(int c0, int lane, int k) { return V == 4 ? c0 + lane * 4 + k : c0 + lane + 64 * k; }
+template <typename T, int V>
+__device__ __forceinline__ void add_row(const typename T::elem* row, int c0, int lane, int W, float* acc) {
+  float f[4];
+  if constexpr (V == 4) {
+    T::load4(row + c0 + lane * 4, f);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[k] = c0 + lane + 64 * k < W ? T::load(row + c0 + lane + 64 * k) : 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) acc[k] += f[k];
+}
+template <typename T, int V>
+__device__ __forceinline__ void add_items(const typename T::elem* dy, long long ldg, const int* spos, int s, int e, int c0, int lane, int W, float* acc) {
+#pragma unroll 8
+  for (int i = s; i < e; ++i) add_row<T, V>(dy + (long long)spos[i] * ldg, c0, lane, W, acc);
+}
+
+// the sum of sorted positions [piece * RUN, + RUN) where they are one run: a wave a block of 256 columns
+template <typename T, int V>
+__global__ __launch_bounds__(256) void embed_piece_kernel(const typename T::elem* __restrict__ dy, long long ldg, const uint32_t* __restrict__ skey,
+                                                          const int* __restrict__ spos, float* __restrict__ part, int W, int Wp) {
+  const int piece = blockIdx.x, lane = threadIdx.x & 63, c0 = (blockIdx.y * 4 + (threadIdx.x >> 6)) * 256;
+  if (c0 >= W || skey[(long long)piece * RUN] != skey[(long long)piece * RUN + RUN - 1]) return;
+  if (V == 4 && c0 + lane * 4 >= W) return;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  add_items<T, V>(dy, ldg, spos, piece * RUN, piece * RUN + RUN, c0, lane, W, acc);
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (col_of<V>(c0, lane, k) < W) part[(long long)piece * Wp + col_of<V>(c0, lane, k)] = acc[k];
+}
+
+// 32 rows of the table a workgroup, 8 a wave, one block of 256 columns
+template <typename T, int V>
+__global__ __launch_bounds__(256) void embed_rows_kernel(const typename T::elem* __restrict__ dy, long long ldg, const uint32_t* __restrict__ skey,
+                                                         const int* __restrict__ spos, const float* __restrict__ part, float* __restrict__ dtable,
+                                                         long long ldd, float scale, int n, int W, int Wp, int vocab, int padding, int accumulate) {
+  __shared__ int first[33];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c0 = blockIdx.y * 256, v0 = blockIdx.x * 32;
+  if (threadIdx.x < 33) {   // the first sorted position whose token is at least v
+    const uint32_t v = (uint32_t)(v0 + threadIdx.x);
+    int lo = 0, hi = n;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (skey[mid] < v) lo = mid + 1;
+      else hi = mid;
+    }
+    first[threadIdx.x] = lo;
+  }
+  __syncthreads();
+  if (V == 4 && c0 + lane * 4 >= W) return;
+  for (int r = wave * 8; r < wave * 8 + 8; ++r) {
+    const int v = v0 + r;
+    if (v >= vocab) return;
+    const int s = __builtin_amdgcn_readfirstlane(first[r]), e = __builtin_amdgcn_readfirstlane(first[r + 1]);
+    const bool none = s == e || v == padding;
+    if (none && accumulate) continue;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    if (!none) {
+      const int ps = (s + RUN - 1) / RUN, pe = e / RUN;
+      if (ps < pe) {
+        add_items<T, V>(dy, ldg, spos, s, ps * RUN, c0, lane, W, acc);
+#pragma unroll 8
+        for (int p = ps; p < pe; ++p) add_row<F32T, V>(part + (long long)p * Wp, c0, lane, W, acc);
+        add_items<T, V>(dy, ldg, spos, pe * RUN, e, c0, lane, W, acc);
+      } else {
+        add_items<T, V>(dy, ldg, spos, s, e, c0, lane, W, acc);
+      }
+    }
+    float* d = dtable + (long long)v * ldd;
+    if constexpr (V == 4) {
+      float f[4] = {0.f, 0.f, 0.f, 0.f};
+      if (accumulate) F32T::load4(d + c0 + lane * 4, f);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f[k] = __builtin_fmaf(acc[k], scale, f[k]);
+      F32T::store4(d + c0 + lane * 4, f);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (col_of<V>(c0, lane, k) < W) {
+          float* p = d + col_of<V>(c0, lane, k);
+          *p = __builtin_fmaf(acc[k], scale, accumulate ? *p : 0.f);
+        }
+    }
+  }
+}
+
+// dpos[l]: a workgroup a row and block of 256 columns, its waves a quarter of the batch each
+template <typename T, int V>
+__global__ __launch_bounds__(256) void embed_pos_kernel(const typename T::elem* __restrict__ dy, long long ldg, float* __restrict__ dpos, int B, int L, int W) {
+  __shared__ float red[4][256];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c0 = blockIdx.x * 256, l = blockIdx.y;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  if (l < L && !(V == 4 && c0 + lane * 4 >= W)) {
+#pragma unroll 8
+    for (int b = wave; b < B; b += 4) add_row<T, V>(dy + ((long long)b * L + l) * ldg, c0, lane, W, acc);
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) red[wave][V == 4 ? lane * 4 + k : lane + 64 * k] = acc[k];
+  __syncthreads();
+  const int c = threadIdx.x;
+  if (c0 + c < W) dpos[(long long)l * W + c0 + c] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+}
+
+// ------------------------------------------------------------------------------------------------------------- host
+struct Plan {
+  int seg, nseg, passes, pieces, Wp;
+  long long hist, part, total;   // offsets in 4-byte words behind the four arrays of n, and all of them
+};
+Plan plan_of(int n, int W, int vocab) {
+  Plan p;
+  p.seg = ((cdiv(n, 256) + 63) / 64) * 64;
+  if (p.seg < 256) p.seg = 256;
+  p.nseg = cdiv(n, p.seg);
+  p.passes = 1;
+  while (p.passes < 4 && ((long long)(vocab - 1) >> (8 * p.passes)) > 0) ++p.passes;
+  p.pieces = n / RUN;
+  p.Wp = (W + 3) / 4 * 4;
+  const long long np = ((long long)n + 3) / 4 * 4;
+  p.hist = (n > RANK_MAX ? 4 : 2) * np;
+  p.part = p.hist + (n > RANK_MAX ? 256LL * p.nseg : 0);
+  p.total = p.part + (long long)p.pieces * p.Wp;
+  return p;
+}
+bool al(const void* p, long long ld, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0 && (ld * (bytes / 4)) % bytes == 0; }
+int elem4(int dtype) { return dtype == DBIR_F32 ? 16 : 8; }   // bytes of four elements
+
+}  // namespace
+
+extern "C" int dbir_embedding_fwd(int table_dtype, const void* table, long long ldt, const long long* tokens, const float* pos, long long ldp,
+                                  int out_dtype, void* out, long long ldo, float scale, int n, int L, int W, int vocab, void* stream) {
+  DBIR_CHECK_ARG(table && tokens && out, "dbir_embedding_fwd: null pointer");
+  DBIR_CHECK_ARG(n > 0 && n < (1 << 30) && L > 0 && W > 0 && vocab > 0 && ldt >= W && ldo >= W && (!pos || ldp >= W), "dbir_embedding_fwd: bad shape");
+  DBIR_CHECK_ARG(table_dtype >= 0 && table_dtype <= 2 && out_dtype >= 0 && out_dtype <= 2, "dbir_embedding_fwd: bad dtype");
+  const bool v4 = W % 4 == 0 && al(table, ldt, elem4(table_dtype)) && al(out, ldo, elem4(out_dtype)) && (!pos || al(pos, ldp, 16));
+  const int nv = v4 ? W / 4 : W;
+  int lg = 0;
+  while (lg < 6 && (1 << lg) < nv) ++lg;
+  const dim3 grid((unsigned)(((((long long)n) << lg) + 255) / 256));
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+#define GO2(TT, TO, V)                                                                                                                        \
+  hipLaunchKernelGGL((embed_fwd_kernel<TT, TO, V>), grid, dim3(256), 0, s, (const TT::elem*)table, ldt, tokens, pos, ldp, (TO::elem*)out, ldo, \
+                     scale, n, L, W, vocab, lg)
+#define GO(TT, TO)          \
+  do {                      \
+    if (v4) GO2(TT, TO, 4); \
+    else GO2(TT, TO, 1);    \
+  } while (0)
+  switch (table_dtype * 3 + out_dtype) {
+    case 0: GO(F16T, F16T); break;
+    case 1: GO(F16T, BF16T); break;
+    case 2: GO(F16T, F32T); break;
+    case 3: GO(BF16T, F16T); break;
+    case 4: GO(BF16T, BF16T); break;
+    case 5: GO(BF16T, F32T); break;
+    case 6: GO(F32T, F16T); break;
+    case 7: GO(F32T, BF16T); break;
+    case 8: GO(F32T, F32T); break;
+  }
+#undef GO
+#undef GO2
+  DBIR_CHECK_LAUNCH("dbir_embedding_fwd");
+  return DBIR_OK;
+}
+
+extern "C" int dbir_embedding_bwd_ws(int n, int W, int vocab, long long* bytes) {
+  DBIR_CHECK_ARG(n > 0 && n < (1 << 30) && W > 0 && vocab > 0 && bytes, "dbir_embedding_bwd_ws: bad arguments");
+  *bytes = plan_of(n, W, vocab).total * 4;
+  return DBIR_OK;
+}
+
+extern "C" int dbir_embedding_bwd(int dtype, const void* dy, long long ldg, const long long* tokens, float* dtable, long long ldd, float* dpos,
+                                  float scale, int n, int L, int W, int vocab, int pos_rows, int padding_idx, int accumulate, void* ws,
+                                  long long ws_bytes, void* stream) {
+  DBIR_CHECK_ARG(dy && tokens && dtable && ws && (dpos || pos_rows == 0), "dbir_embedding_bwd: null pointer");
+  DBIR_CHECK_ARG(n > 0 && n < (1 << 30) && L > 0 && n % L == 0 && W > 0 && vocab > 0 && ldg >= W && ldd >= W, "dbir_embedding_bwd: bad shape");
+  DBIR_CHECK_ARG(pos_rows == 0 || (pos_rows >= L && pos_rows <= 65535), "dbir_embedding_bwd: pos_rows must be 0 or L .. 65535");
+  DBIR_CHECK_ARG(dtype >= 0 && dtype <= 2, "dbir_embedding_bwd: bad dtype");
+  DBIR_CHECK_ARG(cdiv(W, 1024) <= 65535, "dbir_embedding_bwd: W too large");
+  const Plan p = plan_of(n, W, vocab);
+  DBIR_CHECK_ARG(ws_bytes >= p.total * 4 && (reinterpret_cast<uintptr_t>(ws) & 15) == 0,
+                 "dbir_embedding_bwd: the workspace must hold %lld bytes, 16-byte aligned", p.total * 4);
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const long long np = ((long long)n + 3) / 4 * 4;
+  uint32_t* w = reinterpret_cast<uint32_t*>(ws);
+  uint32_t* key[2] = {w, w + 2 * np};
+  int* pos[2] = {reinterpret_cast<int*>(w + np), reinterpret_cast<int*>(w + 3 * np)};
+  int* hist = reinterpret_cast<int*>(w + p.hist);
+  float* part = reinterpret_cast<float*>(w + p.part);
+  int at = 0;
+  if (n <= RANK_MAX) {
+    hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)cdiv(n, 64)), dim3(256), 0, s, tokens, n, vocab, key[0], pos[0]);
+  } else {
+    for (int pass = 0; pass < p.passes; ++pass) {
+      const long long* t = pass == 0 ? tokens : nullptr;
+      const dim3 g((unsigned)cdiv(p.nseg, 4));
+      hipLaunchKernelGGL(embed_count_kernel, g, dim3(256), 0, s, t, key[at], n, vocab, 8 * pass, p.seg, p.nseg, hist);
+      hipLaunchKernelGGL(embed_place_kernel, g, dim3(256), 0, s, t, key[at], pos[at], n, vocab, 8 * pass, p.seg, p.nseg, hist, key[at ^ 1], pos[at ^ 1]);
+      at ^= 1;
+    }
+  }
+  const bool v4 = W % 4 == 0 && al(dy, ldg, elem4(dtype)) && al(dtable, ldd, 16);
+  const dim3 gp((unsigned)p.pieces, (unsigned)cdiv(W, 1024)), gr((unsigned)cdiv(vocab, 32), (unsigned)cdiv(W, 256)), gl((unsigned)cdiv(W, 256), (unsigned)pos_rows);
+#define GO2(T, V)                                                                                                                                \
+  do {                                                                                                                                           \
+    if (p.pieces) hipLaunchKernelGGL((embed_piece_kernel<T, V>), gp, dim3(256), 0, s, (const T::elem*)dy, ldg, key[at], pos[at], part, W, p.Wp);  \
+    hipLaunchKernelGGL((embed_rows_kernel<T, V>), gr, dim3(256), 0, s, (const T::elem*)dy, ldg, key[at], pos[at], part, dtable, ldd, scale, n, W, \
+                       p.Wp, vocab, padding_idx, accumulate);                                                                                    \
+    if (pos_rows) hipLaunchKernelGGL((embed_pos_kernel<T, V>), gl, dim3(256), 0, s, (const T::elem*)dy, ldg, dpos, n / L, L, W);                  \
+  } while (0)
+#define GO(T)          \
+  do {                 \
+    if (v4) GO2(T, 4); \
+    else GO2(T, 1);    \
+  } while (0)
+  if (dtype == DBIR_F16) GO(F16T);
+  else if (dtype == DBIR_BF16) GO(BF16T);
+  else GO(F32T);
+#undef GO
+#undef GO2
+  DBIR_CHECK_LAUNCH("dbir_embedding_bwd");
+  return DBIR_OK;
+}

@@ -9,8 +9,8 @@ from ctypes import POINTER, Structure, c_char_p, c_float, c_int, c_longlong, c_v
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("DBIR_HIP_LIB", os.path.join(_HERE, "libdbir_hip.so"))
 
-F16, BF16 = 0, 1
-ABI_VERSION = 5   # include/dbir.h dbir_abi_version(): checked at load time (a stale libdbir_hip.so must not run silently)
+F16, BF16, F32 = 0, 1, 2
+ABI_VERSION = 6   # include/dbir.h dbir_abi_version(): checked at load time (a stale libdbir_hip.so must not run silently)
 ACT_NONE, ACT_SILU, ACT_GELU, ACT_LRELU, ACT_GEGLU = 0, 1, 2, 3, 4
 MODE_LINEAR, MODE_CONV3X3 = 0, 1
 
@@ -37,6 +37,20 @@ class GemmDesc(Structure):
     ]
 
 
+class AttnDesc(Structure):
+    """Mirror of `dbir_attn_desc` (include/dbir.h) — field order and types must match exactly."""
+    _fields_ = [
+        ("dtype", c_int), ("B", c_int), ("H", c_int), ("Hkv", c_int), ("Lq", c_int), ("Lk", c_int), ("causal", c_int),
+        ("scale", c_float),
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("out", c_void_p), ("lse", c_void_p),
+        ("q_len", c_void_p), ("kv_len", c_void_p),
+        ("dout", c_void_p), ("dq", c_void_p), ("dk", c_void_p), ("dv", c_void_p),
+        ("ws", c_void_p), ("ws_bytes", c_longlong),
+        ("q_stride", c_longlong * 3), ("k_stride", c_longlong * 3), ("v_stride", c_longlong * 3), ("out_stride", c_longlong * 3),
+        ("dout_stride", c_longlong * 3), ("dq_stride", c_longlong * 3), ("dk_stride", c_longlong * 3), ("dv_stride", c_longlong * 3),
+    ]
+
+
 _I, _LL, _F, _P = c_int, c_longlong, c_float, c_void_p
 
 # name -> argtypes (restype is int unless noted).  Kept in one table so tests can check that the library
@@ -44,6 +58,14 @@ _I, _LL, _F, _P = c_int, c_longlong, c_float, c_void_p
 SIGNATURES = {
     "dbir_gemm": [POINTER(GemmDesc), _P],
     "dbir_attention": [_I, _P, _LL, _LL, _P, _LL, _LL, _P, _LL, _LL, _P, _LL, _LL, _I, _I, _I, _I, _F, _P],
+    "dbir_attention_fwd_ws": [POINTER(AttnDesc), POINTER(c_longlong)], "dbir_attention_bwd_ws": [POINTER(AttnDesc), POINTER(c_longlong)],
+    "dbir_attention_fwd": [POINTER(AttnDesc), _P], "dbir_attention_bwd": [POINTER(AttnDesc), _P],
+    "dbir_layernorm_bwd_ws": [_I, _I, POINTER(c_longlong)],
+    "dbir_layernorm_fwd": [_I, _P, _LL, _P, _LL, _P, _P, _P, _I, _I, _F, _P],
+    "dbir_layernorm_bwd": [_I, _P, _LL, _P, _LL, _P, _LL, _P, _LL, _P, _P, _P, _P, _I, _I, _P, _LL, _P],
+    "dbir_embedding_fwd": [_I, _P, _LL, _P, _P, _LL, _I, _P, _LL, _F, _I, _I, _I, _I, _P],
+    "dbir_embedding_bwd_ws": [_I, _I, _I, POINTER(c_longlong)],
+    "dbir_embedding_bwd": [_I, _P, _LL, _P, _P, _LL, _P, _F, _I, _I, _I, _I, _I, _I, _I, _P, _LL, _P],
     "dbir_window_attention": [_I, _P, _LL, _P, _LL, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P],
     "dbir_groupnorm_nchunk": [_I, _I],
     "dbir_groupnorm": [_I, _P, _LL, _P, _LL, _P, _P, _I, _I, _I, _I, _F, _I, _P, _P],

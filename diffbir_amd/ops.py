@@ -13,12 +13,13 @@ Conventions
 """
 import ctypes
 import os
+from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import Optional, Tuple
 
 import torch
 
-from . import autotune, native, tuning
+from . import autotune, native, plan, tuning
 from .native import (ACT_GEGLU, ACT_GELU, ACT_LRELU, ACT_NONE, ACT_SILU, MODE_CONV3X3, MODE_LINEAR,  # noqa: F401
                      GemmDesc)
 
@@ -665,6 +666,219 @@ def causal_attention(qkv: T, heads: int, scale: float) -> T:
     native.check(native.lib().dbir_causal_attention(_dt(qkv), qkv.data_ptr(), qkv.stride(1), out.data_ptr(), heads * 64, B,
                                                     heads, L, scale, _stream()), "dbir_causal_attention")
     return out
+
+
+# ------------------------------------------------------------------------------------------------ training operators
+# Forward passes that keep what the backward pass needs, and the backward passes (include/dbir.h "Training operators").  Plain
+# functions like everything here: a caller who wants torch.autograd wraps them in its own Function.  Results do not depend on
+# the run (no floating-point atomics); workspaces are allocated per call, so calls on several streams and calls captured into
+# several graphs share nothing.
+def _need(ok: bool, msg: str) -> None:
+    if not ok:
+        raise ValueError(msg)
+
+
+def _train_args(what: str, *ts) -> torch.device:
+    """Every tensor on one GPU, and no plan being recorded: a replay would miss these calls."""
+    _gpu(*ts)
+    _need(not plan.recording(), f"{what}: training operators cannot be part of a recorded evaluation")
+    dev = ts[0].device
+    for t in ts:
+        _need(t is None or t.device == dev, f"{what}: tensors on different devices ({dev}, {getattr(t, 'device', None)})")
+    return dev
+
+
+def _on(dev: torch.device):
+    """Launches go to the current stream of the tensors' device."""
+    return nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _dt3(t: T) -> int:
+    return native.F32 if t.dtype == torch.float32 else _dt(t)
+
+
+def _row_ld(t: T, what: str) -> int:
+    """Row stride of [..., C] whose rows lie evenly apart."""
+    C = t.shape[-1]
+    _need(C == 1 or t.stride(-1) == 1, f"{what}: the last dimension must have unit stride")
+    ld, span = None, 0
+    for n, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+        if n > 1:
+            if ld is None:
+                ld, span = st, st * n
+            else:
+                _need(st == span, f"{what}: the rows must lie evenly apart, got shape {tuple(t.shape)} strides {t.stride()}")
+                span = st * n
+    _need(ld is None or ld >= C, f"{what}: the rows overlap, got shape {tuple(t.shape)} strides {t.stride()}")
+    return C if ld is None else ld
+
+
+def _f32_vec(t: T, n: int, what: str) -> None:
+    _need(t.dtype == torch.float32 and t.numel() == n and t.is_contiguous(), f"{what}: expected {n} contiguous f32 values")
+
+
+def _apart(what: str, outs, ins) -> None:
+    """No output may be an input or another output (the backward passes read their inputs more than once)."""
+    ptrs = [t.data_ptr() for t in outs]
+    _need(len(set(ptrs)) == len(ptrs) and not set(ptrs) & {t.data_ptr() for t in ins if t is not None},
+          f"{what}: outputs must not share memory with inputs or each other")
+
+
+def _strides(t: T):
+    """Batch, row and head stride of [B, L, H, 64]; a dimension of one row has no stride."""
+    st = t.stride()
+    return (st[0] if t.shape[0] > 1 else 0, st[1] if t.shape[1] > 1 else 64, st[2] if t.shape[2] > 1 else 0)
+
+
+def _attn_desc(what: str, q: T, k: T, v: T, out: T, lse: T, scale, causal, q_len, kv_len, dout=None, dq=None, dk=None, dv=None):
+    B, Lq, H, _ = q.shape
+    Lk, Hkv = k.shape[1], k.shape[2]
+    for name, t, shape in (("q", q, (B, Lq, H, 64)), ("k", k, (B, Lk, Hkv, 64)), ("v", v, (B, Lk, Hkv, 64)), ("out", out, (B, Lq, H, 64)),
+                           ("dout", dout, (B, Lq, H, 64)), ("dq", dq, (B, Lq, H, 64)), ("dk", dk, (B, Lk, Hkv, 64)), ("dv", dv, (B, Lk, Hkv, 64))):
+        if t is not None:
+            _need(tuple(t.shape) == shape, f"{what}: {name} must have shape {shape}, got {tuple(t.shape)}")
+            _need(t.dtype == q.dtype, f"{what}: {name} is {t.dtype}, q is {q.dtype}")
+            _need(t.stride(3) == 1, f"{what}: {name}: the head dimension must have unit stride")
+    for name, t in (("out", out if dout is None else None), ("dq", dq), ("dk", dk), ("dv", dv)):
+        _need(t is None or all(n == 1 or st for n, st in zip(t.shape, t.stride())), f"{what}: {name} must not be an expanded tensor")
+    for name, t in (("q_len", q_len), ("kv_len", kv_len)):
+        _need(t is None or (t.dtype == torch.int32 and tuple(t.shape) == (B,) and t.is_contiguous()), f"{what}: {name} must be int32 [{B}]")
+    _need(lse.dtype == torch.float32 and tuple(lse.shape) == (B, H, Lq) and lse.is_contiguous(), f"{what}: lse must be contiguous f32 [{B}, {H}, {Lq}]")
+    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    s3 = lambda t: (0, 0, 0) if t is None else _strides(t)  # noqa: E731
+    return native.AttnDesc(_dt(q), B, H, Hkv, Lq, Lk, int(bool(causal)), float(scale), p(q), p(k), p(v), p(out), p(lse), p(q_len), p(kv_len),
+                           p(dout), p(dq), p(dk), p(dv), None, 0, s3(q), s3(k), s3(v), s3(out), s3(dout), s3(dq), s3(dk), s3(dv))
+
+
+def _attn_run(name: str, d, dev) -> None:
+    nbytes = ctypes.c_longlong()
+    native.check(getattr(native.lib(), name + "_ws")(ctypes.byref(d), ctypes.byref(nbytes)), name + "_ws")
+    if nbytes.value:
+        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
+        d.ws, d.ws_bytes = ws.data_ptr(), nbytes.value
+    native.check(getattr(native.lib(), name)(ctypes.byref(d), _stream()), name)
+
+
+def attention_fwd(q: T, k: T, v: T, scale: float, causal: bool = False, q_len: Optional[T] = None, kv_len: Optional[T] = None,
+                  out: Optional[T] = None) -> Tuple[T, T]:
+    """softmax(scale q k^T) v for training -> (out [B, Lq, H, 64], lse f32 [B, H, Lq]).  q: [B, Lq, H, 64], k / v: [B, Lk, Hkv, 64]
+    16-bit views with any strides that are multiples of 8 (heads are shared by H / Hkv queries' heads); causal: query i sees keys
+    j <= i + Lk - Lq; q_len / kv_len: int32 [B] lengths of a padded batch: what lies behind is not read, out is zero there.  A row
+    that sees no key gives zeros and lse = -inf."""
+    dev = _train_args("attention_fwd", q, k, v, out, q_len, kv_len)
+    _need(q.dim() == 4 and k.dim() == 4 and v.dim() == 4 and q.shape[3] == 64, "attention_fwd: q, k, v must be [B, L, heads, 64]")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=dev)
+    d = _attn_desc("attention_fwd", q, k, v, out, lse, scale, causal, q_len, kv_len)
+    _apart("attention_fwd", (out,), (q, k, v))
+    with _on(dev):
+        _attn_run("dbir_attention_fwd", d, dev)
+    return out, lse
+
+
+def attention_bwd(dout: T, q: T, k: T, v: T, out: T, lse: T, scale: float, causal: bool = False, q_len: Optional[T] = None,
+                  kv_len: Optional[T] = None, dq: Optional[T] = None, dk: Optional[T] = None, dv: Optional[T] = None) -> Tuple[T, T, T]:
+    """Gradients (dq, dk, dv) of attention_fwd, shaped like q, k, v, from its out and lse and the same mask arguments; the probabilities
+    are recomputed.  dk / dv are sums over the query heads that share them; rows behind a length get zeros."""
+    dev = _train_args("attention_bwd", dout, q, k, v, out, lse, q_len, kv_len, dq, dk, dv)
+    _need(q.dim() == 4 and k.dim() == 4 and v.dim() == 4 and q.shape[3] == 64, "attention_bwd: q, k, v must be [B, L, heads, 64]")
+    dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if dq is None else dq
+    dk = torch.empty(k.shape, dtype=q.dtype, device=dev) if dk is None else dk
+    dv = torch.empty(v.shape, dtype=q.dtype, device=dev) if dv is None else dv
+    d = _attn_desc("attention_bwd", q, k, v, out, lse, scale, causal, q_len, kv_len, dout, dq, dk, dv)
+    _apart("attention_bwd", (dq, dk, dv), (q, k, v, out, dout))
+    with _on(dev):
+        _attn_run("dbir_attention_bwd", d, dev)
+    return dq, dk, dv
+
+
+def layernorm_fwd(x: T, gamma: T, beta: T, eps: float = 1e-5, out: Optional[T] = None) -> Tuple[T, T]:
+    """LayerNorm over the last dimension for training -> (y, stats f32 [..., 2] = mean | 1 / sigma).  x f16 / bf16 / f32, any width;
+    gamma / beta f32 [C]."""
+    dev = _train_args("layernorm_fwd", x, gamma, beta, out)
+    C = x.shape[-1]
+    out = torch.empty(x.shape, dtype=x.dtype, device=dev) if out is None else out
+    _need(out.shape == x.shape and out.dtype == x.dtype, "layernorm_fwd: out must be like x")
+    _f32_vec(gamma, C, "layernorm_fwd: gamma")
+    _f32_vec(beta, C, "layernorm_fwd: beta")
+    _apart("layernorm_fwd", (out,), (x,))
+    stats = torch.empty(x.shape[:-1] + (2,), dtype=torch.float32, device=dev)
+    with _on(dev):
+        native.check(native.lib().dbir_layernorm_fwd(_dt3(x), x.data_ptr(), _row_ld(x, "layernorm_fwd: x"), out.data_ptr(),
+                                                     _row_ld(out, "layernorm_fwd: out"), gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(),
+                                                     _rows(x), C, eps, _stream()), "dbir_layernorm_fwd")
+    return out, stats
+
+
+def layernorm_bwd(dy: T, x: T, gamma: T, stats: T, dres: Optional[T] = None, dx: Optional[T] = None) -> Tuple[T, T, T]:
+    """Gradients (dx, dgamma f32, dbeta f32) of layernorm_fwd from its x and stats; dres (like x): the gradient that reaches x past the
+    norm (a residual connection) is added to dx."""
+    dev = _train_args("layernorm_bwd", dy, x, gamma, stats, dres, dx)
+    C, M = x.shape[-1], _rows(x)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if dx is None else dx
+    for name, t in (("dy", dy), ("dres", dres), ("dx", dx)):
+        _need(t is None or (t.shape == x.shape and t.dtype == x.dtype), f"layernorm_bwd: {name} must be like x ({tuple(x.shape)}, {x.dtype})")
+    _f32_vec(gamma, C, "layernorm_bwd: gamma")
+    _f32_vec(stats, 2 * M, "layernorm_bwd: stats")
+    _apart("layernorm_bwd", (dx,), (dy, x, dres))
+    dgb = torch.empty((2, C), dtype=torch.float32, device=dev)
+    nbytes = ctypes.c_longlong()
+    native.check(native.lib().dbir_layernorm_bwd_ws(M, C, ctypes.byref(nbytes)), "dbir_layernorm_bwd_ws")
+    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
+    ld = lambda t, n: 0 if t is None else _row_ld(t, "layernorm_bwd: " + n)  # noqa: E731
+    with _on(dev):
+        native.check(native.lib().dbir_layernorm_bwd(_dt3(x), dy.data_ptr(), ld(dy, "dy"), x.data_ptr(), ld(x, "x"),
+                                                     None if dres is None else dres.data_ptr(), ld(dres, "dres"), dx.data_ptr(), ld(dx, "dx"),
+                                                     gamma.data_ptr(), stats.data_ptr(), dgb[0].data_ptr(), dgb[1].data_ptr(), M, C,
+                                                     ws.data_ptr(), nbytes.value, _stream()), "dbir_layernorm_bwd")
+    return dx, dgb[0], dgb[1]
+
+
+def embedding(tokens: T, table: T, scale: float = 1.0, pos: Optional[T] = None, dtype: Optional[torch.dtype] = None,
+              out: Optional[T] = None) -> T:
+    """tokens int64 [..., L] -> scale * table[tokens] (+ pos[:L]) as [..., L, W] in `dtype` (the table's by default).  table f16 / bf16 /
+    f32 [vocab, W], pos f32 [>= L, W]; tokens outside the table read its nearest row, as in clip_embed."""
+    dev = _train_args("embedding", tokens, table, pos, out)
+    _need(tokens.dtype == torch.int64 and tokens.dim() >= 1 and tokens.is_contiguous(), "embedding: tokens must be contiguous int64 [..., L]")
+    _need(table.dim() == 2 and (pos is None or (pos.dim() == 2 and pos.dtype == torch.float32)), "embedding: table must be [vocab, W], pos f32 [L, W]")
+    (vocab, W), L, n = table.shape, tokens.shape[-1], tokens.numel()
+    _need(pos is None or (pos.shape[0] >= L and pos.shape[1] == W), "embedding: pos must be [>= L, W]")
+    if out is None:
+        out = torch.empty(tokens.shape + (W,), dtype=dtype or table.dtype, device=dev)
+    _need(out.shape == tokens.shape + (W,) and dtype in (None, out.dtype), "embedding: out must be [..., L, W] in `dtype`")
+    _apart("embedding", (out,), (table, pos))
+    with _on(dev):
+        native.check(native.lib().dbir_embedding_fwd(_dt3(table), table.data_ptr(), _row_ld(table, "embedding: table"), tokens.data_ptr(),
+                                                     None if pos is None else pos.data_ptr(), 0 if pos is None else _row_ld(pos, "embedding: pos"),
+                                                     _dt3(out), out.data_ptr(), _row_ld(out, "embedding: out"), scale, n, L, W, vocab,
+                                                     _stream()), "dbir_embedding_fwd")
+    return out
+
+
+def embedding_bwd(dy: T, tokens: T, vocab: int, scale: float = 1.0, pos_rows: int = 0, padding_idx: Optional[int] = None,
+                  out: Optional[T] = None, accumulate: bool = False) -> Tuple[T, Optional[T]]:
+    """Gradients of embedding -> (dtable f32 [vocab, W], dpos f32 [pos_rows, W] or None).  dy f16 / bf16 / f32 [..., L, W]; the row of
+    padding_idx gets none; out + accumulate: added to `out`, whose rows that no token names stay untouched."""
+    dev = _train_args("embedding_bwd", dy, tokens, out)
+    _need(tokens.dtype == torch.int64 and tokens.dim() >= 1 and tokens.is_contiguous(), "embedding_bwd: tokens must be contiguous int64 [..., L]")
+    _need(dy.shape[:-1] == tokens.shape, f"embedding_bwd: dy {tuple(dy.shape)} does not fit tokens {tuple(tokens.shape)}")
+    _need(vocab > 0 and (padding_idx is None or 0 <= padding_idx < vocab), "embedding_bwd: padding_idx must be a row of the table")
+    _need(out is not None or not accumulate, "embedding_bwd: accumulate needs `out`")
+    W, L, n = dy.shape[-1], tokens.shape[-1], tokens.numel()
+    out = torch.empty((vocab, W), dtype=torch.float32, device=dev) if out is None else out
+    _need(tuple(out.shape) == (vocab, W) and out.dtype == torch.float32, f"embedding_bwd: out must be f32 [{vocab}, {W}]")
+    _apart("embedding_bwd", (out,), (dy,))
+    dpos = torch.empty((pos_rows, W), dtype=torch.float32, device=dev) if pos_rows else None
+    nbytes = ctypes.c_longlong()
+    native.check(native.lib().dbir_embedding_bwd_ws(n, W, vocab, ctypes.byref(nbytes)), "dbir_embedding_bwd_ws")
+    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
+    with _on(dev):
+        native.check(native.lib().dbir_embedding_bwd(_dt3(dy), dy.data_ptr(), _row_ld(dy, "embedding_bwd: dy"), tokens.data_ptr(), out.data_ptr(),
+                                                     _row_ld(out, "embedding_bwd: out"), None if dpos is None else dpos.data_ptr(), scale, n, L, W,
+                                                     vocab, pos_rows, -1 if padding_idx is None else padding_idx, int(accumulate),
+                                                     ws.data_ptr(), nbytes.value, _stream()), "dbir_embedding_bwd")
+    return out, dpos
 
 
 # ------------------------------------------------------------------------------------------------ elementwise

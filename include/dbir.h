@@ -23,6 +23,7 @@ extern "C" {
 
 #define DBIR_F16 0
 #define DBIR_BF16 1
+#define DBIR_F32 2 /* only where an entry point says so */
 
 /* epilogue activations */
 #define DBIR_ACT_NONE 0
@@ -40,7 +41,8 @@ const char* dbir_last_error(void);
  * 4 since round 4: dbir_gemm_desc.stats holds [sum, M2] per (row tile, column) instead of [sum, sum of squares] (and
  * dbir_groupnorm_from_partials reads that), split-K launches emit them; tile 80 = the fine-phase 256x320 kernel.
  * 5 since round 5: dbir_gemm_desc.upsample == 2 (parity-collapsed upsample convolution), dbir_groupnorm_apply_partials,
- * dbir_copy_rows, dbir_plan_* / dbir_cldm_forward (module-level entry point: a recorded network evaluation replayed from C). */
+ * dbir_copy_rows, dbir_plan_* / dbir_cldm_forward (module-level entry point: a recorded network evaluation replayed from C).
+ * 6: the training operators (dbir_attention_fwd / _bwd, dbir_layernorm_fwd / _bwd, dbir_embedding_fwd / _bwd). */
 int dbir_abi_version(void);
 /* Process-wide tuning / A-B switches (never needed for correctness): DBIR_OPT_ATTN_VARIANT 2 (default) = LDS-resident
  * cross-attention kernel for Lk <= 96 + generic flash kernel otherwise, 3 = generic flash kernel for every shape, 4 / 5 =
@@ -274,6 +276,61 @@ int dbir_xf_head(int dtype, const void* x, long long ldx, const float* gn_scale_
 int dbir_xf_tail(int dtype, const void* attn_out, long long ldo, const void* h, long long ldh, const void* x, long long ldx,
                  void* out, long long ldout, int M, int L, int C, int pair_bs, const void* wstream, long long wstream_bytes,
                  const float* prm, const void* kfrag, const void* vfrag, int Lk, float scale, int stop_after, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Training operators: forward passes that keep what the backward pass needs, and the backward passes.  None of them can be part
+ * of a dbir_plan.  All results are the same in every run (no floating-point atomics).  Workspaces are the caller's, one per call in flight;
+ * nothing in them is kept from one call for the next.
+ *
+ * dbir_attention_fwd / dbir_attention_bwd (csrc/attention_train.hip): softmax(scale Q K^T) V, head_dim 64, 16-bit (dtype f16 / bf16).
+ *   q, out, dout, dq [B, Lq, H, 64]; k, v, dk, dv [B, Lk, Hkv, 64], H % Hkv == 0 (query head h reads key head h / (H / Hkv)); strides are
+ *   those of batch, row and head in elements (multiples of 8; rows at least 64 and less than 2^23 apart; 16-byte aligned bases), so a slice of
+ *   a wider buffer or a [B, H, L, 64] tensor serves as well.
+ *   lse f32 [B, H, Lq] dense: log of the sum of exp(scale q . k) over the visible keys, -infinity where a row sees none.
+ *   causal: query i sees keys j <= i + Lk - Lq.  q_len / kv_len: int32 [B] on the device or NULL: rows of sample b at or behind its length are
+ *   not read (they may hold anything); out, dq, dk, dv are zero and lse is -infinity there.  A row that sees no key: out and dq zero.
+ *   The backward pass takes out and lse of the forward pass.  ws: dbir_attention_bwd_ws bytes (forward: dbir_attention_fwd_ws), 16-byte
+ *   aligned. */
+typedef struct {
+  int dtype, B, H, Hkv, Lq, Lk, causal;
+  float scale;
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  const int *q_len, *kv_len;
+  const void* dout;
+  void *dq, *dk, *dv;
+  void* ws;
+  long long ws_bytes;
+  long long q_stride[3], k_stride[3], v_stride[3], out_stride[3], dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
+} dbir_attn_desc;
+int dbir_attention_fwd_ws(const dbir_attn_desc* d, long long* bytes);
+int dbir_attention_bwd_ws(const dbir_attn_desc* d, long long* bytes);
+int dbir_attention_fwd(const dbir_attn_desc* d, void* stream);
+int dbir_attention_bwd(const dbir_attn_desc* d, void* stream);
+
+/* dbir_layernorm_fwd / dbir_layernorm_bwd (csrc/norm_train.hip): rows of C columns, dtype f16 / bf16 / f32 for x, y, dy, dres, dx (row
+ *   strides ld*, any alignment), everything else f32.  stats [rows, 2]: mean and 1 / sqrt(variance + eps).
+ *   dx = gradient of x (+ dres, the gradient that arrives past the norm, if not NULL); dgamma, dbeta [C] are written, not added to.
+ *   ws: dbir_layernorm_bwd_ws bytes. */
+int dbir_layernorm_bwd_ws(int rows, int C, long long* bytes);
+int dbir_layernorm_fwd(int dtype, const void* x, long long ldx, void* y, long long ldy, const float* gamma, const float* beta,
+                       float* stats, int rows, int C, float eps, void* stream);
+int dbir_layernorm_bwd(int dtype, const void* dy, long long lddy, const void* x, long long ldx, const void* dres, long long lddres,
+                       void* dx, long long lddx, const float* gamma, const float* stats, float* dgamma, float* dbeta, int rows, int C,
+                       float* ws, long long ws_bytes, void* stream);
+
+/* dbir_embedding_fwd / dbir_embedding_bwd (csrc/embedding.hip): out[i, :] = scale table[tokens[i], :] + pos[i % L, :] (pos f32 or NULL)
+ *   for n tokens (int64, clamped to [0, vocab)); table and out f16 / bf16 / f32.
+ *   Backward: dtable f32 [vocab, W] = scale times the sum of dy over the positions of each token, zeros where there are none or the token is
+ *   padding_idx (-1: none); accumulate: added to dtable, rows without a position untouched.  dpos f32 [pos_rows, W] (pos_rows 0, or
+ *   L .. 65535): sum of dy over the batch for l < L, zeros behind.  ws: dbir_embedding_bwd_ws bytes, 16-byte aligned. */
+int dbir_embedding_fwd(int table_dtype, const void* table, long long ldt, const long long* tokens, const float* pos, long long ldpos,
+                       int out_dtype, void* out, long long ldo, float scale, int n, int L, int W, int vocab, void* stream);
+int dbir_embedding_bwd_ws(int n, int W, int vocab, long long* bytes);
+int dbir_embedding_bwd(int dtype, const void* dy, long long lddy, const long long* tokens, float* dtable, long long lddtable, float* dpos,
+                       float scale, int n, int L, int W, int vocab, int pos_rows, int padding_idx, int accumulate, void* ws,
+                       long long ws_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * OpenCLIP text tower (reference diffbir/model/clip.py:37-54 -> open_clip Transformer / ResidualAttentionBlock; its

@@ -1,0 +1,487 @@
+"""-m gpu: the training operators (attention, layer norm and token embedding with their backward passes) against plain 64-bit
+implementations on the same inputs.
+
+Tolerances, with u = torch.finfo(dtype).eps / 2 (a rounding to nearest is off by at most u relative to the value).  Relative 2-norm
+errors: a result rounded once from 32-bit arithmetic is off by at most u, plus the 32-bit sums.
+  layer norm, embedding: f32 sums of n terms are off by less than n 2^-24 of the sum of magnitudes; measured against the result's own norm
+    (random signs: the sum of magnitudes is ~ sqrt(n) times it) 2e-6 covers every size here, so u + 2e-6.
+  attention out: p is rounded for the product (u) and the result (u): 2 u + 1e-5 (1e-5: exp2 and the 32-bit scores, |score| < 20, 20 * 2^-24
+    * a few).  dv: the same.  dq, dk: ds is rounded (u) and the result (u); D = do . out from the rounded out is corrected where a row sees up
+    to 128 keys, and else off by up to u |do| |out| with |out| ~ 1 / sqrt(keys) of |v|: within another u of ds.  6 u + 2e-5 together.
+Single values: 8 times that against the larger of the value and the tensor's rms (a sum of few roundings reaches several of its rms)."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+ops = None
+DEV = None
+F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _setup():
+    global ops, DEV
+    assert torch.cuda.is_available(), "GPU tests need a GPU"
+    from diffbir_amd import native, ops as real_ops
+    native.lib()
+    ops = real_ops
+    DEV = torch.device("cuda:0")
+
+
+def u(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def near(name, got, ref, tol):
+    got, ref = got.double(), ref.double()
+    assert got.shape == ref.shape, name
+    inf = torch.isinf(ref)
+    assert torch.equal(torch.isinf(got), inf) and torch.equal(got[inf], ref[inf]), f"{name}: infinities differ"
+    got, ref = got[~inf], ref[~inf]
+    assert torch.isfinite(got).all(), f"{name}: not finite"
+    if not ref.numel() or not ref.norm():
+        assert not got.numel() or not got.abs().max(), f"{name}: zeros expected"
+        return
+    d, rms = got - ref, ref.norm() / math.sqrt(ref.numel())
+    rel, big = (d.norm() / ref.norm()).item(), (d.abs() / torch.maximum(ref.abs(), rms)).max().item()
+    assert rel <= tol and big <= 8 * tol, f"{name}: rel {rel:.3g} max {big:.3g}, allowed {tol:.3g}"
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+# ------------------------------------------------------------------------------------------------ attention
+def attn_ref(q, k, v, do, scale, causal=False, q_len=None, kv_len=None):
+    """64-bit attention over [B, L, H, 64] and its gradients, one (sample, head) at a time."""
+    q, k, v, do = (t.double() for t in (q, k, v, do))
+    B, Lq, H, D = q.shape
+    Lk, Hkv = k.shape[1], k.shape[2]
+    out, dq, dk, dv = torch.zeros_like(q), torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
+    lse = torch.full((B, H, Lq), -math.inf, dtype=torch.float64, device=q.device)
+    i, j = torch.arange(Lq, device=q.device)[:, None], torch.arange(Lk, device=q.device)[None]
+    for b in range(B):
+        nq = Lq if q_len is None else int(q_len[b])
+        nk = Lk if kv_len is None else int(kv_len[b])
+        if nq == 0 or nk == 0:
+            continue
+        seen = (j[:, :nk] <= i[:nq] + Lk - Lq) if causal else torch.ones(nq, nk, dtype=torch.bool, device=q.device)
+        some = seen.any(1)
+        if not some.any():
+            continue
+        for h in range(H):
+            g = h // (H // Hkv)
+            Q, K, V, G = q[b, :nq, h].contiguous(), k[b, :nk, g].contiguous(), v[b, :nk, g].contiguous(), do[b, :nq, h].contiguous()
+            S = (Q @ K.t() * scale).masked_fill(~seen, -math.inf)
+            L = torch.logsumexp(S, 1)
+            P = torch.where(some[:, None], torch.exp(S - L[:, None]), 0.0)
+            O = P @ V
+            dS = P * (G @ V.t() - (G * O).sum(1, keepdim=True))
+            out[b, :nq, h], lse[b, h, :nq] = O, L
+            dq[b, :nq, h] = dS @ K * scale
+            dk[b, :nk, g] += dS.t() @ Q * scale
+            dv[b, :nk, g] += P.t() @ G
+    return out, lse, dq, dk, dv
+
+
+def attn_inputs(B, H, Hkv, Lq, Lk, dtype, seed, gain=1.0):
+    g = gen(seed)
+    r = lambda *s: torch.randn(*s, device=DEV, generator=g).to(dtype)  # noqa: E731
+    return r(B, Lq, H, 64) * 1.5, r(B, Lk, Hkv, 64), r(B, Lk, Hkv, 64), (torch.randn(B, Lq, H, 64, device=DEV, generator=g) * gain).to(dtype)
+
+
+def attn_check(q, k, v, do, scale=0.125, **kw):
+    dt = q.dtype
+    out, lse = ops.attention_fwd(q, k, v, scale, **kw)
+    dq, dk, dv = ops.attention_bwd(do, q, k, v, out, lse, scale, **kw)
+    ref = attn_ref(q, k, v, do, scale, **kw)
+    near("out", out, ref[0], 2 * u(dt) + 1e-5)
+    near("lse", lse, ref[1], 5e-6)
+    near("dv", dv, ref[4], 2 * u(dt) + 1e-5)
+    near("dq", dq, ref[2], 6 * u(dt) + 2e-5)
+    near("dk", dk, ref[3], 6 * u(dt) + 2e-5)
+    return out, lse, dq, dk, dv
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("B,H,Hkv,Lq,Lk,causal", [
+    (1, 1, 1, 2, 2, False), (1, 1, 1, 32, 32, True), (2, 16, 16, 77, 77, True), (2, 5, 5, 256, 77, False), (1, 2, 1, 64, 64, False),
+    (1, 3, 3, 65, 129, True), (2, 4, 2, 127, 128, True), (1, 8, 1, 129, 63, True), (3, 4, 2, 1, 300, False), (1, 2, 2, 300, 2, False),
+    (1, 2, 2, 5, 1000, True), (1, 10, 5, 1, 2049, True), (2, 3, 1, 513, 511, False), (1, 1, 1, 1500, 1, False), (1, 20, 20, 16, 16, False),
+    (1, 2, 2, 200, 40, True)])
+def test_attention_train(B, H, Hkv, Lq, Lk, causal, dtype):
+    q, k, v, do = attn_inputs(B, H, Hkv, Lq, Lk, dtype, 11)
+    if Lk == 1:   # one key: its probability is 1 and no score has a gradient
+        out, lse = ops.attention_fwd(q, k, v, 0.125)
+        dq, dk, dv = ops.attention_bwd(do, q, k, v, out, lse, 0.125)
+        assert torch.equal(out, v.expand_as(out).contiguous())
+        near("dv", dv, do.double().sum(1, keepdim=True), 2 * u(dtype) + 1e-5)
+        assert dq.abs().max() <= 2e-5 and dk.abs().max() <= 1e-3
+        return
+    attn_check(q, k, v, do, causal=causal)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("Lq,Lk,q_len,kv_len", [
+    (200, 200, (200, 1, 0, 130), (200, 1, 0, 130)), (77, 300, None, (300, 0, 64, 65)), (130, 130, (0, 130, 64, 63), None),
+    (64, 96, (64, 33, 32, 1), (96, 95, 31, 2)), (1, 513, None, (513, 512, 1, 0))])
+def test_attention_train_lengths(Lq, Lk, q_len, kv_len, causal, dtype):
+    """Padded batches: what lies behind a length may be NaN or infinite, and comes out as zeros."""
+    q, k, v, do = attn_inputs(4, 4, 2, Lq, Lk, dtype, 12)
+    ql, kl = (None if t is None else torch.tensor(t, dtype=torch.int32, device=DEV) for t in (q_len, kv_len))
+    clean = [t.clone() for t in (q, k, v, do)]
+    for b in range(4):
+        if q_len is not None:
+            q[b, q_len[b]:], do[b, q_len[b]:] = math.nan, math.inf
+        if kv_len is not None:
+            k[b, kv_len[b]:], v[b, kv_len[b]:] = -math.inf, math.nan
+    out, lse = ops.attention_fwd(q, k, v, 0.125, causal=causal, q_len=ql, kv_len=kl)
+    grads = ops.attention_bwd(do, q, k, v, out, lse, 0.125, causal=causal, q_len=ql, kv_len=kl)
+    ref = attn_ref(*clean, 0.125, causal=causal, q_len=ql, kv_len=kl)
+    t = u(dtype)
+    for name, got, want, tol in zip(("out", "lse", "dq", "dk", "dv"), (out, lse, *grads), ref,
+                                    (2 * t + 1e-5, 5e-6, 6 * t + 2e-5, 6 * t + 2e-5, 2 * t + 1e-5)):
+        near(name, got, want, tol)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_train_layouts(dtype):
+    """Slices of packed buffers, [B, H, L, 64] tensors and an expanded input give the same bits as dense ones."""
+    B, L, H = 2, 150, 3
+    qkv = torch.randn(B, L, 3, H, 64, device=DEV, generator=gen(13)).to(dtype)
+    q, k, v = qkv.unbind(2)
+    do = torch.randn(B, H, L, 64, device=DEV, generator=gen(14)).to(dtype).transpose(1, 2)
+    dense = attn_check(q.contiguous(), k.contiguous(), v.contiguous(), do.contiguous(), causal=True)
+    out = torch.full((B, H, L, 64), 7.0, device=DEV, dtype=dtype).transpose(1, 2)
+    _, lse = ops.attention_fwd(q, k, v, 0.125, causal=True, out=out)
+    grad = torch.full((B, L, 4, H, 64), 7.0, device=DEV, dtype=dtype)
+    dq, dk, dv = grad[:, :, 0], grad[:, :, 1], grad[:, :, 2]
+    got = ops.attention_bwd(do, q, k, v, out, lse, 0.125, causal=True, dq=dq, dk=dk, dv=dv)
+    assert got[0] is dq
+    for a, b in zip(dense, (out, lse, dq, dk, dv)):
+        assert torch.equal(a, b)
+    assert (grad[:, :, 3] == 7).all()
+    one = k[:1].expand(B, L, H, 64)
+    a = ops.attention_fwd(q, one, v, 0.125)
+    b = ops.attention_fwd(q, one.contiguous(), v, 0.125)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("gain", [1e-4, 30.0, 3000.0])
+def test_attention_train_f16_gradient_range(gain):
+    """f16: unscaled gradients (ds far below 2^-14) and loss-scaled ones (p ds beyond 65504 unscaled) keep their digits.  dq, dk of gradients of 1e-4
+    are below 2^-14 themselves: half a step of 2^-24 is 2^-25 absolute, on top."""
+    q, k, v, do = attn_inputs(1, 2, 2, 1024, 1024, F16, 15, gain)
+    v = v * 4
+    out, lse = ops.attention_fwd(q, k, v, 0.125)
+    dq, dk, dv = ops.attention_bwd(do, q, k, v, out, lse, 0.125)
+    ref = attn_ref(q, k, v, do, 0.125)
+    for name, got, want, m in (("dq", dq, ref[2], 6), ("dk", dk, ref[3], 6), ("dv", dv, ref[4], 2)):
+        rms = want.norm().item() / math.sqrt(want.numel())
+        # p ranges over 2^-24 .. 1 in f16 steps of 2^-24 * 2^-e below 2^-14: within 4 u of the typical p at these sizes
+        near(name, got, want, (m + 4) * u(F16) + 2e-5 + 2.0 ** -25 / rms)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_attention_train_large_scores(dtype):
+    """Scores of several hundred: one key takes nearly all of a row; nothing overflows."""
+    q, k, v, do = attn_inputs(1, 2, 2, 200, 200, dtype, 16)
+    q = q * 20
+    out, lse = ops.attention_fwd(q, k, v, 0.125)
+    ref = attn_ref(q, k, v, do, 0.125)
+    near("out", out, ref[0], 2 * u(dtype) + 2e-4)    # |s| < 300: 2^-24 * 300 * 8 sums of 64 products = 1.5e-4 of p
+    near("lse", lse, ref[1], 5e-6)
+    assert all(torch.isfinite(t).all() for t in ops.attention_bwd(do, q, k, v, out, lse, 0.125))
+
+
+def test_attention_train_against_differences():
+    """The gradient against central differences of the forward pass's own 64-bit formula in random directions."""
+    q, k, v, do = attn_inputs(1, 2, 1, 40, 50, F16, 17)
+    out, lse = ops.attention_fwd(q, k, v, 0.125, causal=True)
+    grads = ops.attention_bwd(do, q, k, v, out, lse, 0.125, causal=True)
+    f = lambda a, b, c: (attn_ref(a, b, c, do, 0.125, causal=True)[0] * do.double()).sum().item()  # noqa: E731
+    base = [t.double() for t in (q, k, v)]
+    for n in range(3):
+        d = torch.randn(base[n].shape, device=DEV, generator=gen(18 + n), dtype=torch.float64)
+        lo, hi = ([t + (s * d if i == n else 0) for i, t in enumerate(base)] for s in (-1e-4, 1e-4))
+        diff, got = (f(*hi) - f(*lo)) / 2e-4, (grads[n].double() * d).sum().item()
+        # a sum of n values that are off by at most 6 u each of rms size, with random signs
+        assert abs(diff - got) <= (6 * u(F16) + 1e-4) * 4 * grads[n].double().norm().item(), (n, diff, got)
+
+
+def test_attention_train_same_bits_and_streams():
+    """The same result in every run, on another stream than the tensors' own, with two calls in flight."""
+    q, k, v, do = attn_inputs(2, 4, 2, 700, 900, BF16, 19)
+    out, lse = ops.attention_fwd(q, k, v, 0.125, causal=True)
+    ref = (out, lse, *ops.attention_bwd(do, q, k, v, out, lse, 0.125, causal=True))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                o, l = ops.attention_fwd(q, k, v, 0.125, causal=True)
+                got.append((o, l, *ops.attention_bwd(do, q, k, v, o, l, 0.125, causal=True)))
+        torch.cuda.synchronize()
+        for g in got:
+            for a, b in zip(ref, g):
+                assert torch.equal(a, b)
+
+
+def test_attention_train_far_rows():
+    """Rows whose offset passes 2^31 elements."""
+    L, ld = 300, 1 << 23
+    buf = torch.empty((L - 1) * (ld - 8) + 64, dtype=BF16, device=DEV)
+    k = buf.as_strided((1, L, 1, 64), (0, ld - 8, 64, 1))
+    src = torch.randn(1, L, 1, 64, device=DEV, generator=gen(20)).to(BF16)
+    k.copy_(src)
+    q, _, v, do = attn_inputs(1, 1, 1, 70, L, BF16, 21)
+    assert (L - 1) * (ld - 8) > 1 << 31
+    o1, l1 = ops.attention_fwd(q, k, v, 0.125)
+    o2, l2 = ops.attention_fwd(q, src, v, 0.125)
+    assert torch.equal(o1, o2) and torch.equal(l1, l2)
+    for a, b in zip(ops.attention_bwd(do, q, k, v, o1, l1, 0.125), ops.attention_bwd(do, q, src, v, o2, l2, 0.125)):
+        assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------------------------------------ layer norm
+def ln_ref(x, dy, gamma, beta, eps, dres=None):
+    x, dy, gamma, beta = (t.double() for t in (x, dy, gamma, beta))
+    mean = x.mean(-1, keepdim=True)
+    var = ((x - mean) ** 2).mean(-1, keepdim=True)
+    rstd = (var + eps) ** -0.5
+    xh = (x - mean) * rstd
+    a = dy * gamma
+    dx = rstd * (a - a.mean(-1, keepdim=True) - xh * (a * xh).mean(-1, keepdim=True))
+    dims = tuple(range(x.dim() - 1))
+    return xh * gamma + beta, torch.cat([mean, rstd], -1), dx if dres is None else dx + dres.double(), (dy * xh).sum(dims), dy.sum(dims)
+
+
+def ln_inputs(shape, dtype, seed, res=True):
+    g = gen(seed)
+    r = lambda *s: torch.randn(*s, device=DEV, generator=g)  # noqa: E731
+    C = shape[-1]
+    return ((2 * r(*shape) + r(C)).to(dtype), r(*shape).to(dtype), 1 + 0.2 * r(C), 0.2 * r(C), r(*shape).to(dtype) if res else None)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("rows,C", [(1, 64), (3, 3), (5, 8), (154, 1024), (1000, 320), (257, 640), (66, 1280), (33, 1283), (7, 100), (2, 8192),
+                                    (9, 8200), (1, 20000), (4097, 40), (130, 2560), (61, 4096), (19, 5120), (300, 1032)])
+def test_layernorm_train(rows, C, dtype):
+    x, dy, gamma, beta, dres = ln_inputs((rows, C), dtype, 31)
+    y, stats = ops.layernorm_fwd(x, gamma, beta, eps=1e-5)
+    ref = ln_ref(x, dy, gamma, beta, 1e-5, dres)
+    tol = u(dtype) + 2e-6
+    near("y", y, ref[0], tol)
+    near("stats", stats, ref[1], 2e-6)
+    dx, dg, db = ops.layernorm_bwd(dy, x, gamma, stats, dres=dres)
+    near("dx", dx, ref[2], tol)
+    near("dgamma", dg, ref[3], 5e-6)
+    near("dbeta", db, ref[4], 5e-6)
+    dx, dg2, db2 = ops.layernorm_bwd(dy, x, gamma, stats)
+    near("dx without residual", dx, ln_ref(x, dy, gamma, beta, 1e-5)[2], tol)
+    assert torch.equal(dg, dg2) and torch.equal(db, db2)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("off,ld", [(0, 336), (8, 336), (1, 321), (3, 1000)])
+def test_layernorm_train_strided_rows(off, ld, dtype):
+    """Rows inside wider buffers, also at addresses that no wide load is aligned to; what lies between the rows stays."""
+    rows, C = 50, 320
+    x, dy, gamma, beta, dres = ln_inputs((rows, C), dtype, 32)
+    wide = lambda t: torch.full((rows * ld + off,), 7.0, dtype=dtype, device=DEV)[off:].view(rows, ld)[:, :C].copy_(t)  # noqa: E731
+    xs, dys, rs, ys, dxs = wide(x), wide(dy), wide(dres), wide(x), wide(x)
+    y, stats = ops.layernorm_fwd(xs, gamma, beta, out=ys)
+    dx, dg, db = ops.layernorm_bwd(dys, xs, gamma, stats, dres=rs, dx=dxs)
+    ref = ln_ref(x, dy, gamma, beta, 1e-5, dres)
+    near("y", y, ref[0], u(dtype) + 2e-6)
+    near("dx", dx, ref[2], u(dtype) + 2e-6)
+    near("dgamma", dg, ref[3], 5e-6)
+    near("dbeta", db, ref[4], 5e-6)
+    for t in (ys, dxs):
+        full = t.as_strided((rows - 1, ld), (ld, 1), t.storage_offset())
+        assert (full[:, C:] == 7).all()
+
+
+def test_layernorm_train_offset_rows():
+    """Rows far from zero with a small spread: the variance is that of the deviations (2^-24 of the offset 1000 is 6e-5, against a spread of 1)."""
+    x, dy, gamma, beta, _ = ln_inputs((64, 640), F32, 33, False)
+    x = torch.randn(64, 640, device=DEV, generator=gen(34)) + 1000.0
+    y, stats = ops.layernorm_fwd(x, gamma, beta)
+    ref = ln_ref(x, dy, gamma, beta, 1e-5)
+    near("y", y, ref[0], 2e-4)
+    near("dx", ops.layernorm_bwd(dy, x, gamma, stats)[0], ref[2], 2e-4)
+
+
+def test_layernorm_train_constant_rows_and_width_one():
+    x = torch.full((4, 320), 3.0, dtype=F16, device=DEV)
+    gamma, beta = torch.ones(320, device=DEV), torch.full((320,), 0.5, device=DEV)
+    y, stats = ops.layernorm_fwd(x, gamma, beta)
+    assert (y == 0.5).all() and (stats[:, 0] == 3).all()
+    x1, one = torch.randn(9, 1, device=DEV), torch.ones(1, device=DEV)
+    y, stats = ops.layernorm_fwd(x1, one, one)
+    assert (y == 1).all()
+    dx, dg, db = ops.layernorm_bwd(torch.ones(9, 1, device=DEV), x1, one, stats)
+    assert (dx == 0).all() and (dg == 0).all() and (db == 9).all()
+
+
+def test_layernorm_train_against_differences():
+    x, dy, gamma, beta, _ = ln_inputs((6, 77), F32, 35, False)
+    _, stats = ops.layernorm_fwd(x, gamma, beta)
+    grads = ops.layernorm_bwd(dy, x, gamma, stats)
+    base = [t.double() for t in (x, gamma, beta)]
+    f = lambda a, g, b: (ln_ref(a, dy, g, b, 1e-5)[0] * dy.double()).sum().item()  # noqa: E731
+    for n in range(3):
+        d = torch.randn(base[n].shape, device=DEV, dtype=torch.float64, generator=gen(36 + n))
+        lo, hi = ([t + (s * d if i == n else 0) for i, t in enumerate(base)] for s in (-1e-4, 1e-4))
+        diff, got = (f(*hi) - f(*lo)) / 2e-4, (grads[n].double() * d).sum().item()
+        assert abs(diff - got) <= 1e-5 * 4 * max(1.0, grads[n].double().norm().item())
+
+
+# ------------------------------------------------------------------------------------------------ embedding
+def emb_ref(tok, table, dy, scale, pos, vocab, padding=None):
+    t = tok.clamp(0, vocab - 1)
+    x = table.double()[t] * scale
+    if pos is not None:
+        x = x + pos[: tok.shape[-1]].double()
+    d = torch.zeros(vocab, dy.shape[-1], dtype=torch.float64, device=DEV).index_add_(0, t.flatten(), dy.double().reshape(-1, dy.shape[-1]) * scale)
+    if padding is not None:
+        d[padding] = 0
+    return x, d
+
+
+@pytest.mark.parametrize("tdtype,dtype", [(F32, F32), (F32, BF16), (F16, F32), (BF16, BF16), (F16, F16), (BF16, F16), (F16, BF16), (BF16, F32), (F32, F16)])
+@pytest.mark.parametrize("B,L,V,W", [(1, 1, 1, 1), (2, 77, 1000, 1024), (3, 5, 7, 3), (1, 333, 300, 64), (4, 1024, 70000, 20), (40, 125, 33, 260),
+                                     (1, 4097, 257, 5), (2, 2048, 65537, 12)])
+def test_embedding_train(B, L, V, W, tdtype, dtype):
+    g = gen(41)
+    tok = (torch.rand(B, L, device=DEV, generator=g) ** 2 * V).long().clamp_(max=V - 1)
+    if V > 5:
+        tok[0, 0], tok[-1, -1] = -3, V + 9     # read the nearest row, and give it their gradient
+    table, pos = torch.randn(V, W, device=DEV, generator=g).to(tdtype), torch.randn(L + 2, W, device=DEV, generator=g)
+    dy = torch.randn(B, L, W, device=DEV, generator=g).to(dtype)
+    x = ops.embedding(tok, table, scale=1.7, pos=pos, dtype=dtype)
+    ref, dref = emb_ref(tok, table, dy, 1.7, pos, V)
+    near("x", x, ref, u(dtype) + 2e-7)
+    near("x without positions", ops.embedding(tok, table, dtype=dtype), emb_ref(tok, table, dy, 1.0, None, V)[0], u(dtype) + 2e-7)
+    dt, dpos = ops.embedding_bwd(dy, tok, V, scale=1.7, pos_rows=L + 2)
+    near("dtable", dt, dref, 5e-6)
+    near("dpos", dpos[:L], dy.double().sum(0), 5e-6)
+    assert (dpos[L:] == 0).all()
+    again, none = ops.embedding_bwd(dy, tok, V, scale=1.7)
+    assert none is None and torch.equal(dt, again)
+
+
+@pytest.mark.parametrize("n", [63, 64, 65, 4096, 4097, 20000])
+@pytest.mark.parametrize("pattern", ["one", "two", "distinct", "padded"])
+def test_embedding_train_runs(n, pattern):
+    """One token everywhere, two in turn, all different, long padding: whole numbers, so every sum is exact and the order of the sort shows nowhere."""
+    V, W, g = 20000, 36, gen(42)
+    tok = {"one": torch.full((n,), 19999, device=DEV), "two": torch.arange(n, device=DEV) % 2 * 777, "distinct": torch.randperm(V, device=DEV, generator=g)[:n],
+           "padded": torch.where(torch.arange(n, device=DEV) < n // 3, torch.randint(0, V, (n,), device=DEV, generator=g), 0)}[pattern].long()
+    dy = torch.randint(-8, 9, (n, W), device=DEV, generator=g).float()
+    dt, dpos = ops.embedding_bwd(dy, tok, V, scale=0.5)
+    ref = torch.zeros(V, W, device=DEV).index_add_(0, tok, dy * 0.5)
+    assert torch.equal(dt, ref)
+    keep = torch.randint(-8, 9, (V, W), device=DEV, generator=g).float()
+    acc = keep.clone()
+    got, _ = ops.embedding_bwd(dy, tok, V, scale=0.5, out=acc, accumulate=True)
+    assert got is acc and torch.equal(acc, keep + ref)
+    pad = int(tok[-1])
+    dt, _ = ops.embedding_bwd(dy, tok, V, scale=0.5, padding_idx=pad)
+    ref[pad] = 0
+    assert torch.equal(dt, ref)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("off,ld", [(0, 72), (4, 68), (1, 65), (3, 71)])
+def test_embedding_train_strided(off, ld, dtype):
+    V, W, B, L, g = 50, 64, 2, 30, gen(43)
+    wide = lambda n, dt: torch.full((n * ld + off,), 7.0, dtype=dt, device=DEV)[off:].view(n, ld)[:, :W]  # noqa: E731
+    table = wide(V, dtype).copy_(torch.randn(V, W, device=DEV, generator=g))
+    dy = wide(B * L, dtype).copy_(torch.randn(B * L, W, device=DEV, generator=g)).view(B, L, W)
+    tok = torch.randint(0, V, (B, L), device=DEV, generator=g)
+    out = wide(B * L, dtype).view(B, L, W)
+    x = ops.embedding(tok, table, scale=2.0, out=out)
+    ref, dref = emb_ref(tok, table, dy, 2.0, None, V)
+    near("x", x, ref, u(dtype) + 2e-7)
+    dt = wide(V, F32)
+    near("dtable", ops.embedding_bwd(dy, tok, V, scale=2.0, out=dt)[0], dref, 5e-6)
+    assert (dt.as_strided((V - 1, ld), (ld, 1), dt.storage_offset())[:, W:] == 7).all()
+
+
+# ------------------------------------------------------------------------------------------------ together, graphs
+def _block(tok, table, pos, g1, b1, wq, do_up, heads, dt):
+    """Embedding -> layer norm -> packed projection -> causal attention, then all the way back to the table."""
+    B, L = tok.shape
+    W = table.shape[1]
+    x = ops.embedding(tok, table, scale=1.0, pos=pos, dtype=F32)
+    n, stats = ops.layernorm_fwd(x, g1, b1)
+    qkv = (n.to(dt).reshape(B * L, W) @ wq).view(B, L, 3, heads, 64)
+    o, lse = ops.attention_fwd(qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2], 0.125, causal=True)
+    grad = torch.empty_like(qkv)
+    ops.attention_bwd(do_up, qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2], o, lse, 0.125, causal=True, dq=grad[:, :, 0], dk=grad[:, :, 1], dv=grad[:, :, 2])
+    dn = (grad.reshape(B * L, -1) @ wq.t().contiguous()).view(B, L, W).float()
+    dx, dg, db = ops.layernorm_bwd(dn, x, g1, stats, dres=do_up.reshape(B, L, W).float())
+    dtab, dpos = ops.embedding_bwd(dx, tok, table.shape[0], pos_rows=pos.shape[0])
+    return o, dg, db, dtab, dpos
+
+
+def _block_inputs(seed, dt, B=2, L=77, V=500, heads=2):
+    g = gen(seed)
+    W = heads * 64
+    r = lambda *s: torch.randn(*s, device=DEV, generator=g)  # noqa: E731
+    return (torch.randint(0, V, (B, L), device=DEV, generator=g), r(V, W), 0.1 * r(L, W), 1 + 0.1 * r(W), 0.1 * r(W),
+            (r(W, 3 * W) / W ** 0.5).to(dt), r(B, L, heads, 64).to(dt))
+
+
+def test_training_block_matches_autograd():
+    """The operators one after another as a block uses them, against torch's 64-bit autograd on the CPU.  f16 activations between the steps:
+    each of ~8 roundings moves the result by at most u."""
+    dt, heads = F16, 2
+    tok, table, pos, g1, b1, wq, up = _block_inputs(51, dt)
+    got = _block(tok, table, pos, g1, b1, wq, up, heads, dt)
+    tab, ps, g, b = (t.double().cpu().requires_grad_() for t in (table, pos, g1, b1))
+    x = tab[tok.cpu()] + ps
+    n = torch.nn.functional.layer_norm(x, (x.shape[-1],), g, b, 1e-5)
+    B, L, W = x.shape
+    qkv = (n.reshape(B * L, W) @ wq.double().cpu()).view(B, L, 3, heads, 64)
+    q, k, v = (qkv[:, :, i].transpose(1, 2) for i in range(3))
+    s = (q @ k.transpose(2, 3)) * 0.125
+    s = s.masked_fill(torch.ones(L, L).triu(1).bool(), -math.inf)
+    o = (s.softmax(-1) @ v).transpose(1, 2)
+    ((o * up.double().cpu()).sum() + (x * up.double().cpu().reshape(B, L, W)).sum()).backward()
+    for name, a, r in zip(("out", "dgamma", "dbeta", "dtable", "dpos"), got, (o.detach(), g.grad, b.grad, tab.grad, ps.grad)):
+        near(name, a.cpu(), r, 8 * 2 * u(dt))
+
+
+def test_training_block_in_two_graphs():
+    """Captured twice, the graphs replayed in turn and on two streams at once with eager work between: bitwise the eager result."""
+    dt, heads = BF16, 2
+    sets = [_block_inputs(52 + i, dt) for i in range(2)]
+    want = [_block(*s, heads, dt) for s in sets]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for s in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(_block(*s, heads, dt))
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in sets]
+    for turn in range(4):
+        for o in outs:
+            for t in o:
+                t.fill_(math.nan)
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        eager = _block(*sets[turn % 2], heads, dt)
+        torch.cuda.synchronize()
+        for o, w in zip(outs + [eager], want + [want[turn % 2]]):
+            for a, b in zip(o, w):
+                assert torch.equal(a, b), turn

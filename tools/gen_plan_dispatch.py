@@ -14,7 +14,9 @@ from diffbir_amd import native  # noqa: E402
 
 OUT = os.path.join(ROOT, "diffbir_amd", "csrc", "plan_dispatch.inc")
 NOT_RECORDABLE = {"dbir_groupnorm_nchunk", "dbir_xf_tile_bytes", "dbir_xf_head_tiles", "dbir_xf_tail_tiles", "dbir_xf_geometry", "dbir_xf2_geometry",
-                  "dbir_abi_version", "dbir_set_option", "dbir_cldm_forward"}
+                  "dbir_abi_version", "dbir_set_option", "dbir_cldm_forward",
+                  # training operators: not part of a network evaluation (ops.py refuses them while one is recorded)
+                  "dbir_attention_fwd", "dbir_attention_bwd", "dbir_layernorm_fwd", "dbir_layernorm_bwd", "dbir_embedding_fwd", "dbir_embedding_bwd"}
 CT = {native._I: ("int", "(int)a[{k}].i"), native._LL: ("long long", "a[{k}].i"), native._F: ("float", "(float)a[{k}].f"),
       native._P: ("void*", "a[{k}].p")}
 
