@@ -478,16 +478,22 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_q_kernel(const Args a) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
-bool good_layout(const void* p, const long long* s, int rows) {   // batch, row, head strides
-  return p && (reinterpret_cast<uintptr_t>(p) & 15) == 0 && s[0] >= 0 && s[1] >= 0 && s[2] >= 0 && s[0] % 8 == 0 && s[1] % 8 == 0 &&
-         s[2] % 8 == 0 && (rows == 1 || s[1] >= HD) && s[1] < (1 << 23);
+// batch, row, head strides of a tensor of n[0], n[1], n[2] of them; 0: fit, else what is wrong
+const char* bad_layout(const void* p, const long long* s, int B, int rows, int heads, bool written) {
+  if (!p || (reinterpret_cast<uintptr_t>(p) & 15)) return "must be 16-byte aligned and not NULL";
+  const int n[3] = {B, rows, heads};
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (s[i] < 0 || s[i] % 8 || (written && s[i] == 0))) return "needs strides that are multiples of 8 elements (an output: none of 0)";
+  if (rows > 1 && (s[1] < HD || s[1] >= (1 << 23))) return "needs rows at least 64 and less than 2^23 elements apart";
+  return nullptr;
 }
-#define CHECK_LAYOUT(P, S, ROWS)                                                                                              \
-  DBIR_CHECK_ARG(good_layout(d->P, d->S, ROWS),                                                                               \
-                 "%s: " #P " must be 16-byte aligned with strides that are multiples of 8 elements, rows at least 64 apart and " \
-                 "less than 2^23", name)
+#define CHECK_LAYOUT(P, S, ROWS, HEADS, WRITTEN)                                    \
+  do {                                                                              \
+    const char* bad_ = bad_layout(d->P, d->S, d->B, d->ROWS, d->HEADS, WRITTEN);     \
+    DBIR_CHECK_ARG(!bad_, "%s: " #P " %s", name, bad_);                             \
+  } while (0)
 
-int check_desc(const dbir_attn_desc* d, const char* name) {
+int check_desc(const dbir_attn_desc* d, const char* name, bool bwd) {
   DBIR_CHECK_ARG(d, "%s: null descriptor", name);
   DBIR_CHECK_ARG(d->dtype == DBIR_F16 || d->dtype == DBIR_BF16, "%s: bad dtype %d", name, d->dtype);
   DBIR_CHECK_ARG(d->B > 0 && d->H > 0 && d->Hkv > 0 && d->Lq > 0 && d->Lk > 0 && d->H % d->Hkv == 0,
@@ -497,10 +503,23 @@ int check_desc(const dbir_attn_desc* d, const char* name) {
                      (long long)cdiv(d->Lk, 128) * d->B * d->Hkv < 2147483647LL, "%s: grid too large", name);
   DBIR_CHECK_ARG(d->scale > 0.f && d->scale < INFINITY, "%s: scale must be positive and finite", name);
   DBIR_CHECK_ARG(d->lse, "%s: null lse", name);
-  CHECK_LAYOUT(q, q_stride, d->Lq);
-  CHECK_LAYOUT(k, k_stride, d->Lk);
-  CHECK_LAYOUT(v, v_stride, d->Lk);
-  CHECK_LAYOUT(out, out_stride, d->Lq);
+  CHECK_LAYOUT(q, q_stride, Lq, H, false);
+  CHECK_LAYOUT(k, k_stride, Lk, Hkv, false);
+  CHECK_LAYOUT(v, v_stride, Lk, Hkv, false);
+  CHECK_LAYOUT(out, out_stride, Lq, H, !bwd);
+  if (!bwd) {
+    DBIR_CHECK_ARG(d->out != d->q && d->out != d->k && d->out != d->v, "%s: out must not be an input", name);
+    return DBIR_OK;
+  }
+  CHECK_LAYOUT(dout, dout_stride, Lq, H, false);
+  CHECK_LAYOUT(dq, dq_stride, Lq, H, true);
+  CHECK_LAYOUT(dk, dk_stride, Lk, Hkv, true);
+  CHECK_LAYOUT(dv, dv_stride, Lk, Hkv, true);
+  const void *in[5] = {d->q, d->k, d->v, d->out, d->dout}, *to[3] = {d->dq, d->dk, d->dv};
+  for (int i = 0; i < 3; ++i) {
+    for (int j = 0; j < 5; ++j) DBIR_CHECK_ARG(to[i] != in[j], "%s: dq, dk, dv must not be inputs", name);
+    DBIR_CHECK_ARG(to[i] != to[(i + 1) % 3], "%s: dq, dk, dv must not be one tensor", name);
+  }
   return DBIR_OK;
 }
 
@@ -512,7 +531,9 @@ Args to_args(const dbir_attn_desc* d) {
   const long long* from[8] = {d->q_stride, d->k_stride, d->v_stride, d->out_stride, d->dout_stride, d->dq_stride, d->dk_stride, d->dv_stride};
   long long* to[8] = {a.qs, a.ks, a.vs, a.os, a.gs, a.dqs, a.dks, a.dvs};
   for (int i = 0; i < 8; ++i)
-    for (int j = 0; j < 3; ++j) to[i][j] = from[i][j];
+    for (int j = 0; j < 3; ++j) to[i][j] = from[i][j];   // (the row stride of one row is used for addresses that are not read)
+  if (d->Lq == 1) a.qs[1] = a.gs[1] = HD;
+  if (d->Lk == 1) a.ks[1] = a.vs[1] = HD;
   a.lse = d->lse; a.q_len = d->q_len; a.kv_len = d->kv_len;
   a.B = d->B; a.H = d->H; a.Hkv = d->Hkv; a.Lq = d->Lq; a.Lk = d->Lk; a.causal = d->causal; a.scale = d->scale;
   a.Lqp = (d->Lq + 63) / 64 * 64;
@@ -520,27 +541,27 @@ Args to_args(const dbir_attn_desc* d) {
 }
 
 // floats of the backward pass's workspace: nl2 | nd | gmax | vmax
-long long bwd_ws_floats(const dbir_attn_desc* d) {
-  const long long lqp = ((long long)d->Lq + 63) / 64 * 64, bh = (long long)d->B * d->H;
-  return bh * lqp * 2 + (d->dtype == DBIR_F16 ? bh * (lqp / 64) + (long long)d->B * d->Hkv * ((d->Lk + 63) / 64) : 0);
+long long bwd_ws_floats(int dtype, int B, int H, int Hkv, int Lq, int Lk) {
+  const long long lqp = ((long long)Lq + 63) / 64 * 64, bh = (long long)B * H;
+  return bh * lqp * 2 + (dtype == DBIR_F16 ? bh * (lqp / 64) + (long long)B * Hkv * ((Lk + 63) / 64) : 0);
 }
 
 }  // namespace
 
-extern "C" int dbir_attention_fwd_ws(const dbir_attn_desc* d, long long* bytes) {
-  DBIR_CHECK_ARG(d && bytes, "dbir_attention_fwd_ws: bad arguments");
+extern "C" int dbir_attention_fwd_ws(int dtype, int B, int H, int Hkv, int Lq, int Lk, long long* bytes) {
+  DBIR_CHECK_ARG(bytes && B > 0 && H > 0 && Hkv > 0 && Lq > 0 && Lk > 0, "dbir_attention_fwd_ws: bad arguments");
   *bytes = 0;
   return DBIR_OK;
 }
 
-extern "C" int dbir_attention_bwd_ws(const dbir_attn_desc* d, long long* bytes) {
-  DBIR_CHECK_ARG(d && bytes && d->B > 0 && d->H > 0 && d->Hkv > 0 && d->Lq > 0 && d->Lk > 0, "dbir_attention_bwd_ws: bad arguments");
-  *bytes = bwd_ws_floats(d) * 4;
+extern "C" int dbir_attention_bwd_ws(int dtype, int B, int H, int Hkv, int Lq, int Lk, long long* bytes) {
+  DBIR_CHECK_ARG(bytes && B > 0 && H > 0 && Hkv > 0 && Lq > 0 && Lk > 0, "dbir_attention_bwd_ws: bad arguments");
+  *bytes = bwd_ws_floats(dtype, B, H, Hkv, Lq, Lk) * 4;
   return DBIR_OK;
 }
 
 extern "C" int dbir_attention_fwd(const dbir_attn_desc* d, void* stream) {
-  if (int rc = check_desc(d, "dbir_attention_fwd")) return rc;
+  if (int rc = check_desc(d, "dbir_attention_fwd", false)) return rc;
   const Args a = to_args(d);
   const dim3 grid((unsigned)(cdiv(d->Lq, 128) * d->B * d->H));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
@@ -552,13 +573,10 @@ extern "C" int dbir_attention_fwd(const dbir_attn_desc* d, void* stream) {
 
 extern "C" int dbir_attention_bwd(const dbir_attn_desc* d, void* stream) {
   const char* name = "dbir_attention_bwd";
-  if (int rc = check_desc(d, name)) return rc;
-  CHECK_LAYOUT(dout, dout_stride, d->Lq);
-  CHECK_LAYOUT(dq, dq_stride, d->Lq);
-  CHECK_LAYOUT(dk, dk_stride, d->Lk);
-  CHECK_LAYOUT(dv, dv_stride, d->Lk);
-  DBIR_CHECK_ARG(d->ws && d->ws_bytes >= bwd_ws_floats(d) * 4 && (reinterpret_cast<uintptr_t>(d->ws) & 15) == 0,
-                 "%s: the workspace must hold %lld bytes, 16-byte aligned", name, bwd_ws_floats(d) * 4);
+  if (int rc = check_desc(d, name, true)) return rc;
+  const long long need = bwd_ws_floats(d->dtype, d->B, d->H, d->Hkv, d->Lq, d->Lk) * 4;
+  DBIR_CHECK_ARG(d->ws && d->ws_bytes >= need && (reinterpret_cast<uintptr_t>(d->ws) & 15) == 0,
+                 "%s: the workspace must hold %lld bytes, 16-byte aligned", name, need);
   Args a = to_args(d);
   const long long bh = (long long)d->B * d->H;
   const int f16 = d->dtype == DBIR_F16, nqb = a.Lqp / 64, nkb = cdiv(d->Lk, 64);

@@ -193,43 +193,68 @@ __global__ __launch_bounds__(256) void embed_piece_kernel(const typename T::elem
     if (col_of<V>(c0, lane, k) < W) part[(long long)piece * Wp + col_of<V>(c0, lane, k)] = acc[k];
 }
 
-// 32 rows of the table a workgroup, 8 a wave, one block of 256 columns
+// the sum of sorted positions [s, e) of one token: single ones up to the first whole piece, pieces, single ones again
 template <typename T, int V>
+__device__ __forceinline__ void add_run(const typename T::elem* dy, long long ldg, const int* spos, const float* part, int Wp, int s, int e, int c0, int lane,
+                                        int W, float* acc) {
+  const int ps = (s + RUN - 1) / RUN, pe = e / RUN;
+  if (ps < pe) {
+    add_items<T, V>(dy, ldg, spos, s, ps * RUN, c0, lane, W, acc);
+#pragma unroll 8
+    for (int p = ps; p < pe; ++p) add_row<F32T, V>(part + (long long)p * Wp, c0, lane, W, acc);
+    add_items<T, V>(dy, ldg, spos, pe * RUN, e, c0, lane, W, acc);
+  } else {
+    add_items<T, V>(dy, ldg, spos, s, e, c0, lane, W, acc);
+  }
+}
+__device__ __forceinline__ int first_at_least(const uint32_t* skey, int n, uint32_t v) {   // the first sorted position whose token is at least v
+  int lo = 0, hi = n;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (skey[mid] < v) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// SHARED: one row of the table a workgroup, its positions split over the four waves (small tables); else 32 rows, 8 a wave, most of them
+// empty.  One block of 256 columns either way.
+template <typename T, int V, bool SHARED>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const typename T::elem* __restrict__ dy, long long ldg, const uint32_t* __restrict__ skey,
                                                          const int* __restrict__ spos, const float* __restrict__ part, float* __restrict__ dtable,
                                                          long long ldd, float scale, int n, int W, int Wp, int vocab, int padding, int accumulate) {
-  __shared__ int first[33];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c0 = blockIdx.y * 256, v0 = blockIdx.x * 32;
-  if (threadIdx.x < 33) {   // the first sorted position whose token is at least v
-    const uint32_t v = (uint32_t)(v0 + threadIdx.x);
-    int lo = 0, hi = n;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (skey[mid] < v) lo = mid + 1;
-      else hi = mid;
-    }
-    first[threadIdx.x] = lo;
-  }
+  constexpr int ROWS = SHARED ? 1 : 32;
+  __shared__ int first[ROWS + 1];
+  __shared__ float join[SHARED ? 3 : 1][SHARED ? 256 : 1];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c0 = blockIdx.y * 256, v0 = blockIdx.x * ROWS;
+  if (threadIdx.x <= ROWS) first[threadIdx.x] = first_at_least(skey, n, (uint32_t)(v0 + threadIdx.x));
   __syncthreads();
-  if (V == 4 && c0 + lane * 4 >= W) return;
-  for (int r = wave * 8; r < wave * 8 + 8; ++r) {
+  const bool lane_ok = V == 1 || c0 + lane * 4 < W;
+  for (int r = SHARED ? 0 : wave * 8; r < (SHARED ? 1 : wave * 8 + 8); ++r) {
     const int v = v0 + r;
     if (v >= vocab) return;
-    const int s = __builtin_amdgcn_readfirstlane(first[r]), e = __builtin_amdgcn_readfirstlane(first[r + 1]);
+    int s = __builtin_amdgcn_readfirstlane(first[r]), e = __builtin_amdgcn_readfirstlane(first[r + 1]);
     const bool none = s == e || v == padding;
     if (none && accumulate) continue;
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
     if (!none) {
-      const int ps = (s + RUN - 1) / RUN, pe = e / RUN;
-      if (ps < pe) {
-        add_items<T, V>(dy, ldg, spos, s, ps * RUN, c0, lane, W, acc);
-#pragma unroll 8
-        for (int p = ps; p < pe; ++p) add_row<F32T, V>(part + (long long)p * Wp, c0, lane, W, acc);
-        add_items<T, V>(dy, ldg, spos, pe * RUN, e, c0, lane, W, acc);
-      } else {
-        add_items<T, V>(dy, ldg, spos, s, e, c0, lane, W, acc);
+      if (SHARED) {   // a quarter of the positions each, whole pieces where there are some
+        const int per = ((e - s + 3) / 4 + (e - s > 8 * RUN ? RUN - 1 : 0)) / (e - s > 8 * RUN ? RUN : 1) * (e - s > 8 * RUN ? RUN : 1);
+        s = min(e, s + wave * per);
+        e = min(e, s + per);
+      }
+      if (lane_ok) add_run<T, V>(dy, ldg, spos, part, Wp, s, e, c0, lane, W, acc);
+      if (SHARED) {
+        if (wave) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) join[wave - 1][k * 64 + lane] = acc[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] = (acc[k] + join[0][k * 64 + lane]) + (join[1][k * 64 + lane] + join[2][k * 64 + lane]);
       }
     }
+    if ((SHARED && wave) || !lane_ok) continue;
     float* d = dtable + (long long)v * ldd;
     if constexpr (V == 4) {
       float f[4] = {0.f, 0.f, 0.f, 0.f};
@@ -295,6 +320,7 @@ extern "C" int dbir_embedding_fwd(int table_dtype, const void* table, long long 
   DBIR_CHECK_ARG(table && tokens && out, "dbir_embedding_fwd: null pointer");
   DBIR_CHECK_ARG(n > 0 && n < (1 << 30) && L > 0 && W > 0 && vocab > 0 && ldt >= W && ldo >= W && (!pos || ldp >= W), "dbir_embedding_fwd: bad shape");
   DBIR_CHECK_ARG(table_dtype >= 0 && table_dtype <= 2 && out_dtype >= 0 && out_dtype <= 2, "dbir_embedding_fwd: bad dtype");
+  DBIR_CHECK_ARG(out != table && out != (const void*)pos, "dbir_embedding_fwd: out must not be an input");
   const bool v4 = W % 4 == 0 && al(table, ldt, elem4(table_dtype)) && al(out, ldo, elem4(out_dtype)) && (!pos || al(pos, ldp, 16));
   const int nv = v4 ? W / 4 : W;
   int lg = 0;
@@ -339,6 +365,7 @@ extern "C" int dbir_embedding_bwd(int dtype, const void* dy, long long ldg, cons
   DBIR_CHECK_ARG(n > 0 && n < (1 << 30) && L > 0 && n % L == 0 && W > 0 && vocab > 0 && ldg >= W && ldd >= W, "dbir_embedding_bwd: bad shape");
   DBIR_CHECK_ARG(pos_rows == 0 || (pos_rows >= L && pos_rows <= 65535), "dbir_embedding_bwd: pos_rows must be 0 or L .. 65535");
   DBIR_CHECK_ARG(dtype >= 0 && dtype <= 2, "dbir_embedding_bwd: bad dtype");
+  DBIR_CHECK_ARG(dtable != dy, "dbir_embedding_bwd: dtable must not be dy");
   DBIR_CHECK_ARG(cdiv(W, 1024) <= 65535, "dbir_embedding_bwd: W too large");
   const Plan p = plan_of(n, W, vocab);
   DBIR_CHECK_ARG(ws_bytes >= p.total * 4 && (reinterpret_cast<uintptr_t>(ws) & 15) == 0,
@@ -363,12 +390,17 @@ extern "C" int dbir_embedding_bwd(int dtype, const void* dy, long long ldg, cons
     }
   }
   const bool v4 = W % 4 == 0 && al(dy, ldg, elem4(dtype)) && al(dtable, ldd, 16);
-  const dim3 gp((unsigned)p.pieces, (unsigned)cdiv(W, 1024)), gr((unsigned)cdiv(vocab, 32), (unsigned)cdiv(W, 256)), gl((unsigned)cdiv(W, 256), (unsigned)pos_rows);
+  const bool shared = vocab <= 8 * 1024;   // below, 32 rows a workgroup do not fill the chip
+  const dim3 gp((unsigned)p.pieces, (unsigned)cdiv(W, 1024)), gr((unsigned)(shared ? vocab : cdiv(vocab, 32)), (unsigned)cdiv(W, 256)), gl((unsigned)cdiv(W, 256), (unsigned)pos_rows);
 #define GO2(T, V)                                                                                                                                \
   do {                                                                                                                                           \
     if (p.pieces) hipLaunchKernelGGL((embed_piece_kernel<T, V>), gp, dim3(256), 0, s, (const T::elem*)dy, ldg, key[at], pos[at], part, W, p.Wp);  \
-    hipLaunchKernelGGL((embed_rows_kernel<T, V>), gr, dim3(256), 0, s, (const T::elem*)dy, ldg, key[at], pos[at], part, dtable, ldd, scale, n, W, \
-                       p.Wp, vocab, padding_idx, accumulate);                                                                                    \
+    if (shared)                                                                                                                                  \
+      hipLaunchKernelGGL((embed_rows_kernel<T, V, true>), gr, dim3(256), 0, s, (const T::elem*)dy, ldg, key[at], pos[at], part, dtable, ldd,      \
+                         scale, n, W, p.Wp, vocab, padding_idx, accumulate);                                                                     \
+    else                                                                                                                                         \
+      hipLaunchKernelGGL((embed_rows_kernel<T, V, false>), gr, dim3(256), 0, s, (const T::elem*)dy, ldg, key[at], pos[at], part, dtable, ldd,     \
+                         scale, n, W, p.Wp, vocab, padding_idx, accumulate);                                                                     \
     if (pos_rows) hipLaunchKernelGGL((embed_pos_kernel<T, V>), gl, dim3(256), 0, s, (const T::elem*)dy, ldg, dpos, n / L, L, W);                  \
   } while (0)
 #define GO(T)          \

@@ -12,19 +12,27 @@ namespace {
 
 struct F32T {
   typedef float elem;
+  static constexpr int wide = 4;   // elements of 16 bytes
   static __device__ __forceinline__ float load(const float* p) { return *p; }
   static __device__ __forceinline__ void store(float* p, float v) { *p = v; }
+  static __device__ __forceinline__ void unpack(const uint4& v, float* f) {
+    f[0] = __builtin_bit_cast(float, v.x); f[1] = __builtin_bit_cast(float, v.y); f[2] = __builtin_bit_cast(float, v.z); f[3] = __builtin_bit_cast(float, v.w);
+  }
+  static __device__ __forceinline__ uint4 pack(const float* f) {
+    return make_uint4(__builtin_bit_cast(uint32_t, f[0]), __builtin_bit_cast(uint32_t, f[1]), __builtin_bit_cast(uint32_t, f[2]), __builtin_bit_cast(uint32_t, f[3]));
+  }
 };
-struct F16T {
+template <typename T>
+struct H16T {
   typedef u16 elem;
-  static __device__ __forceinline__ float load(const u16* p) { return F16::to_f32(*p); }
-  static __device__ __forceinline__ void store(u16* p, float v) { *p = F16::from_f32(v); }
+  static constexpr int wide = 8;
+  static __device__ __forceinline__ float load(const u16* p) { return T::to_f32(*p); }
+  static __device__ __forceinline__ void store(u16* p, float v) { *p = T::from_f32(v); }
+  static __device__ __forceinline__ void unpack(const uint4& v, float* f) { unpack8<T>(v, f); }
+  static __device__ __forceinline__ uint4 pack(const float* f) { return pack8<T>(f); }
 };
-struct BF16T {
-  typedef u16 elem;
-  static __device__ __forceinline__ float load(const u16* p) { return BF16::to_f32(*p); }
-  static __device__ __forceinline__ void store(u16* p, float v) { *p = BF16::from_f32(v); }
-};
+typedef H16T<F16> F16T;
+typedef H16T<BF16> BF16T;
 
 __device__ __forceinline__ float block_sum(float v, float* red) {   // 256 threads
   v = wave_sum(v);
@@ -34,7 +42,191 @@ __device__ __forceinline__ float block_sum(float v, float* red) {   // 256 threa
   return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// Any C, any alignment: a workgroup a row, element by element.
+// Rows held in registers: LPR lanes a row, VPL vectors of V elements a lane (V = 16 bytes' worth, or 1 where the rows are not aligned for
+// that), vector v = lane + LPR i.  A group goes through rows `step` apart with gamma (beta) and the column sums in its registers.
+// Every byte is read once: the bound is memory (figures at the host rule below).
+template <typename T, int V>
+__device__ __forceinline__ void load_vec(const typename T::elem* p, float* f) {
+  if constexpr (V == 1) f[0] = T::load(p);
+  else T::unpack(*reinterpret_cast<const uint4*>(p), f);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(typename T::elem* p, const float* f) {
+  if constexpr (V == 1) T::store(p, f[0]);
+  else *reinterpret_cast<uint4*>(p) = T::pack(f);
+}
+template <int LPR>
+__device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+  for (int o = (LPR > 64 ? 64 : LPR) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+// two sums over the lanes of a row; with four waves a row through `red`, whose halves are used in turn (one barrier a call)
+template <int LPR>
+__device__ __forceinline__ void row_sum2(float& a, float& b, float (*red)[8], int& turn) {
+  a = row_sum<LPR>(a);
+  b = row_sum<LPR>(b);
+  if constexpr (LPR == 256) {
+    float* r = red[turn];
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0) {
+      r[threadIdx.x >> 6] = a;
+      r[4 + (threadIdx.x >> 6)] = b;
+    }
+    __syncthreads();
+    a = (r[0] + r[1]) + (r[2] + r[3]);
+    b = (r[4] + r[5]) + (r[6] + r[7]);
+  }
+}
+
+template <typename T, int V, int LPR, int VPL>
+__global__ __launch_bounds__(256) void ln_fwd_kernel(const typename T::elem* __restrict__ x, long long ldx, typename T::elem* __restrict__ y, long long ldy,
+                                                     const float* __restrict__ gamma, const float* __restrict__ beta, float* __restrict__ stats, int rows,
+                                                     int C, float eps) {
+  constexpr int GROUPS = 256 / LPR;
+  __shared__ float red[2][8];
+  const int l = threadIdx.x % LPR, nv = C / V, step = gridDim.x * GROUPS;
+  int turn = 0;
+  float g[VPL][V], b[VPL][V];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      const bool ok = l + LPR * i < nv;
+      g[i][e] = ok ? gamma[(l + LPR * i) * V + e] : 0.f;
+      b[i][e] = ok ? beta[(l + LPR * i) * V + e] : 0.f;
+    }
+  for (int row = blockIdx.x * GROUPS + threadIdx.x / LPR; row < rows; row += step) {   // (LPR = 256: the same for the whole workgroup)
+    const typename T::elem* xr = x + (long long)row * ldx;
+    float f[VPL][V], s = 0.f, q = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      if (l + LPR * i < nv) {
+        load_vec<T, V>(xr + (l + LPR * i) * V, f[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[i][e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) s += f[i][e];
+    }
+    row_sum2<LPR>(s, q, red, turn);
+    const float mean = s / (float)C;
+    q = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        f[i][e] -= mean;
+        q += l + LPR * i < nv ? f[i][e] * f[i][e] : 0.f;
+      }
+    float z = 0.f;
+    row_sum2<LPR>(q, z, red, turn);
+    const float rstd = 1.f / sqrtf(q / (float)C + eps);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (l + LPR * i < nv) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[i][e] = __builtin_fmaf(f[i][e] * rstd, g[i][e], b[i][e]);
+        store_vec<T, V>(y + (long long)row * ldy + (l + LPR * i) * V, f[i]);
+      }
+    if (l == 0) *reinterpret_cast<float2*>(stats + 2LL * row) = make_float2(mean, rstd);
+  }
+}
+
+// dx, and this workgroup's sums of the columns: part[workgroup][0][c] = sum dy xh, [1][c] = sum dy
+template <typename T, int V, int LPR, int VPL>
+__global__ __launch_bounds__(256) void ln_bwd_kernel(const typename T::elem* __restrict__ dy, long long ldg, const typename T::elem* __restrict__ x,
+                                                     long long ldx, const typename T::elem* __restrict__ dres, long long ldr,
+                                                     typename T::elem* __restrict__ dx, long long ldd, const float* __restrict__ gamma,
+                                                     const float* __restrict__ stats, float* __restrict__ part, int rows, int C) {
+  constexpr int GROUPS = 256 / LPR, WAVES = LPR == 256 ? 1 : 4;   // waves that hold the same columns
+  __shared__ float red[2][8];
+  __shared__ float cols[WAVES > 1 ? 3 * 64 * V : 1];
+  const int l = threadIdx.x % LPR, nv = C / V, step = gridDim.x * GROUPS;
+  const float inv = 1.f / (float)C;
+  int turn = 0;
+  float g[VPL][V], sg[VPL][V], sb[VPL][V];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      g[i][e] = l + LPR * i < nv ? gamma[(l + LPR * i) * V + e] : 0.f;
+      sg[i][e] = sb[i][e] = 0.f;
+    }
+  for (int row = blockIdx.x * GROUPS + threadIdx.x / LPR; row < rows; row += step) {
+    const float2 st = *reinterpret_cast<const float2*>(stats + 2LL * row);
+    float xh[VPL][V], d[VPL][V], r[VPL][V], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int c = (l + LPR * i) * V;
+      if (l + LPR * i < nv) {
+        load_vec<T, V>(x + (long long)row * ldx + c, xh[i]);
+        load_vec<T, V>(dy + (long long)row * ldg + c, d[i]);
+        if (dres) load_vec<T, V>(dres + (long long)row * ldr + c, r[i]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) xh[i][e] = d[i][e] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        xh[i][e] = (xh[i][e] - st.x) * st.y;
+        sg[i][e] = __builtin_fmaf(d[i][e], xh[i][e], sg[i][e]);
+        sb[i][e] += d[i][e];
+        d[i][e] *= g[i][e];
+        s1 += d[i][e];
+        s2 = __builtin_fmaf(d[i][e], xh[i][e], s2);   // (lanes without a column: d = 0)
+      }
+    row_sum2<LPR>(s1, s2, red, turn);
+    s1 *= inv;
+    s2 *= inv;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (l + LPR * i < nv) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          d[i][e] = st.y * (d[i][e] - __builtin_fmaf(xh[i][e], s2, s1));
+          if (dres) d[i][e] += r[i][e];
+        }
+        store_vec<T, V>(dx + (long long)row * ldd + (l + LPR * i) * V, d[i]);
+      }
+  }
+  float* out = part + (long long)blockIdx.x * 2 * C;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i)
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      float t[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        t[e] = which ? sb[i][e] : sg[i][e];
+#pragma unroll
+        for (int o = LPR; o < 64; o <<= 1) t[e] += __shfl_xor(t[e], o, 64);
+      }
+      if constexpr (WAVES > 1) {
+        const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+        __syncthreads();
+        if (wave) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) cols[((wave - 1) * V + e) * 64 + lane] = t[e];
+        }
+        __syncthreads();
+        if (wave == 0) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) t[e] += cols[e * 64 + lane] + (cols[(V + e) * 64 + lane] + cols[(2 * V + e) * 64 + lane]);
+        }
+      }
+      if ((int)threadIdx.x < LPR && l + LPR * i < nv) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) out[which * C + (l + LPR * i) * V + e] = t[e];
+      }
+    }
+}
+
+// Wider rows than registers hold: a workgroup a row, element by element, read again where it is needed again.
 template <typename T>
 __global__ __launch_bounds__(256) void ln_fwd_any_kernel(const typename T::elem* __restrict__ x, long long ldx, typename T::elem* __restrict__ y,
                                                          long long ldy, const float* __restrict__ gamma, const float* __restrict__ beta,
@@ -100,19 +292,21 @@ __global__ __launch_bounds__(256) void ln_cols_any_kernel(const typename T::elem
   part[(long long)blockIdx.y * 2 * C + C + c] = b;
 }
 
-// sums of `n` partial rows of 2 C columns: 32 columns a workgroup, 8 threads a column
+// sums of `n` partial rows of 2 C columns: 16 columns a workgroup, 16 threads a column
 __global__ __launch_bounds__(256) void ln_join_kernel(const float* __restrict__ part, int n, int C, float* __restrict__ dgamma, float* __restrict__ dbeta) {
-  __shared__ float red[8][32];
-  const int lane = threadIdx.x & 31, sl = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+  __shared__ float red[16][17];
+  const int lane = threadIdx.x & 15, sl = threadIdx.x >> 4, c = blockIdx.x * 16 + lane;
   float s = 0.f;
-  if (c < 2 * C)
-    for (int i = sl; i < n; i += 8) s += part[(long long)i * 2 * C + c];
+  if (c < 2 * C) {
+#pragma unroll 8
+    for (int i = sl; i < n; i += 16) s += part[(long long)i * 2 * C + c];
+  }
   red[sl][lane] = s;
   __syncthreads();
   if (sl == 0 && c < 2 * C) {
     s = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s += red[i][lane];
+    for (int i = 0; i < 16; ++i) s += red[i][lane];
     if (c < C) dgamma[c] = s;
     else dbeta[c - C] = s;
   }
@@ -123,29 +317,106 @@ int any_chunks(int rows, int C) {   // partial rows: about 2048 workgroups over 
   return n < want ? n : (want < 1 ? 1 : want);
 }
 
+// How a row is laid over lanes: by its vectors (wide: all rows 16-byte aligned) or single elements.
+struct Shape {
+  int v, lpr, vpl;   // v = 0: too wide for registers
+};
+Shape shape_of(int dtype, int C, bool wide) {
+  const int v = wide ? (dtype == DBIR_F32 ? 4 : 8) : 1, nv = C / v;
+  if (!wide) return nv <= 256 ? Shape{1, 64, 4} : nv <= 2048 ? Shape{1, 256, 8} : nv <= 4096 ? Shape{1, 256, 16} : Shape{0, 0, 0};
+  return nv <= 8 ? Shape{v, 8, 1} : nv <= 32 ? Shape{v, 32, 1} : nv <= 64 ? Shape{v, 32, 2} : nv <= 128 ? Shape{v, 64, 2} : nv <= 192 ? Shape{v, 64, 3} :
+         nv <= 320 ? Shape{v, 64, 5} : nv <= 512 ? Shape{v, 256, 2} : nv <= 1024 ? Shape{v, 256, 4} : Shape{0, 0, 0};
+}
+bool is_wide(int dtype, int C, const void* p, long long ld) {
+  const int v = dtype == DBIR_F32 ? 4 : 8;
+  return C % v == 0 && ld % v == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
+// workgroups of the backward pass = partial rows of the column sums: one row a group up to 512 workgroups (two a CU), then more rows a group
+int bwd_groups(int rows, const Shape& sh) {
+  const int n = cdiv(rows, 256 / sh.lpr);
+  return n < 512 ? n : 512;
+}
+int bwd_parts(int dtype, int rows, int C, bool wide) {
+  const Shape sh = shape_of(dtype, C, wide);
+  return sh.v ? bwd_groups(rows, sh) : any_chunks(rows, C);
+}
+
+#define EACH_SHAPE(GO, T)                                                                              \
+  do {                                                                                                 \
+    if (sh.v > 1) {                                                                                    \
+      if (sh.lpr == 8) GO(T, T::wide, 8, 1);                                                           \
+      else if (sh.lpr == 32 && sh.vpl == 1) GO(T, T::wide, 32, 1);                                     \
+      else if (sh.lpr == 32) GO(T, T::wide, 32, 2);                                                    \
+      else if (sh.lpr == 64 && sh.vpl == 2) GO(T, T::wide, 64, 2);                                     \
+      else if (sh.lpr == 64 && sh.vpl == 3) GO(T, T::wide, 64, 3);                                     \
+      else if (sh.lpr == 64) GO(T, T::wide, 64, 5);                                                    \
+      else if (sh.vpl == 2) GO(T, T::wide, 256, 2);                                                    \
+      else GO(T, T::wide, 256, 4);                                                                     \
+    } else if (sh.lpr == 64) GO(T, 1, 64, 4);                                                          \
+    else if (sh.vpl == 8) GO(T, 1, 256, 8);                                                            \
+    else GO(T, 1, 256, 16);                                                                            \
+  } while (0)
+
+template <typename T>
+void launch_fwd(const Shape& sh, const void* x, long long ldx, void* y, long long ldy, const float* gamma, const float* beta, float* stats, int rows, int C,
+                float eps, hipStream_t s) {
+  typedef typename T::elem E;
+  if (!sh.v) {
+    hipLaunchKernelGGL(ln_fwd_any_kernel<T>, dim3((unsigned)rows), dim3(256), 0, s, (const E*)x, ldx, (E*)y, ldy, gamma, beta, stats, C, eps);
+    return;
+  }
+  const int n = cdiv(rows, 256 / sh.lpr);
+  const dim3 grid((unsigned)(n < 2048 ? n : 2048));
+#define GO(TT, V, LPR, VPL) \
+  hipLaunchKernelGGL((ln_fwd_kernel<TT, V, LPR, VPL>), grid, dim3(256), 0, s, (const E*)x, ldx, (E*)y, ldy, gamma, beta, stats, rows, C, eps)
+  EACH_SHAPE(GO, T);
+#undef GO
+}
+
+template <typename T>
+void launch_bwd(const Shape& sh, int n, const void* dy, long long ldg, const void* x, long long ldx, const void* dres, long long ldr, void* dx, long long ldd,
+                const float* gamma, const float* stats, float* ws, int rows, int C, hipStream_t s) {
+  typedef typename T::elem E;
+  if (!sh.v) {
+    hipLaunchKernelGGL(ln_bwd_any_kernel<T>, dim3((unsigned)rows), dim3(256), 0, s, (const E*)dy, ldg, (const E*)x, ldx, (const E*)dres, ldr, (E*)dx, ldd,
+                       gamma, stats, C);
+    hipLaunchKernelGGL(ln_cols_any_kernel<T>, dim3((unsigned)cdiv(C, 256), (unsigned)n), dim3(256), 0, s, (const E*)dy, ldg, (const E*)x, ldx, stats, ws,
+                       rows, C, cdiv(rows, n));
+    return;
+  }
+#define GO(TT, V, LPR, VPL)                                                                                                                            \
+  hipLaunchKernelGGL((ln_bwd_kernel<TT, V, LPR, VPL>), dim3((unsigned)n), dim3(256), 0, s, (const E*)dy, ldg, (const E*)x, ldx, (const E*)dres, ldr, (E*)dx, \
+                     ldd, gamma, stats, ws, rows, C)
+  EACH_SHAPE(GO, T);
+#undef GO
+}
+
 }  // namespace
 
 extern "C" int dbir_layernorm_bwd_ws(int rows, int C, long long* bytes) {
   DBIR_CHECK_ARG(rows > 0 && C > 0 && bytes, "dbir_layernorm_bwd_ws: bad arguments");
-  *bytes = 8LL * C * any_chunks(rows, C);
+  int n = 0;   // whatever type and alignment the call has
+  for (int dtype = 0; dtype < 3; ++dtype)
+    for (int wide = 0; wide < 2; ++wide) {
+      const int m = bwd_parts(dtype, rows, C, wide && C % (dtype == DBIR_F32 ? 4 : 8) == 0);
+      n = m > n ? m : n;
+    }
+  *bytes = 8LL * C * n;
   return DBIR_OK;
 }
 
 extern "C" int dbir_layernorm_fwd(int dtype, const void* x, long long ldx, void* y, long long ldy, const float* gamma, const float* beta,
                                   float* stats, int rows, int C, float eps, void* stream) {
   DBIR_CHECK_ARG(x && y && gamma && beta && stats, "dbir_layernorm_fwd: null pointer");
-  DBIR_CHECK_ARG(rows > 0 && C > 0 && ldx >= C && ldy >= C, "dbir_layernorm_fwd: bad rows / C / ld");
+  DBIR_CHECK_ARG(rows > 0 && rows <= (1 << 30) && C > 0 && ldx >= C && ldy >= C, "dbir_layernorm_fwd: bad rows / C / ld");
+  DBIR_CHECK_ARG(x != y, "dbir_layernorm_fwd: y must not be x");
+  DBIR_CHECK_ARG(dtype >= DBIR_F16 && dtype <= DBIR_F32, "dbir_layernorm_fwd: bad dtype %d", dtype);
+  DBIR_CHECK_ARG((reinterpret_cast<uintptr_t>(stats) & 7) == 0, "dbir_layernorm_fwd: stats must be 8-byte aligned");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-#define GO(T) \
-  hipLaunchKernelGGL(ln_fwd_any_kernel<T>, dim3((unsigned)rows), dim3(256), 0, s, (const T::elem*)x, ldx, (T::elem*)y, ldy, gamma, beta, stats, C, eps)
-  if (dtype == DBIR_F16) GO(F16T);
-  else if (dtype == DBIR_BF16) GO(BF16T);
-  else if (dtype == DBIR_F32) GO(F32T);
-  else {
-    dbir_set_error("dbir_layernorm_fwd: bad dtype %d", dtype);
-    return DBIR_ERR_ARG;
-  }
-#undef GO
+  const Shape sh = shape_of(dtype, C, is_wide(dtype, C, x, ldx) && is_wide(dtype, C, y, ldy));
+  if (dtype == DBIR_F16) launch_fwd<F16T>(sh, x, ldx, y, ldy, gamma, beta, stats, rows, C, eps, s);
+  else if (dtype == DBIR_BF16) launch_fwd<BF16T>(sh, x, ldx, y, ldy, gamma, beta, stats, rows, C, eps, s);
+  else launch_fwd<F32T>(sh, x, ldx, y, ldy, gamma, beta, stats, rows, C, eps, s);
   DBIR_CHECK_LAUNCH("dbir_layernorm_fwd");
   return DBIR_OK;
 }
@@ -154,26 +425,19 @@ extern "C" int dbir_layernorm_bwd(int dtype, const void* dy, long long ldg, cons
                                   void* dx, long long ldd, const float* gamma, const float* stats, float* dgamma, float* dbeta, int rows, int C,
                                   float* ws, long long ws_bytes, void* stream) {
   DBIR_CHECK_ARG(dy && x && dx && gamma && stats && dgamma && dbeta && ws, "dbir_layernorm_bwd: null pointer");
-  DBIR_CHECK_ARG(rows > 0 && C > 0 && ldg >= C && ldx >= C && ldd >= C && (!dres || ldr >= C), "dbir_layernorm_bwd: bad rows / C / ld");
-  const int n = any_chunks(rows, C), chunk = cdiv(rows, n);
+  DBIR_CHECK_ARG(rows > 0 && rows <= (1 << 30) && C > 0 && ldg >= C && ldx >= C && ldd >= C && (!dres || ldr >= C), "dbir_layernorm_bwd: bad rows / C / ld");
+  DBIR_CHECK_ARG(dx != x && dx != dy && dx != dres, "dbir_layernorm_bwd: dx must not be an input");
+  DBIR_CHECK_ARG(dtype >= DBIR_F16 && dtype <= DBIR_F32, "dbir_layernorm_bwd: bad dtype %d", dtype);
+  DBIR_CHECK_ARG(((reinterpret_cast<uintptr_t>(stats) & 7) | (reinterpret_cast<uintptr_t>(ws) & 3)) == 0, "dbir_layernorm_bwd: stats must be 8-byte aligned");
+  const bool wide = is_wide(dtype, C, dy, ldg) && is_wide(dtype, C, x, ldx) && is_wide(dtype, C, dx, ldd) && (!dres || is_wide(dtype, C, dres, ldr));
+  const Shape sh = shape_of(dtype, C, wide);
+  const int n = bwd_parts(dtype, rows, C, wide);
   DBIR_CHECK_ARG(ws_bytes >= 8LL * C * n, "dbir_layernorm_bwd: the workspace must hold %lld bytes", 8LL * C * n);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-#define GO(T)                                                                                                                                    \
-  do {                                                                                                                                           \
-    hipLaunchKernelGGL(ln_bwd_any_kernel<T>, dim3((unsigned)rows), dim3(256), 0, s, (const T::elem*)dy, ldg, (const T::elem*)x, ldx,              \
-                       (const T::elem*)dres, ldr, (T::elem*)dx, ldd, gamma, stats, C);                                                           \
-    hipLaunchKernelGGL(ln_cols_any_kernel<T>, dim3((unsigned)cdiv(C, 256), (unsigned)n), dim3(256), 0, s, (const T::elem*)dy, ldg,                \
-                       (const T::elem*)x, ldx, stats, ws, rows, C, chunk);                                                                       \
-  } while (0)
-  if (dtype == DBIR_F16) GO(F16T);
-  else if (dtype == DBIR_BF16) GO(BF16T);
-  else if (dtype == DBIR_F32) GO(F32T);
-  else {
-    dbir_set_error("dbir_layernorm_bwd: bad dtype %d", dtype);
-    return DBIR_ERR_ARG;
-  }
-#undef GO
-  hipLaunchKernelGGL(ln_join_kernel, dim3((unsigned)cdiv(2 * C, 32)), dim3(256), 0, s, ws, n, C, dgamma, dbeta);
+  if (dtype == DBIR_F16) launch_bwd<F16T>(sh, n, dy, ldg, x, ldx, dres, ldr, dx, ldd, gamma, stats, ws, rows, C, s);
+  else if (dtype == DBIR_BF16) launch_bwd<BF16T>(sh, n, dy, ldg, x, ldx, dres, ldr, dx, ldd, gamma, stats, ws, rows, C, s);
+  else launch_bwd<F32T>(sh, n, dy, ldg, x, ldx, dres, ldr, dx, ldd, gamma, stats, ws, rows, C, s);
+  hipLaunchKernelGGL(ln_join_kernel, dim3((unsigned)cdiv(2 * C, 16)), dim3(256), 0, s, ws, n, C, dgamma, dbeta);
   DBIR_CHECK_LAUNCH("dbir_layernorm_bwd");
   return DBIR_OK;
 }

@@ -58,8 +58,8 @@ _I, _LL, _F, _P = c_int, c_longlong, c_float, c_void_p
 SIGNATURES = {
     "dbir_gemm": [POINTER(GemmDesc), _P],
     "dbir_attention": [_I, _P, _LL, _LL, _P, _LL, _LL, _P, _LL, _LL, _P, _LL, _LL, _I, _I, _I, _I, _F, _P],
-    "dbir_attention_fwd_ws": [POINTER(AttnDesc), POINTER(c_longlong)], "dbir_attention_bwd_ws": [POINTER(AttnDesc), POINTER(c_longlong)],
-    "dbir_attention_fwd": [POINTER(AttnDesc), _P], "dbir_attention_bwd": [POINTER(AttnDesc), _P],
+    "dbir_attention_fwd_ws": [_I, _I, _I, _I, _I, _I, POINTER(c_longlong)], "dbir_attention_bwd_ws": [_I, _I, _I, _I, _I, _I, POINTER(c_longlong)],
+    "dbir_attention_fwd": [_P, _P], "dbir_attention_bwd": [_P, _P],   # (dbir_attn_desc*: an AttnDesc or its packed bytes)
     "dbir_layernorm_bwd_ws": [_I, _I, POINTER(c_longlong)],
     "dbir_layernorm_fwd": [_I, _P, _LL, _P, _LL, _P, _P, _P, _I, _I, _F, _P],
     "dbir_layernorm_bwd": [_I, _P, _LL, _P, _LL, _P, _LL, _P, _LL, _P, _P, _P, _P, _I, _I, _P, _LL, _P],

@@ -13,8 +13,9 @@ Conventions
 """
 import ctypes
 import os
-from contextlib import nullcontext
+import struct
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -672,108 +673,95 @@ def causal_attention(qkv: T, heads: int, scale: float) -> T:
 # Forward passes that keep what the backward pass needs, and the backward passes (include/dbir.h "Training operators").  Plain
 # functions like everything here: a caller who wants torch.autograd wraps them in its own Function.  Results do not depend on
 # the run (no floating-point atomics); workspaces are allocated per call, so calls on several streams and calls captured into
-# several graphs share nothing.
-def _need(ok: bool, msg: str) -> None:
-    if not ok:
-        raise ValueError(msg)
+# several graphs share nothing.  At the small end a call is its host time: the checks are one condition each, strides, overlaps
+# and sizes are checked by the C entry, and workspace sizes are remembered by shape.
+_DT3 = {torch.float16: native.F16, torch.bfloat16: native.BF16, torch.float32: native.F32}
+_ATTN_PACK = struct.Struct("@7if12Pq24q").pack   # dbir_attn_desc (native.AttnDesc)
 
 
-def _train_args(what: str, *ts) -> torch.device:
-    """Every tensor on one GPU, and no plan being recorded: a replay would miss these calls."""
-    _gpu(*ts)
-    _need(not plan.recording(), f"{what}: training operators cannot be part of a recorded evaluation")
-    dev = ts[0].device
-    for t in ts:
-        _need(t is None or t.device == dev, f"{what}: tensors on different devices ({dev}, {getattr(t, 'device', None)})")
+def _train_device(what: str, first: T, *others) -> int:
+    """The GPU that every tensor is on; no plan being recorded (its replay would miss these calls)."""
+    dev = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            _gpu(first, t)
+            raise ValueError(f"{what}: tensors on different devices ({first.device}, {t.device})")
+    if dev < 0:
+        _gpu(first)
+    if plan.recording():
+        raise ValueError(f"{what}: training operators cannot be part of a recorded evaluation")
     return dev
 
 
-def _on(dev: torch.device):
-    """Launches go to the current stream of the tensors' device."""
-    return nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+def _train_call(name: str, dev: int, *args) -> None:
+    """The C entry on the current stream of the tensors' device."""
+    fn = getattr(native.lib(), name)
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, _stream())
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream())
+    if rc:
+        native.check(rc, name)
 
 
-def _dt3(t: T) -> int:
-    return native.F32 if t.dtype == torch.float32 else _dt(t)
+@lru_cache(maxsize=1024)
+def _ws_bytes(name: str, *args) -> int:
+    n = ctypes.c_longlong()
+    native.check(getattr(native.lib(), name)(*args, ctypes.byref(n)), name)
+    return n.value
 
 
 def _row_ld(t: T, what: str) -> int:
     """Row stride of [..., C] whose rows lie evenly apart."""
     C = t.shape[-1]
-    _need(C == 1 or t.stride(-1) == 1, f"{what}: the last dimension must have unit stride")
-    ld, span = None, 0
+    if t.is_contiguous():
+        return C
+    ld, span, even = None, 0, C == 1 or t.stride(-1) == 1
     for n, st in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
         if n > 1:
             if ld is None:
                 ld, span = st, st * n
             else:
-                _need(st == span, f"{what}: the rows must lie evenly apart, got shape {tuple(t.shape)} strides {t.stride()}")
-                span = st * n
-    _need(ld is None or ld >= C, f"{what}: the rows overlap, got shape {tuple(t.shape)} strides {t.stride()}")
-    return C if ld is None else ld
+                even, span = even and st == span, st * n
+    ld = C if ld is None else ld
+    if not even or ld < C:
+        raise ValueError(f"{what}: the rows must lie evenly apart with unit stride inside, got shape {tuple(t.shape)} strides {t.stride()}")
+    return ld
 
 
-def _f32_vec(t: T, n: int, what: str) -> None:
-    _need(t.dtype == torch.float32 and t.numel() == n and t.is_contiguous(), f"{what}: expected {n} contiguous f32 values")
-
-
-def _apart(what: str, outs, ins) -> None:
-    """No output may be an input or another output (the backward passes read their inputs more than once)."""
-    ptrs = [t.data_ptr() for t in outs]
-    _need(len(set(ptrs)) == len(ptrs) and not set(ptrs) & {t.data_ptr() for t in ins if t is not None},
-          f"{what}: outputs must not share memory with inputs or each other")
-
-
-def _strides(t: T):
-    """Batch, row and head stride of [B, L, H, 64]; a dimension of one row has no stride."""
-    st = t.stride()
-    return (st[0] if t.shape[0] > 1 else 0, st[1] if t.shape[1] > 1 else 64, st[2] if t.shape[2] > 1 else 0)
-
-
-def _attn_desc(what: str, q: T, k: T, v: T, out: T, lse: T, scale, causal, q_len, kv_len, dout=None, dq=None, dk=None, dv=None):
-    B, Lq, H, _ = q.shape
-    Lk, Hkv = k.shape[1], k.shape[2]
-    for name, t, shape in (("q", q, (B, Lq, H, 64)), ("k", k, (B, Lk, Hkv, 64)), ("v", v, (B, Lk, Hkv, 64)), ("out", out, (B, Lq, H, 64)),
-                           ("dout", dout, (B, Lq, H, 64)), ("dq", dq, (B, Lq, H, 64)), ("dk", dk, (B, Lk, Hkv, 64)), ("dv", dv, (B, Lk, Hkv, 64))):
-        if t is not None:
-            _need(tuple(t.shape) == shape, f"{what}: {name} must have shape {shape}, got {tuple(t.shape)}")
-            _need(t.dtype == q.dtype, f"{what}: {name} is {t.dtype}, q is {q.dtype}")
-            _need(t.stride(3) == 1, f"{what}: {name}: the head dimension must have unit stride")
-    for name, t in (("out", out if dout is None else None), ("dq", dq), ("dk", dk), ("dv", dv)):
-        _need(t is None or all(n == 1 or st for n, st in zip(t.shape, t.stride())), f"{what}: {name} must not be an expanded tensor")
-    for name, t in (("q_len", q_len), ("kv_len", kv_len)):
-        _need(t is None or (t.dtype == torch.int32 and tuple(t.shape) == (B,) and t.is_contiguous()), f"{what}: {name} must be int32 [{B}]")
-    _need(lse.dtype == torch.float32 and tuple(lse.shape) == (B, H, Lq) and lse.is_contiguous(), f"{what}: lse must be contiguous f32 [{B}, {H}, {Lq}]")
-    p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    s3 = lambda t: (0, 0, 0) if t is None else _strides(t)  # noqa: E731
-    return native.AttnDesc(_dt(q), B, H, Hkv, Lq, Lk, int(bool(causal)), float(scale), p(q), p(k), p(v), p(out), p(lse), p(q_len), p(kv_len),
-                           p(dout), p(dq), p(dk), p(dv), None, 0, s3(q), s3(k), s3(v), s3(out), s3(dout), s3(dq), s3(dk), s3(dv))
-
-
-def _attn_run(name: str, d, dev) -> None:
-    nbytes = ctypes.c_longlong()
-    native.check(getattr(native.lib(), name + "_ws")(ctypes.byref(d), ctypes.byref(nbytes)), name + "_ws")
-    if nbytes.value:
-        ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
-        d.ws, d.ws_bytes = ws.data_ptr(), nbytes.value
-    native.check(getattr(native.lib(), name)(ctypes.byref(d), _stream()), name)
+def _attn_lens(what: str, B: int, q_len: Optional[T], kv_len: Optional[T]):
+    for t in (q_len, kv_len):
+        if t is not None and not (t.dtype == torch.int32 and t.shape == (B,) and t.is_contiguous()):
+            raise ValueError(f"{what}: q_len / kv_len must be contiguous int32 [{B}]")
+    return (0 if q_len is None else q_len.data_ptr()), (0 if kv_len is None else kv_len.data_ptr())
 
 
 def attention_fwd(q: T, k: T, v: T, scale: float, causal: bool = False, q_len: Optional[T] = None, kv_len: Optional[T] = None,
                   out: Optional[T] = None) -> Tuple[T, T]:
     """softmax(scale q k^T) v for training -> (out [B, Lq, H, 64], lse f32 [B, H, Lq]).  q: [B, Lq, H, 64], k / v: [B, Lk, Hkv, 64]
-    16-bit views with any strides that are multiples of 8 (heads are shared by H / Hkv queries' heads); causal: query i sees keys
+    16-bit views with any strides that are multiples of 8 (a key head serves H / Hkv query heads); causal: query i sees keys
     j <= i + Lk - Lq; q_len / kv_len: int32 [B] lengths of a padded batch: what lies behind is not read, out is zero there.  A row
     that sees no key gives zeros and lse = -inf."""
-    dev = _train_args("attention_fwd", q, k, v, out, q_len, kv_len)
-    _need(q.dim() == 4 and k.dim() == 4 and v.dim() == 4 and q.shape[3] == 64, "attention_fwd: q, k, v must be [B, L, heads, 64]")
+    dev = _train_device("attention_fwd", q, k, v, out, q_len, kv_len)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32, device=dev)
-    d = _attn_desc("attention_fwd", q, k, v, out, lse, scale, causal, q_len, kv_len)
-    _apart("attention_fwd", (out,), (q, k, v))
-    with _on(dev):
-        _attn_run("dbir_attention_fwd", d, dev)
+        out = torch.empty_like(q)
+    qs, ks, dt = q.shape, k.shape, q.dtype
+    if len(qs) != 4 or len(ks) != 4 or qs[3] != 64 or ks[3] != 64 or ks[0] != qs[0] or v.shape != ks or out.shape != qs:
+        raise ValueError(f"attention_fwd: q, out must be [B, Lq, H, 64] and k, v [B, Lk, Hkv, 64], got {[tuple(t.shape) for t in (q, out, k, v)]}")
+    if k.dtype != dt or v.dtype != dt or out.dtype != dt:
+        raise TypeError("attention_fwd: q, k, v, out must have one type")
+    sq, sk, sv, so = q.stride(), k.stride(), v.stride(), out.stride()
+    if not sq[3] == sk[3] == sv[3] == so[3] == 1:
+        raise ValueError("attention_fwd: the head dimension must have unit stride")
+    B, Lq, H, _ = qs
+    lens = _attn_lens("attention_fwd", B, q_len, kv_len)
+    lse = torch.empty((B, H, Lq), dtype=torch.float32, device=q.device)
+    nws = _ws_bytes("dbir_attention_fwd_ws", _dt(q), B, H, ks[2], Lq, ks[1])
+    ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
+    _train_call("dbir_attention_fwd", dev, _ATTN_PACK(
+        _dt(q), B, H, ks[2], Lq, ks[1], bool(causal), scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), *lens,
+        0, 0, 0, 0, ws.data_ptr() if nws else 0, nws, *sq[:3], *sk[:3], *sv[:3], *so[:3], 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0))
     return out, lse
 
 
@@ -781,78 +769,98 @@ def attention_bwd(dout: T, q: T, k: T, v: T, out: T, lse: T, scale: float, causa
                   kv_len: Optional[T] = None, dq: Optional[T] = None, dk: Optional[T] = None, dv: Optional[T] = None) -> Tuple[T, T, T]:
     """Gradients (dq, dk, dv) of attention_fwd, shaped like q, k, v, from its out and lse and the same mask arguments; the probabilities
     are recomputed.  dk / dv are sums over the query heads that share them; rows behind a length get zeros."""
-    dev = _train_args("attention_bwd", dout, q, k, v, out, lse, q_len, kv_len, dq, dk, dv)
-    _need(q.dim() == 4 and k.dim() == 4 and v.dim() == 4 and q.shape[3] == 64, "attention_bwd: q, k, v must be [B, L, heads, 64]")
-    dq = torch.empty(q.shape, dtype=q.dtype, device=dev) if dq is None else dq
-    dk = torch.empty(k.shape, dtype=q.dtype, device=dev) if dk is None else dk
-    dv = torch.empty(v.shape, dtype=q.dtype, device=dev) if dv is None else dv
-    d = _attn_desc("attention_bwd", q, k, v, out, lse, scale, causal, q_len, kv_len, dout, dq, dk, dv)
-    _apart("attention_bwd", (dq, dk, dv), (q, k, v, out, dout))
-    with _on(dev):
-        _attn_run("dbir_attention_bwd", d, dev)
+    dev = _train_device("attention_bwd", q, k, v, dout, out, lse, q_len, kv_len, dq, dk, dv)
+    if dq is None:
+        dq = torch.empty_like(q)
+    if dk is None:
+        dk = torch.empty_like(k)
+    if dv is None:
+        dv = torch.empty_like(v)
+    qs, ks, dt = q.shape, k.shape, q.dtype
+    if len(qs) != 4 or len(ks) != 4 or qs[3] != 64 or ks[3] != 64 or ks[0] != qs[0] or not (v.shape == dk.shape == dv.shape == ks) or \
+            not (out.shape == dout.shape == dq.shape == qs):
+        raise ValueError("attention_bwd: q, out, dout, dq must be [B, Lq, H, 64] and k, v, dk, dv [B, Lk, Hkv, 64], got "
+                         f"{[tuple(t.shape) for t in (q, out, dout, dq, k, v, dk, dv)]}")
+    if not (k.dtype == v.dtype == out.dtype == dout.dtype == dq.dtype == dk.dtype == dv.dtype == dt):
+        raise TypeError("attention_bwd: all tensors but lse must have one type")
+    B, Lq, H, _ = qs
+    if lse.dtype != torch.float32 or lse.shape != (B, H, Lq) or not lse.is_contiguous():
+        raise ValueError(f"attention_bwd: lse must be contiguous f32 [{B}, {H}, {Lq}]")
+    st = [t.stride() for t in (q, k, v, out, dout, dq, dk, dv)]
+    if not all(x[3] == 1 for x in st):
+        raise ValueError("attention_bwd: the head dimension must have unit stride")
+    lens = _attn_lens("attention_bwd", B, q_len, kv_len)
+    nws = _ws_bytes("dbir_attention_bwd_ws", _dt(q), B, H, ks[2], Lq, ks[1])
+    ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
+    _train_call("dbir_attention_bwd", dev, _ATTN_PACK(
+        _dt(q), B, H, ks[2], Lq, ks[1], bool(causal), scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), *lens,
+        dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), nws, *[n for x in st for n in x[:3]]))
     return dq, dk, dv
 
 
 def layernorm_fwd(x: T, gamma: T, beta: T, eps: float = 1e-5, out: Optional[T] = None) -> Tuple[T, T]:
     """LayerNorm over the last dimension for training -> (y, stats f32 [..., 2] = mean | 1 / sigma).  x f16 / bf16 / f32, any width;
     gamma / beta f32 [C]."""
-    dev = _train_args("layernorm_fwd", x, gamma, beta, out)
-    C = x.shape[-1]
-    out = torch.empty(x.shape, dtype=x.dtype, device=dev) if out is None else out
-    _need(out.shape == x.shape and out.dtype == x.dtype, "layernorm_fwd: out must be like x")
-    _f32_vec(gamma, C, "layernorm_fwd: gamma")
-    _f32_vec(beta, C, "layernorm_fwd: beta")
-    _apart("layernorm_fwd", (out,), (x,))
-    stats = torch.empty(x.shape[:-1] + (2,), dtype=torch.float32, device=dev)
-    with _on(dev):
-        native.check(native.lib().dbir_layernorm_fwd(_dt3(x), x.data_ptr(), _row_ld(x, "layernorm_fwd: x"), out.data_ptr(),
-                                                     _row_ld(out, "layernorm_fwd: out"), gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(),
-                                                     _rows(x), C, eps, _stream()), "dbir_layernorm_fwd")
+    dev = _train_device("layernorm_fwd", x, gamma, beta, out)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    shape, dt = x.shape, _DT3.get(x.dtype)
+    C = shape[-1]
+    if dt is None or out.dtype != x.dtype or gamma.dtype != torch.float32 or beta.dtype != torch.float32:
+        raise TypeError("layernorm_fwd: x and out must have one type (f16, bf16 or f32), gamma and beta f32")
+    if out.shape != shape or gamma.shape != (C,) or beta.shape != (C,) or not gamma.is_contiguous() or not beta.is_contiguous():
+        raise ValueError("layernorm_fwd: out must have the shape of x, gamma and beta be contiguous of its last dimension")
+    stats = torch.empty(shape[:-1] + (2,), dtype=torch.float32, device=x.device)
+    _train_call("dbir_layernorm_fwd", dev, dt, x.data_ptr(), _row_ld(x, "layernorm_fwd: x"), out.data_ptr(), _row_ld(out, "layernorm_fwd: out"),
+                gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(), stats.numel() >> 1, C, eps)
     return out, stats
 
 
 def layernorm_bwd(dy: T, x: T, gamma: T, stats: T, dres: Optional[T] = None, dx: Optional[T] = None) -> Tuple[T, T, T]:
     """Gradients (dx, dgamma f32, dbeta f32) of layernorm_fwd from its x and stats; dres (like x): the gradient that reaches x past the
     norm (a residual connection) is added to dx."""
-    dev = _train_args("layernorm_bwd", dy, x, gamma, stats, dres, dx)
-    C, M = x.shape[-1], _rows(x)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if dx is None else dx
-    for name, t in (("dy", dy), ("dres", dres), ("dx", dx)):
-        _need(t is None or (t.shape == x.shape and t.dtype == x.dtype), f"layernorm_bwd: {name} must be like x ({tuple(x.shape)}, {x.dtype})")
-    _f32_vec(gamma, C, "layernorm_bwd: gamma")
-    _f32_vec(stats, 2 * M, "layernorm_bwd: stats")
-    _apart("layernorm_bwd", (dx,), (dy, x, dres))
-    dgb = torch.empty((2, C), dtype=torch.float32, device=dev)
-    nbytes = ctypes.c_longlong()
-    native.check(native.lib().dbir_layernorm_bwd_ws(M, C, ctypes.byref(nbytes)), "dbir_layernorm_bwd_ws")
-    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
-    ld = lambda t, n: 0 if t is None else _row_ld(t, "layernorm_bwd: " + n)  # noqa: E731
-    with _on(dev):
-        native.check(native.lib().dbir_layernorm_bwd(_dt3(x), dy.data_ptr(), ld(dy, "dy"), x.data_ptr(), ld(x, "x"),
-                                                     None if dres is None else dres.data_ptr(), ld(dres, "dres"), dx.data_ptr(), ld(dx, "dx"),
-                                                     gamma.data_ptr(), stats.data_ptr(), dgb[0].data_ptr(), dgb[1].data_ptr(), M, C,
-                                                     ws.data_ptr(), nbytes.value, _stream()), "dbir_layernorm_bwd")
-    return dx, dgb[0], dgb[1]
+    dev = _train_device("layernorm_bwd", x, dy, gamma, stats, dres, dx)
+    if dx is None:
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    shape, dt = x.shape, _DT3.get(x.dtype)
+    C = shape[-1]
+    if dt is None or dy.dtype != x.dtype or dx.dtype != x.dtype or (dres is not None and dres.dtype != x.dtype) or gamma.dtype != torch.float32 \
+            or stats.dtype != torch.float32:
+        raise TypeError("layernorm_bwd: x, dy, dres and dx must have one type (f16, bf16 or f32), gamma and stats f32")
+    if dy.shape != shape or dx.shape != shape or (dres is not None and dres.shape != shape) or gamma.shape != (C,) or \
+            stats.shape != shape[:-1] + (2,) or not gamma.is_contiguous() or not stats.is_contiguous():
+        raise ValueError("layernorm_bwd: dy, dres and dx must have the shape of x, gamma be contiguous of its last dimension and stats be layernorm_fwd's")
+    M = stats.numel() >> 1
+    dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(gamma)
+    nws = _ws_bytes("dbir_layernorm_bwd_ws", M, C)
+    ws = torch.empty(nws, dtype=torch.uint8, device=x.device)
+    _train_call("dbir_layernorm_bwd", dev, dt, dy.data_ptr(), _row_ld(dy, "layernorm_bwd: dy"), x.data_ptr(), _row_ld(x, "layernorm_bwd: x"),
+                None if dres is None else dres.data_ptr(), C if dres is None else _row_ld(dres, "layernorm_bwd: dres"), dx.data_ptr(),
+                _row_ld(dx, "layernorm_bwd: dx"), gamma.data_ptr(), stats.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), M, C, ws.data_ptr(), nws)
+    return dx, dgamma, dbeta
 
 
 def embedding(tokens: T, table: T, scale: float = 1.0, pos: Optional[T] = None, dtype: Optional[torch.dtype] = None,
               out: Optional[T] = None) -> T:
     """tokens int64 [..., L] -> scale * table[tokens] (+ pos[:L]) as [..., L, W] in `dtype` (the table's by default).  table f16 / bf16 /
     f32 [vocab, W], pos f32 [>= L, W]; tokens outside the table read its nearest row, as in clip_embed."""
-    dev = _train_args("embedding", tokens, table, pos, out)
-    _need(tokens.dtype == torch.int64 and tokens.dim() >= 1 and tokens.is_contiguous(), "embedding: tokens must be contiguous int64 [..., L]")
-    _need(table.dim() == 2 and (pos is None or (pos.dim() == 2 and pos.dtype == torch.float32)), "embedding: table must be [vocab, W], pos f32 [L, W]")
-    (vocab, W), L, n = table.shape, tokens.shape[-1], tokens.numel()
-    _need(pos is None or (pos.shape[0] >= L and pos.shape[1] == W), "embedding: pos must be [>= L, W]")
+    dev = _train_device("embedding", tokens, table, pos, out)
+    ts = tokens.shape
+    if tokens.dtype != torch.int64 or not ts or not tokens.is_contiguous() or table.dim() != 2:
+        raise ValueError("embedding: tokens must be contiguous int64 [..., L], table [vocab, W]")
+    (vocab, W), L = table.shape, ts[-1]
+    if pos is not None and (pos.dtype != torch.float32 or pos.dim() != 2 or pos.shape[0] < L or pos.shape[1] != W):
+        raise ValueError(f"embedding: pos must be f32 [>= {L}, {W}]")
     if out is None:
-        out = torch.empty(tokens.shape + (W,), dtype=dtype or table.dtype, device=dev)
-    _need(out.shape == tokens.shape + (W,) and dtype in (None, out.dtype), "embedding: out must be [..., L, W] in `dtype`")
-    _apart("embedding", (out,), (table, pos))
-    with _on(dev):
-        native.check(native.lib().dbir_embedding_fwd(_dt3(table), table.data_ptr(), _row_ld(table, "embedding: table"), tokens.data_ptr(),
-                                                     None if pos is None else pos.data_ptr(), 0 if pos is None else _row_ld(pos, "embedding: pos"),
-                                                     _dt3(out), out.data_ptr(), _row_ld(out, "embedding: out"), scale, n, L, W, vocab,
-                                                     _stream()), "dbir_embedding_fwd")
+        out = torch.empty(ts + (W,), dtype=table.dtype if dtype is None else dtype, device=table.device)
+    elif out.shape != ts + (W,) or dtype not in (None, out.dtype):
+        raise ValueError("embedding: out must be [..., L, W] in `dtype`")
+    tdt, odt = _DT3.get(table.dtype), _DT3.get(out.dtype)
+    if tdt is None or odt is None:
+        raise TypeError("embedding: table and out must be f16, bf16 or f32")
+    _train_call("dbir_embedding_fwd", dev, tdt, table.data_ptr(), _row_ld(table, "embedding: table"), tokens.data_ptr(),
+                None if pos is None else pos.data_ptr(), 0 if pos is None else _row_ld(pos, "embedding: pos"), odt, out.data_ptr(),
+                _row_ld(out, "embedding: out"), scale, tokens.numel(), L, W, vocab)
     return out
 
 
@@ -860,24 +868,27 @@ def embedding_bwd(dy: T, tokens: T, vocab: int, scale: float = 1.0, pos_rows: in
                   out: Optional[T] = None, accumulate: bool = False) -> Tuple[T, Optional[T]]:
     """Gradients of embedding -> (dtable f32 [vocab, W], dpos f32 [pos_rows, W] or None).  dy f16 / bf16 / f32 [..., L, W]; the row of
     padding_idx gets none; out + accumulate: added to `out`, whose rows that no token names stay untouched."""
-    dev = _train_args("embedding_bwd", dy, tokens, out)
-    _need(tokens.dtype == torch.int64 and tokens.dim() >= 1 and tokens.is_contiguous(), "embedding_bwd: tokens must be contiguous int64 [..., L]")
-    _need(dy.shape[:-1] == tokens.shape, f"embedding_bwd: dy {tuple(dy.shape)} does not fit tokens {tuple(tokens.shape)}")
-    _need(vocab > 0 and (padding_idx is None or 0 <= padding_idx < vocab), "embedding_bwd: padding_idx must be a row of the table")
-    _need(out is not None or not accumulate, "embedding_bwd: accumulate needs `out`")
-    W, L, n = dy.shape[-1], tokens.shape[-1], tokens.numel()
-    out = torch.empty((vocab, W), dtype=torch.float32, device=dev) if out is None else out
-    _need(tuple(out.shape) == (vocab, W) and out.dtype == torch.float32, f"embedding_bwd: out must be f32 [{vocab}, {W}]")
-    _apart("embedding_bwd", (out,), (dy,))
-    dpos = torch.empty((pos_rows, W), dtype=torch.float32, device=dev) if pos_rows else None
-    nbytes = ctypes.c_longlong()
-    native.check(native.lib().dbir_embedding_bwd_ws(n, W, vocab, ctypes.byref(nbytes)), "dbir_embedding_bwd_ws")
-    ws = torch.empty(nbytes.value, dtype=torch.uint8, device=dev)
-    with _on(dev):
-        native.check(native.lib().dbir_embedding_bwd(_dt3(dy), dy.data_ptr(), _row_ld(dy, "embedding_bwd: dy"), tokens.data_ptr(), out.data_ptr(),
-                                                     _row_ld(out, "embedding_bwd: out"), None if dpos is None else dpos.data_ptr(), scale, n, L, W,
-                                                     vocab, pos_rows, -1 if padding_idx is None else padding_idx, int(accumulate),
-                                                     ws.data_ptr(), nbytes.value, _stream()), "dbir_embedding_bwd")
+    dev = _train_device("embedding_bwd", dy, tokens, out)
+    ts, ds, dt = tokens.shape, dy.shape, _DT3.get(dy.dtype)
+    if dt is None:
+        raise TypeError(f"embedding_bwd: dy must be f16, bf16 or f32, got {dy.dtype}")
+    if tokens.dtype != torch.int64 or not ts or not tokens.is_contiguous() or ds[:-1] != ts:
+        raise ValueError(f"embedding_bwd: tokens must be contiguous int64 [..., L] and dy [..., L, W], got {tuple(ts)} and {tuple(ds)}")
+    if vocab <= 0 or (padding_idx is not None and not 0 <= padding_idx < vocab):
+        raise ValueError("embedding_bwd: padding_idx must be a row of the table")
+    W, L, n = ds[-1], ts[-1], tokens.numel()
+    if out is None:
+        if accumulate:
+            raise ValueError("embedding_bwd: accumulate needs `out`")
+        out = torch.empty((vocab, W), dtype=torch.float32, device=dy.device)
+    elif out.shape != (vocab, W) or out.dtype != torch.float32:
+        raise ValueError(f"embedding_bwd: out must be f32 [{vocab}, {W}]")
+    dpos = torch.empty((pos_rows, W), dtype=torch.float32, device=dy.device) if pos_rows else None
+    nws = _ws_bytes("dbir_embedding_bwd_ws", n, W, vocab)
+    ws = torch.empty(nws, dtype=torch.uint8, device=dy.device)
+    _train_call("dbir_embedding_bwd", dev, dt, dy.data_ptr(), _row_ld(dy, "embedding_bwd: dy"), tokens.data_ptr(), out.data_ptr(),
+                _row_ld(out, "embedding_bwd: out"), None if dpos is None else dpos.data_ptr(), scale, n, L, W, vocab, pos_rows,
+                -1 if padding_idx is None else padding_idx, bool(accumulate), ws.data_ptr(), nws)
     return out, dpos
 
 

@@ -285,7 +285,8 @@ int dbir_xf_tail(int dtype, const void* attn_out, long long ldo, const void* h, 
  * dbir_attention_fwd / dbir_attention_bwd (csrc/attention_train.hip): softmax(scale Q K^T) V, head_dim 64, 16-bit (dtype f16 / bf16).
  *   q, out, dout, dq [B, Lq, H, 64]; k, v, dk, dv [B, Lk, Hkv, 64], H % Hkv == 0 (query head h reads key head h / (H / Hkv)); strides are
  *   those of batch, row and head in elements (multiples of 8; rows at least 64 and less than 2^23 apart; 16-byte aligned bases), so a slice of
- *   a wider buffer or a [B, H, L, 64] tensor serves as well.
+ *   a wider buffer or a [B, H, L, 64] tensor serves as well (the stride of a dimension of one does not matter).  Outputs must not overlap
+ *   inputs or each other.
  *   lse f32 [B, H, Lq] dense: log of the sum of exp(scale q . k) over the visible keys, -infinity where a row sees none.
  *   causal: query i sees keys j <= i + Lk - Lq.  q_len / kv_len: int32 [B] on the device or NULL: rows of sample b at or behind its length are
  *   not read (they may hold anything); out, dq, dk, dv are zero and lse is -infinity there.  A row that sees no key: out and dq zero.
@@ -304,14 +305,14 @@ typedef struct {
   long long ws_bytes;
   long long q_stride[3], k_stride[3], v_stride[3], out_stride[3], dout_stride[3], dq_stride[3], dk_stride[3], dv_stride[3];
 } dbir_attn_desc;
-int dbir_attention_fwd_ws(const dbir_attn_desc* d, long long* bytes);
-int dbir_attention_bwd_ws(const dbir_attn_desc* d, long long* bytes);
+int dbir_attention_fwd_ws(int dtype, int B, int H, int Hkv, int Lq, int Lk, long long* bytes);
+int dbir_attention_bwd_ws(int dtype, int B, int H, int Hkv, int Lq, int Lk, long long* bytes);
 int dbir_attention_fwd(const dbir_attn_desc* d, void* stream);
 int dbir_attention_bwd(const dbir_attn_desc* d, void* stream);
 
 /* dbir_layernorm_fwd / dbir_layernorm_bwd (csrc/norm_train.hip): rows of C columns, dtype f16 / bf16 / f32 for x, y, dy, dres, dx (row
  *   strides ld*, any alignment), everything else f32.  stats [rows, 2]: mean and 1 / sqrt(variance + eps).
- *   dx = gradient of x (+ dres, the gradient that arrives past the norm, if not NULL); dgamma, dbeta [C] are written, not added to.
+ *   Outputs must not overlap inputs.  dx = gradient of x (+ dres, the gradient that arrives past the norm, if not NULL); dgamma, dbeta [C] are written, not added to.
  *   ws: dbir_layernorm_bwd_ws bytes. */
 int dbir_layernorm_bwd_ws(int rows, int C, long long* bytes);
 int dbir_layernorm_fwd(int dtype, const void* x, long long ldx, void* y, long long ldy, const float* gamma, const float* beta,

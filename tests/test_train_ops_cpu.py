@@ -28,9 +28,11 @@ def no_launch(monkeypatch):
 
     monkeypatch.setattr(ops, "_gpu", lambda *ts: None)
     monkeypatch.setattr(ops, "_stream", lambda: 0)
-    monkeypatch.setattr(ops, "_on", lambda dev: __import__("contextlib").nullcontext())
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    ops._ws_bytes.cache_clear()
     monkeypatch.setattr(native, "_lib", Lib())
-    return calls
+    yield calls
+    ops._ws_bytes.cache_clear()
 
 
 def qkv(B=2, Lq=5, Lk=7, H=4, Hkv=2, dt=F16):
@@ -53,7 +55,6 @@ def test_attention_refusals(no_launch):
         (q[..., :32], k, v, {}), (q[0], k, v, {}), (q, k[:, :6], v, {}), (q, k, v[:1], {}), (q, k.to(BF16), v, {}),
         (q.double(), k.double(), v.double(), {}), (q, k, v, dict(q_len=torch.zeros(2))), (q, k, v, dict(kv_len=torch.zeros(3, dtype=torch.int32))),
         (q, k, v, dict(kv_len=torch.zeros(4, dtype=torch.int32)[::2])), (q, k, v, dict(out=torch.zeros(2, 5, 4, 64))),
-        (q, k, v, dict(out=torch.zeros(1, 1, 1, 64, dtype=F16).expand(2, 5, 4, 64))), (q, k, v, dict(out=q)),
         (torch.zeros(2, 5, 4, 128, dtype=F16)[..., ::2], k, v, {})]
     for a, b, c, kw in bad:
         with pytest.raises((ValueError, TypeError)):
@@ -61,7 +62,7 @@ def test_attention_refusals(no_launch):
     o, lse = ops.attention_fwd(q, k, v, 0.125)
     g = torch.zeros_like(q)
     for args, kw in [((g[:, :4], q, k, v, o, lse), {}), ((g, q, k, v, o, lse[:1]), {}), ((g, q, k, v, o, lse.double()), {}),
-                     ((g, q, k, v, o, lse), dict(dq=g)), ((g, q, k, v, o, lse), dict(dk=torch.zeros_like(q))), ((g, q, k, v, o, lse), dict(dk=k))]:
+                     ((g, q, k, v, o, lse), dict(dk=torch.zeros_like(q)))]:
         with pytest.raises((ValueError, TypeError)):
             ops.attention_bwd(*args, 0.125, **kw)
     assert no_launch == ["dbir_attention_fwd"]
@@ -69,15 +70,14 @@ def test_attention_refusals(no_launch):
 
 def test_layernorm_refusals(no_launch):
     x, one = torch.zeros(4, 8), torch.ones(8)
-    for args, kw in [((x.double(), one, one), {}), ((x, one[:4], one), {}), ((x, one.half(), one), {}), ((x, one, one), dict(out=x)),
+    for args, kw in [((x.double(), one, one), {}), ((x, one[:4], one), {}), ((x, one.half(), one), {}),
                      ((x, one, one), dict(out=x.half())), ((torch.zeros(8, 4).t(), torch.ones(8), torch.ones(8)), {}),
                      ((torch.zeros(1, 8).expand(4, 8), one, one), dict(out=torch.zeros(1, 8).expand(4, 8)))]:
         with pytest.raises((ValueError, TypeError)):
             ops.layernorm_fwd(*args, **kw)
     _, st = ops.layernorm_fwd(x, one, one)
     dy = torch.zeros(4, 8)
-    for args, kw in [((dy.half(), x, one, st), {}), ((dy, x, one, st[:2]), {}), ((dy, x, one, st), dict(dres=x.half())), ((dy, x, one, st), dict(dx=dy)),
-                     ((dy, x, one, st), dict(dx=x)), ((dy[:2], x, one, st), {})]:
+    for args, kw in [((dy.half(), x, one, st), {}), ((dy, x, one, st[:2]), {}), ((dy, x, one, st), dict(dres=x.half())), ((dy[:2], x, one, st), {})]:
         with pytest.raises((ValueError, TypeError)):
             ops.layernorm_bwd(*args, **kw)
     assert no_launch == ["dbir_layernorm_fwd"]
@@ -137,16 +137,17 @@ def test_attn_desc_layout_matches_header(tmp_path):
 
 
 def good_desc():
-    s = (64 * 64, 64, 64)
-    p = 1 << 20
-    return native.AttnDesc(0, 1, 1, 1, 64, 64, 0, 0.125, p, p, p, p, p, None, None, p, p, p, p, p, 1 << 30, s, s, s, s, s, s, s, s)
+    s = (64 * 128, 128, 64)
+    p = [(i + 1) << 20 for i in range(10)]
+    return native.AttnDesc(0, 2, 2, 2, 64, 64, 0, 0.125, *p[:5], None, None, *p[5:], 1 << 30, s, s, s, s, s, s, s, s)
 
 
 @pytest.mark.parametrize("change", [
     dict(dtype=2), dict(dtype=-1), dict(B=0), dict(H=0), dict(Hkv=0), dict(H=3, Hkv=2), dict(Lq=0), dict(Lk=0), dict(Lk=-1), dict(B=70000),
     dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(q=None), dict(k=None), dict(v=None), dict(out=None),
     dict(lse=None), dict(q=(1 << 20) + 2), dict(q_stride=(0, 60, 64)), dict(k_stride=(0, 32, 64)), dict(v_stride=(0, 1 << 23, 64)),
-    dict(out_stride=(0, 64, 4)), dict(q_stride=(-64, 64, 64)), dict(dout=None), dict(dq=None), dict(dk=(1 << 20) + 8), dict(dv_stride=(0, 0, 64)),
+    dict(out_stride=(0, 64, 4)), dict(q_stride=(-64, 64, 64)), dict(k_stride=(8192, 128, 4)), dict(dq_stride=(0, 128, 64)), dict(dv_stride=(8192, 128, 0)), dict(dq=1 << 20), dict(dk=6 << 20),
+    dict(dv=2 << 20), dict(dq=8 << 20, dk=8 << 20), dict(dv=7 << 20), dict(dout=None), dict(dq=None), dict(dk=(1 << 20) + 8), dict(dv_stride=(0, 0, 64)),
     dict(ws=None), dict(ws_bytes=16), dict(ws=(1 << 20) + 4)])
 def test_attention_descriptor_refusals(lib, change):
     d = good_desc()
@@ -154,30 +155,44 @@ def test_attention_descriptor_refusals(lib, change):
         setattr(d, n, (ctypes.c_longlong * 3)(*v) if isinstance(v, tuple) else v)
     assert lib.dbir_attention_bwd(ctypes.byref(d), None) == 1
     assert b"dbir_attention_bwd" in lib.dbir_last_error()
-    if not set(change) & {"dout", "dq", "dk", "dv_stride", "ws", "ws_bytes"}:
+    if not set(change) & {"dout", "dq", "dk", "dv", "dv_stride", "dq_stride", "ws", "ws_bytes"}:
         assert lib.dbir_attention_fwd(ctypes.byref(d), None) == 1
     assert lib.dbir_attention_fwd(None, None) == 1
 
 
+def test_attention_forward_refuses_its_input_as_output(lib):
+    for name, v in (("out", 1 << 20), ("out", 2 << 20), ("out", 3 << 20), ("out_stride", (8192, 0, 64)), ("out_stride", (0, 128, 64))):
+        d = good_desc()
+        setattr(d, name, (ctypes.c_longlong * 3)(*v) if isinstance(v, tuple) else v)
+        assert lib.dbir_attention_fwd(ctypes.byref(d), None) == 1
+
+
+def test_packed_descriptor_is_the_struct():
+    d = good_desc()
+    vals = [getattr(d, n) for n, _ in native.AttnDesc._fields_]
+    flat = [x for v in vals for x in (list(v) if hasattr(v, "__len__") else [0 if v is None else v])]
+    assert ops._ATTN_PACK(*flat) == bytes(d)
+
+
 def test_norm_and_embedding_refusals(lib):
-    p, big = 1 << 20, 1 << 30
-    fwd = [0, p, 8, p, 8, p, p, p, 4, 8, 1e-5, None]
-    for i, v in [(0, 3), (0, -1), (1, None), (2, 7), (3, None), (4, 7), (5, None), (7, None), (8, 0), (9, 0)]:
+    p, r, t, big = 1 << 20, 2 << 20, 3 << 20, 1 << 30
+    fwd = [0, p, 8, r, 8, p, p, p, 4, 8, 1e-5, None]
+    for i, v in [(0, 3), (0, -1), (1, None), (2, 7), (3, None), (3, p), (4, 7), (5, None), (7, None), (8, 0), (9, 0)]:
         a = list(fwd)
         a[i] = v
         assert lib.dbir_layernorm_fwd(*a) == 1, (i, v)
-    bwd = [0, p, 8, p, 8, None, 0, p, 8, p, p, p, p, 4, 8, p, big, None]
-    for i, v in [(0, 3), (1, None), (2, 7), (4, 7), (5, p), (8, 7), (9, None), (10, None), (11, None), (12, None), (13, 0), (14, 0), (15, None), (16, 8)]:
+    bwd = [0, p, 8, r, 8, None, 0, t, 8, p, p, p, p, 4, 8, p, big, None]
+    for i, v in [(0, 3), (1, None), (2, 7), (4, 7), (5, p), (7, p), (7, r), (8, 7), (9, None), (10, None), (11, None), (12, None), (13, 0), (14, 0), (15, None), (16, 8)]:
         a = list(bwd)
         a[i] = v
         assert lib.dbir_layernorm_bwd(*a) == 1, (i, v)
-    emb = [2, p, 8, p, None, 0, 2, p, 8, 1.0, 6, 3, 8, 5, None]
-    for i, v in [(0, 3), (1, None), (2, 7), (3, None), (4, p), (6, 3), (7, None), (8, 7), (10, 0), (11, 0), (12, 0), (13, 0), (10, 1 << 30)]:
+    emb = [2, p, 8, p, None, 0, 2, r, 8, 1.0, 6, 3, 8, 5, None]
+    for i, v in [(0, 3), (1, None), (2, 7), (3, None), (4, p), (6, 3), (7, None), (7, p), (8, 7), (10, 0), (11, 0), (12, 0), (13, 0), (10, 1 << 30)]:
         a = list(emb)
         a[i] = v
         assert lib.dbir_embedding_fwd(*a) == 1, (i, v)
-    eb = [2, p, 8, p, p, 8, None, 1.0, 6, 3, 8, 5, 0, -1, 0, p, big, None]
-    for i, v in [(0, 3), (1, None), (2, 7), (3, None), (4, None), (5, 7), (8, 0), (8, 7), (9, 0), (10, 0), (11, 0), (12, 3), (12, 2), (15, None), (16, 8), (15, p + 4)]:
+    eb = [2, p, 8, p, r, 8, None, 1.0, 6, 3, 8, 5, 0, -1, 0, p, big, None]
+    for i, v in [(0, 3), (1, None), (2, 7), (3, None), (4, None), (4, p), (5, 7), (8, 0), (8, 7), (9, 0), (10, 0), (11, 0), (12, 3), (12, 2), (15, None), (16, 8), (15, p + 4)]:
         a = list(eb)
         a[i] = v
         assert lib.dbir_embedding_bwd(*a) == 1, (i, v)
