@@ -30,6 +30,8 @@ struct Args {
   const int *q_len, *kv_len;
   float *nl2, *nd;        // [B * H, Lqp]: -lse * log2(e) and -D, -inf and 0 behind the last row
   float *gmax, *vmax;     // f16: per 64 rows the largest row norm of dout / v
+  float *part, *part_row; // with several splits: their sums [split][head][row][64] (dk, dv: [128]) and a number per row
+  int splits;
   int B, H, Hkv, Lq, Lk, causal, Lqp;
   float scale;
 };
@@ -113,6 +115,20 @@ __device__ __forceinline__ void store_cols(u16* row, const f32x16* acc, float mu
       *reinterpret_cast<uint2*>(row + t * 32 + 8 * g + 4 * hi) = pk;
     }
 }
+// the same as f32 into a partial sum
+__device__ __forceinline__ void store_cols_f32(float* row, const f32x16* acc, float mul, int hi) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<float4*>(row + t * 32 + 8 * g + 4 * hi) =
+          make_float4(acc[t][4 * g] * mul, acc[t][4 * g + 1] * mul, acc[t][4 * g + 2] * mul, acc[t][4 * g + 3] * mul);
+}
+// split s of n tiles
+__device__ __forceinline__ void split_range(int n, int s, int splits, int& t0, int& t1) {
+  t0 = (int)((long long)n * s / splits);
+  t1 = (int)((long long)n * (s + 1) / splits);
+}
 __device__ __forceinline__ int row_of(int r, int hi) { return (r & 3) + 8 * (r >> 2) + 4 * hi; }
 __device__ __forceinline__ int clamp_len(const int* len, int b, int most) {
   const int n = len ? len[b] : most;
@@ -124,12 +140,13 @@ __device__ __forceinline__ void tile_ready() {
 }
 
 // ---------------------------------------------------------------------------------------------------------------- forward
-// 128 queries a workgroup, 32 a wave; keys in tiles of 64, double buffered.
+// 128 queries a workgroup, 32 a wave; keys in tiles of 64, double buffered.  With few workgroups the keys are split over several
+// (host rule): each leaves its normalised sum and lse, attn_fwd_join_kernel weighs them.
 template <typename T>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char lds[4 * TILE_BYTES];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
-  const int nqb = (a.Lq + 127) >> 7, w = xcd_range(blockIdx.x, gridDim.x);
+  const int nqb = (a.Lq + 127) >> 7, ws = xcd_range(blockIdx.x, gridDim.x), split = ws % a.splits, w = ws / a.splits;
   const int bh = w / nqb, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
   const int qb = a.causal ? nqb - 1 - w % nqb : w % nqb;   // (long rows first)
   const int nk = clamp_len(a.kv_len, b, a.Lk), nq = clamp_len(a.q_len, b, a.Lq), off = a.Lk - a.Lq;
@@ -147,21 +164,20 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Args a) {
   const float c = a.scale * LOG2E;
   f32x16 acc[2] = {splat(0.f), splat(0.f)};
   float m = -INFINITY, l = 0.f;   // running maximum (times c) and sum
-  const int nt = kend > 0 ? (kend + TILE - 1) / TILE : 0;
-  if (nt) {
-    stage_tile(lds, kp, a.ks[1], 0, nk, wave, lane);
-    stage_tile(lds + TILE_BYTES, vp, a.vs[1], 0, nk, wave, lane);
-  }
-  for (int t = 0; t < nt; ++t) {
+  int t0, t1;
+  split_range(kend > 0 ? (kend + TILE - 1) / TILE : 0, split, a.splits, t0, t1);
+  auto stage = [&](int t) {
+    char* p = lds + (t & 1) * 2 * TILE_BYTES;
+    stage_tile(p, kp, a.ks[1], t * TILE, nk, wave, lane);
+    stage_tile(p + TILE_BYTES, vp, a.vs[1], t * TILE, nk, wave, lane);
+  };
+  if (t0 < t1) stage(t0);
+  for (int t = t0; t < t1; ++t) {
     const int key0 = t * TILE;
     const char *kt = lds + (t & 1) * 2 * TILE_BYTES, *vt = kt + TILE_BYTES;
     tile_ready();
-    if (t + 1 < nt) {
-      char* nxt = lds + ((t + 1) & 1) * 2 * TILE_BYTES;
-      stage_tile(nxt, kp, a.ks[1], key0 + TILE, nk, wave, lane);
-      stage_tile(nxt + TILE_BYTES, vp, a.vs[1], key0 + TILE, nk, wave, lane);
-    }
-    if (key0 >= wend) continue;
+    if (t + 1 < t1) stage(t + 1);
+    if (key0 >= wend || w0 >= nq) continue;
     f32x16 s[2] = {splat(0.f), splat(0.f)};
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb)
@@ -206,10 +222,70 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Args a) {
   }
   if (row < a.Lq) {
     const bool some = q_ok && l != 0.f;   // (a NaN stays one)
-    store_cols<T>(a.o + b * a.os[0] + (long long)row * a.os[1] + h * a.os[2], acc, some ? 1.f / l : 0.f, hi);
-    if (hi == 0) a.lse[(long long)bh * a.Lq + row] = some ? (m + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+    const float inv = some ? 1.f / l : 0.f, lse = some ? (m + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+    const long long at = (long long)bh * a.Lq + row, pat = (long long)split * a.B * a.H * a.Lq + at;
+    if (a.splits == 1) store_cols<T>(a.o + b * a.os[0] + (long long)row * a.os[1] + h * a.os[2], acc, inv, hi);
+    else store_cols_f32(a.part + pat * HD, acc, inv, hi);
+    if (hi == 0) (a.splits == 1 ? a.lse + at : a.part_row + pat)[0] = lse;
   }
 }
+
+// 16 rows a workgroup, 16 lanes a row, 4 columns a lane
+template <typename T>
+__global__ __launch_bounds__(256) void attn_fwd_join_kernel(const Args a) {
+  const long long rows = (long long)a.B * a.H * a.Lq, at = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (at >= rows) return;
+  const int c = (threadIdx.x & 15) * 4;
+  float m = -INFINITY;
+  bool nan = false;
+  for (int s = 0; s < a.splits; ++s) {
+    const float l = a.part_row[s * rows + at];
+    m = fmaxf(m, l);
+    nan |= l != l;
+  }
+  float o[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float w = m == -INFINITY && !nan ? 0.f : __builtin_amdgcn_exp2f((a.part_row[s * rows + at] - m) * LOG2E);
+    const float4 v = *reinterpret_cast<const float4*>(a.part + (s * rows + at) * HD + c);
+    o[0] = __builtin_fmaf(w, v.x, o[0]);
+    o[1] = __builtin_fmaf(w, v.y, o[1]);
+    o[2] = __builtin_fmaf(w, v.z, o[2]);
+    o[3] = __builtin_fmaf(w, v.w, o[3]);
+    sum += w;
+  }
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  const int row = (int)(at % a.Lq), bh = (int)(at / a.Lq), b = bh / a.H, h = bh % a.H;
+  *reinterpret_cast<uint2*>(a.o + b * a.os[0] + (long long)row * a.os[1] + h * a.os[2] + c) =
+      make_uint2(T::pack2(o[0] * inv, o[1] * inv), T::pack2(o[2] * inv, o[3] * inv));
+  if (c == 0) a.lse[at] = sum != 0.f ? m + __builtin_amdgcn_logf(sum) * LN2 : -INFINITY;
+}
+
+// the f32 sums of the splits -> 16 bits; WIDTH 64: dq (and the corrections of D), 128: dk and dv
+template <typename T, int WIDTH>
+__global__ __launch_bounds__(256) void attn_bwd_join_kernel(const Args a) {
+  constexpr int LPR = WIDTH / 4;
+  const int L = WIDTH == 64 ? a.Lq : a.Lk, H = WIDTH == 64 ? a.H : a.Hkv;
+  const long long rows = (long long)a.B * H * L, at = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  if (at >= rows) return;
+  const int c = (threadIdx.x % LPR) * 4;
+  float o[4] = {0.f, 0.f, 0.f, 0.f}, d = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s) {
+    const float4 v = *reinterpret_cast<const float4*>(a.part + (s * rows + at) * WIDTH + c);
+    o[0] += v.x;
+    o[1] += v.y;
+    o[2] += v.z;
+    o[3] += v.w;
+    if (WIDTH == 64 && c == 0) d += a.part_row[s * rows + at];
+  }
+  const int row = (int)(at % L), bh = (int)(at / L), b = bh / H, h = bh % H;
+  u16* to = WIDTH == 64 ? a.dq + b * a.dqs[0] + (long long)row * a.dqs[1] + h * a.dqs[2] + c :
+            c < 64      ? a.dk + b * a.dks[0] + (long long)row * a.dks[1] + h * a.dks[2] + c :
+                          a.dv + b * a.dvs[0] + (long long)row * a.dvs[1] + h * a.dvs[2] + c - 64;
+  *reinterpret_cast<uint2*>(to) = make_uint2(T::pack2(o[0], o[1]), T::pack2(o[2], o[3]));
+  if (WIDTH == 64 && c == 0) a.nd[(long long)bh * a.Lqp + row] -= d;
+}
+
 
 // ---------------------------------------------------------------------------------------------------------------- backward
 // D and the negated statistics of 64 rows, 8 lanes a row; f16 also the largest norms (scale_exp below).
@@ -305,13 +381,13 @@ __device__ __forceinline__ float scale_exp<F16>(const Args& a, int b, int hk, in
 }
 
 // dk, dv: 128 keys a workgroup, 32 a wave (their k, v operands and sums stay in registers); queries in tiles of 64, double buffered,
-// over all heads that share these keys.
+// over all heads that share these keys; with few workgroups these rounds are split over several (host rule).
 template <typename T>
 __global__ __launch_bounds__(256, 2) void attn_bwd_kv_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char lds[2 * (2 * TILE_BYTES + 512)];
   __shared__ float red[8];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
-  const int nkb = (a.Lk + 127) >> 7, w = xcd_range(blockIdx.x, gridDim.x);
+  const int nkb = (a.Lk + 127) >> 7, ws = xcd_range(blockIdx.x, gridDim.x), split = ws % a.splits, w = ws / a.splits;
   const int bh = w / nkb, b = bh / a.Hkv, hk = bh % a.Hkv, grp = a.H / a.Hkv, k0 = (w % nkb) * 128;
   const int nk = clamp_len(a.kv_len, b, a.Lk), nq = clamp_len(a.q_len, b, a.Lq), off = a.Lk - a.Lq;
   const int key = k0 + wave * 32 + (lane & 31);
@@ -333,12 +409,15 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_kv_kernel(const Args a) {
       __builtin_amdgcn_raw_ptr_buffer_load_lds(srd, (lds_ptr)(p + 2 * TILE_BYTES + wave * 256), 4, lane * 4, 0, 0, 0);
     }
   };
-  if (nt) stage(0);
-  for (int it = 0; it < nt * grp; ++it) {
+  int it0, it1;
+  split_range(nt * grp, split, a.splits, it0, it1);
+  if (it0 < it1) stage(it0);
+  for (int it = it0; it < it1; ++it) {
     const char *qt = lds + (it & 1) * (2 * TILE_BYTES + 512), *gt = qt + TILE_BYTES;
     const float* st = reinterpret_cast<const float*>(gt + TILE_BYTES);
     tile_ready();
-    if (it + 1 < nt * grp) stage(it + 1);
+    if (it + 1 < it1) stage(it + 1);
+    if (k0 + wave * 32 >= nk) continue;
     const int q0 = (qt0 + it % nt) * TILE;
 #pragma unroll
     for (int sb = 0; sb < 2; ++sb) {
@@ -383,8 +462,14 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_kv_kernel(const Args a) {
     const float un = k_ok ? __builtin_amdgcn_exp2f(-e) : 0.f;
     if (!k_ok)
       for (int d = 0; d < 2; ++d) dk[d] = dv[d] = splat(0.f);   // (whatever the sums of a key that nobody sees are)
-    store_cols<T>(a.dk + b * a.dks[0] + (long long)key * a.dks[1] + hk * a.dks[2], dk, un * a.scale, hi);
-    store_cols<T>(a.dv + b * a.dvs[0] + (long long)key * a.dvs[1] + hk * a.dvs[2], dv, un, hi);
+    if (a.splits == 1) {
+      store_cols<T>(a.dk + b * a.dks[0] + (long long)key * a.dks[1] + hk * a.dks[2], dk, un * a.scale, hi);
+      store_cols<T>(a.dv + b * a.dvs[0] + (long long)key * a.dvs[1] + hk * a.dvs[2], dv, un, hi);
+    } else {
+      float* p = a.part + (((long long)split * a.B * a.Hkv + bh) * a.Lk + key) * 128;
+      store_cols_f32(p, dk, un * a.scale, hi);
+      store_cols_f32(p + 64, dv, un, hi);
+    }
   }
 }
 
@@ -396,7 +481,7 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_q_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char lds[4 * TILE_BYTES];
   __shared__ float red[8];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
-  const int nqb = (a.Lq + 127) >> 7, w = xcd_range(blockIdx.x, gridDim.x);
+  const int nqb = (a.Lq + 127) >> 7, ws = xcd_range(blockIdx.x, gridDim.x), split = ws % a.splits, w = ws / a.splits;
   const int bh = w / nqb, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
   const int qb = a.causal ? nqb - 1 - w % nqb : w % nqb;
   const int nk = clamp_len(a.kv_len, b, a.Lk), nq = clamp_len(a.q_len, b, a.Lq), off = a.Lk - a.Lq;
@@ -416,6 +501,10 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_q_kernel(const Args a) {
   float nd = q_ok ? a.nd[(long long)bh * a.Lqp + row] : 0.f, sum = 0.f;
   f32x16 acc[2] = {splat(0.f), splat(0.f)};
   const int nt = kend > 0 ? (kend + TILE - 1) / TILE : 0;
+  const bool few = nt <= 2;
+  int t0, t1;
+  split_range(nt, split, a.splits, t0, t1);
+  if (few) t0 = 0, t1 = split == 0 ? nt : 0;   // (the first split alone)
   auto stage = [&](int t) {
     char* p = lds + (t & 1) * 2 * TILE_BYTES;
     stage_tile(p, kp, a.ks[1], t * TILE, nk, wave, lane);
@@ -439,24 +528,26 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_q_kernel(const Args a) {
     for (int r = 0; r < 16; ++r) sum += dp[r];
     return dp;
   };
-  if (nt) stage(0);
-  const bool few = nt <= 2;
-  if (few) {
-    if (nt == 2) stage(1);
+  if (t0 < t1) stage(t0);
+  if (few && t1) {
+    if (t1 == 2) stage(1);
     tile_ready();
-    for (int t = 0; t < nt; ++t)
+    for (int t = 0; t < t1; ++t)
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
-        if (t * TILE + kb * 32 < wend) ds_of(lds + t * 2 * TILE_BYTES, t * TILE, kb);
-    nd -= (sum + __shfl_xor(sum, 32, 64)) * un;
+        if (t * TILE + kb * 32 < wend && w0 < nq) ds_of(lds + t * 2 * TILE_BYTES, t * TILE, kb);
+    sum = (sum + __shfl_xor(sum, 32, 64)) * un;
+    nd -= sum;
   }
-  for (int t = 0; t < nt; ++t) {
+  const float fix = sum;
+  for (int t = t0; t < t1; ++t) {
     const int key0 = t * TILE;
     const char* kt = lds + (t & 1) * 2 * TILE_BYTES;
     if (!few) {
       tile_ready();
-      if (t + 1 < nt) stage(t + 1);
+      if (t + 1 < t1) stage(t + 1);
     }
+    if (w0 >= nq) continue;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       if (key0 + kb * 32 >= wend) continue;
@@ -469,11 +560,18 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_q_kernel(const Args a) {
       }
     }
   }
-  if (!few) nd -= (sum + __shfl_xor(sum, 32, 64)) * un;
-  if (q_ok && hi == 0) a.nd[(long long)bh * a.Lqp + row] = nd;
+  sum = q_ok ? (few ? fix : (sum + __shfl_xor(sum, 32, 64)) * un) : 0.f;
+  if (!few) nd -= sum;
   if (row < a.Lq) {
     if (!q_ok) acc[0] = acc[1] = splat(0.f);
-    store_cols<T>(a.dq + b * a.dqs[0] + (long long)row * a.dqs[1] + h * a.dqs[2], acc, q_ok ? un * a.scale : 0.f, hi);
+    const long long at = (long long)bh * a.Lq + row, pat = (long long)split * a.B * a.H * a.Lq + at;
+    if (a.splits == 1) {
+      store_cols<T>(a.dq + b * a.dqs[0] + (long long)row * a.dqs[1] + h * a.dqs[2], acc, q_ok ? un * a.scale : 0.f, hi);
+      if (q_ok && hi == 0) a.nd[(long long)bh * a.Lqp + row] = nd;
+    } else {
+      store_cols_f32(a.part + pat * HD, acc, q_ok ? un * a.scale : 0.f, hi);
+      if (hi == 0) a.part_row[pat] = sum;
+    }
   }
 }
 
@@ -499,8 +597,8 @@ int check_desc(const dbir_attn_desc* d, const char* name, bool bwd) {
   DBIR_CHECK_ARG(d->B > 0 && d->H > 0 && d->Hkv > 0 && d->Lq > 0 && d->Lk > 0 && d->H % d->Hkv == 0,
                  "%s: bad sizes B %d H %d Hkv %d Lq %d Lk %d", name, d->B, d->H, d->Hkv, d->Lq, d->Lk);
   DBIR_CHECK_ARG(d->Lq <= (1 << 30) && d->Lk <= (1 << 30), "%s: more than 2^30 rows", name);
-  DBIR_CHECK_ARG((long long)d->B * d->H <= 65535 && (long long)cdiv(d->Lq, 128) * d->B * d->H < 2147483647LL &&
-                     (long long)cdiv(d->Lk, 128) * d->B * d->Hkv < 2147483647LL, "%s: grid too large", name);
+  DBIR_CHECK_ARG((long long)d->B * d->H <= 65535 && (long long)cdiv(d->Lq, 128) * d->B * d->H < (1 << 24) &&
+                     (long long)cdiv(d->Lk, 128) * d->B * d->Hkv < (1 << 24), "%s: grid too large", name);
   DBIR_CHECK_ARG(d->scale > 0.f && d->scale < INFINITY, "%s: scale must be positive and finite", name);
   DBIR_CHECK_ARG(d->lse, "%s: null lse", name);
   CHECK_LAYOUT(q, q_stride, Lq, H, false);
@@ -540,62 +638,103 @@ Args to_args(const dbir_attn_desc* d) {
   return a;
 }
 
-// floats of the backward pass's workspace: nl2 | nd | gmax | vmax
-long long bwd_ws_floats(int dtype, int B, int H, int Hkv, int Lq, int Lk) {
-  const long long lqp = ((long long)Lq + 63) / 64 * 64, bh = (long long)B * H;
-  return bh * lqp * 2 + (dtype == DBIR_F16 ? bh * (lqp / 64) + (long long)B * Hkv * ((Lk + 63) / 64) : 0);
+// Splits of `tiles` rounds when `groups` workgroups would run: from 256 (one a CU) on none; else as many as give two a CU, at
+// least two rounds each.  (The sums of the splits cost a pass over splits x rows x 64 floats.)
+int splits_of(long long groups, long long tiles) {
+  if (groups >= 256) return 1;
+  long long s = (512 + groups - 1) / groups;
+  if (s > tiles / 2) s = tiles / 2;
+  return s < 1 ? 1 : (int)s;
 }
+struct Plan {
+  int fwd, q, kv;             // splits
+  long long lqp, rows_floats; // padded queries; nl2 | nd | gmax | vmax
+  long long part_floats;      // the largest of the splits' sums, dq's first
+};
+Plan plan_of(int dtype, int B, int H, int Hkv, int Lq, int Lk) {
+  Plan p;
+  const long long bh = (long long)B * H, bk = (long long)B * Hkv;
+  p.fwd = p.q = splits_of(bh * cdiv(Lq, 128), cdiv(Lk, TILE));
+  p.kv = splits_of(bk * cdiv(Lk, 128), (long long)cdiv(Lq, TILE) * (H / Hkv));
+  p.lqp = ((long long)Lq + 63) / 64 * 64;
+  p.rows_floats = (bh * p.lqp * 2 + (dtype == DBIR_F16 ? bh * (p.lqp / 64) + bk * ((Lk + 63) / 64) : 0) + 3) / 4 * 4;
+  const long long nq = p.q > 1 ? p.q * bh * Lq * (HD + 1) : 0, nk = p.kv > 1 ? p.kv * bk * Lk * 128 : 0;
+  p.part_floats = nq > nk ? nq : nk;
+  return p;
+}
+long long fwd_ws_bytes(const Plan& p, int B, int H, int Lq) { return p.fwd > 1 ? 4LL * p.fwd * B * H * Lq * (HD + 1) : 0; }
 
 }  // namespace
 
 extern "C" int dbir_attention_fwd_ws(int dtype, int B, int H, int Hkv, int Lq, int Lk, long long* bytes) {
-  DBIR_CHECK_ARG(bytes && B > 0 && H > 0 && Hkv > 0 && Lq > 0 && Lk > 0, "dbir_attention_fwd_ws: bad arguments");
-  *bytes = 0;
+  DBIR_CHECK_ARG(bytes && B > 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && Lq > 0 && Lk > 0, "dbir_attention_fwd_ws: bad arguments");
+  *bytes = fwd_ws_bytes(plan_of(dtype, B, H, Hkv, Lq, Lk), B, H, Lq);
   return DBIR_OK;
 }
 
 extern "C" int dbir_attention_bwd_ws(int dtype, int B, int H, int Hkv, int Lq, int Lk, long long* bytes) {
-  DBIR_CHECK_ARG(bytes && B > 0 && H > 0 && Hkv > 0 && Lq > 0 && Lk > 0, "dbir_attention_bwd_ws: bad arguments");
-  *bytes = bwd_ws_floats(dtype, B, H, Hkv, Lq, Lk) * 4;
+  DBIR_CHECK_ARG(bytes && B > 0 && H > 0 && Hkv > 0 && H % Hkv == 0 && Lq > 0 && Lk > 0, "dbir_attention_bwd_ws: bad arguments");
+  const Plan p = plan_of(dtype, B, H, Hkv, Lq, Lk);
+  *bytes = (p.rows_floats + p.part_floats) * 4;
   return DBIR_OK;
 }
 
 extern "C" int dbir_attention_fwd(const dbir_attn_desc* d, void* stream) {
-  if (int rc = check_desc(d, "dbir_attention_fwd", false)) return rc;
-  const Args a = to_args(d);
-  const dim3 grid((unsigned)(cdiv(d->Lq, 128) * d->B * d->H));
+  const char* name = "dbir_attention_fwd";
+  if (int rc = check_desc(d, name, false)) return rc;
+  const Plan p = plan_of(d->dtype, d->B, d->H, d->Hkv, d->Lq, d->Lk);
+  const long long need = fwd_ws_bytes(p, d->B, d->H, d->Lq), rows = (long long)d->B * d->H * d->Lq;
+  DBIR_CHECK_ARG(!need || (d->ws && d->ws_bytes >= need && (reinterpret_cast<uintptr_t>(d->ws) & 15) == 0),
+                 "%s: the workspace must hold %lld bytes, 16-byte aligned", name, need);
+  Args a = to_args(d);
+  a.splits = p.fwd;
+  a.part = reinterpret_cast<float*>(d->ws);
+  a.part_row = a.part + p.fwd * rows * HD;
+  const dim3 grid((unsigned)(cdiv(d->Lq, 128) * d->B * d->H * p.fwd)), gj((unsigned)cdiv(rows, 16));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (d->dtype == DBIR_F16) hipLaunchKernelGGL(attn_fwd_kernel<F16>, grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL(attn_fwd_kernel<BF16>, grid, dim3(256), 0, s, a);
-  DBIR_CHECK_LAUNCH("dbir_attention_fwd");
+  if (d->dtype == DBIR_F16) {
+    hipLaunchKernelGGL(attn_fwd_kernel<F16>, grid, dim3(256), 0, s, a);
+    if (p.fwd > 1) hipLaunchKernelGGL(attn_fwd_join_kernel<F16>, gj, dim3(256), 0, s, a);
+  } else {
+    hipLaunchKernelGGL(attn_fwd_kernel<BF16>, grid, dim3(256), 0, s, a);
+    if (p.fwd > 1) hipLaunchKernelGGL(attn_fwd_join_kernel<BF16>, gj, dim3(256), 0, s, a);
+  }
+  DBIR_CHECK_LAUNCH(name);
   return DBIR_OK;
 }
+
+namespace {
+template <typename T>
+void launch_bwd(Args a, const Plan& p, int f16, hipStream_t s) {
+  const long long bh = (long long)a.B * a.H, bk = (long long)a.B * a.Hkv, nq = bh * a.Lq, nk = bk * a.Lk;
+  const int nqb = a.Lqp / 64, nkb = cdiv(a.Lk, 64);
+  hipLaunchKernelGGL(attn_bwd_rows_kernel<T>, dim3((unsigned)(nqb + (f16 ? nkb : 0)), (unsigned)bh), dim3(256), 0, s, a, nqb, f16);
+  a.splits = p.q;
+  a.part_row = a.part + p.q * nq * HD;
+  hipLaunchKernelGGL(attn_bwd_q_kernel<T>, dim3((unsigned)(cdiv(a.Lq, 128) * bh * p.q)), dim3(256), 0, s, a);
+  if (p.q > 1) hipLaunchKernelGGL((attn_bwd_join_kernel<T, 64>), dim3((unsigned)cdiv(nq, 16)), dim3(256), 0, s, a);
+  a.splits = p.kv;
+  hipLaunchKernelGGL(attn_bwd_kv_kernel<T>, dim3((unsigned)(cdiv(a.Lk, 128) * bk * p.kv)), dim3(256), 0, s, a);
+  if (p.kv > 1) hipLaunchKernelGGL((attn_bwd_join_kernel<T, 128>), dim3((unsigned)cdiv(nk, 8)), dim3(256), 0, s, a);
+}
+}  // namespace
 
 extern "C" int dbir_attention_bwd(const dbir_attn_desc* d, void* stream) {
   const char* name = "dbir_attention_bwd";
   if (int rc = check_desc(d, name, true)) return rc;
-  const long long need = bwd_ws_floats(d->dtype, d->B, d->H, d->Hkv, d->Lq, d->Lk) * 4;
+  const Plan p = plan_of(d->dtype, d->B, d->H, d->Hkv, d->Lq, d->Lk);
+  const long long need = (p.rows_floats + p.part_floats) * 4, bh = (long long)d->B * d->H;
   DBIR_CHECK_ARG(d->ws && d->ws_bytes >= need && (reinterpret_cast<uintptr_t>(d->ws) & 15) == 0,
                  "%s: the workspace must hold %lld bytes, 16-byte aligned", name, need);
   Args a = to_args(d);
-  const long long bh = (long long)d->B * d->H;
-  const int f16 = d->dtype == DBIR_F16, nqb = a.Lqp / 64, nkb = cdiv(d->Lk, 64);
   a.nl2 = reinterpret_cast<float*>(d->ws);
   a.nd = a.nl2 + bh * a.Lqp;
   a.gmax = a.nd + bh * a.Lqp;
-  a.vmax = a.gmax + bh * nqb;
+  a.vmax = a.gmax + bh * (a.Lqp / 64);
+  a.part = a.nl2 + p.rows_floats;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const dim3 g0((unsigned)(nqb + (f16 ? nkb : 0)), (unsigned)bh), g1((unsigned)(cdiv(d->Lk, 128) * d->B * d->Hkv)),
-      g2((unsigned)(cdiv(d->Lq, 128) * d->B * d->H));
-  if (f16) {
-    hipLaunchKernelGGL(attn_bwd_rows_kernel<F16>, g0, dim3(256), 0, s, a, nqb, 1);
-    hipLaunchKernelGGL(attn_bwd_q_kernel<F16>, g2, dim3(256), 0, s, a);
-    hipLaunchKernelGGL(attn_bwd_kv_kernel<F16>, g1, dim3(256), 0, s, a);
-  } else {
-    hipLaunchKernelGGL(attn_bwd_rows_kernel<BF16>, g0, dim3(256), 0, s, a, nqb, 0);
-    hipLaunchKernelGGL(attn_bwd_q_kernel<BF16>, g2, dim3(256), 0, s, a);
-    hipLaunchKernelGGL(attn_bwd_kv_kernel<BF16>, g1, dim3(256), 0, s, a);
-  }
+  if (d->dtype == DBIR_F16) launch_bwd<F16>(a, p, 1, s);
+  else launch_bwd<BF16>(a, p, 0, s);
   DBIR_CHECK_LAUNCH(name);
   return DBIR_OK;
 }

@@ -35,7 +35,7 @@ typedef H16T<F16> F16T;
 typedef H16T<BF16> BF16T;
 
 constexpr int RUN = 64;          // sorted positions of a piece that is summed ahead
-constexpr int RANK_MAX = 4096;   // up to here the sort is one launch that counts for every token how many go before it
+constexpr int RANK_MAX = 16384;  // up to here the sort is one launch that counts for every token how many go before it
 
 __device__ __forceinline__ uint32_t clamp_token(long long t, int vocab) { return (uint32_t)(t < 0 ? 0 : (t >= vocab ? vocab - 1 : t)); }
 
@@ -50,6 +50,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const typename TT::elem*
   const int lpr = 1 << lpr_log;
   const typename TT::elem* t = table + (long long)clamp_token(tokens[row], vocab) * ldt;
   const float* p = pos ? pos + (row % L) * ldp : nullptr;
+#pragma unroll 4
   for (int c = ((int)id & (lpr - 1)) * V; c < W; c += lpr * V) {
     if constexpr (V == 4) {
       float f[4], q[4] = {0.f, 0.f, 0.f, 0.f};
@@ -65,29 +66,46 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const typename TT::elem*
 }
 
 // ------------------------------------------------------------------------------------------------------------- sort
-// rank of each token among all: 64 tokens a workgroup, each wave compares them with a quarter of the tokens
-__global__ __launch_bounds__(256) void embed_rank_kernel(const long long* __restrict__ tokens, int n, int vocab, uint32_t* __restrict__ skey,
-                                                         int* __restrict__ spos) {
-  __shared__ __attribute__((aligned(16))) uint32_t keys[1024];
-  __shared__ int part[4][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.x * 64 + lane;
+// Rank of each token among all: 64 tokens a workgroup, 16 waves that compare them with 256 of every 4096 tokens each.  Of equal tokens the
+// earlier goes first: all that lie before the workgroup's count up to equality, all behind it only below it, and only a wave's own stretch looks
+// at places.  Two instructions a pair: n^2 / (64 lanes x 1024 SIMDs) of them take less than a radix sort's launches up to RANK_MAX.
+__global__ __launch_bounds__(1024) void embed_rank_kernel(const long long* __restrict__ tokens, int n, int vocab, uint32_t* __restrict__ skey,
+                                                          int* __restrict__ spos) {
+  __shared__ __attribute__((aligned(16))) uint32_t keys[4096];
+  __shared__ int part[16][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), first = blockIdx.x * 64, i = first + lane;
   const uint32_t mine = i < n ? clamp_token(tokens[i], vocab) : 0;
   int before = 0;
-  for (int base = 0; base < n; base += 1024) {
+  for (int base = 0; base < n; base += 4096) {
     __syncthreads();
-    for (int j = threadIdx.x; j < 1024; j += 256) keys[j] = base + j < n ? clamp_token(tokens[base + j], vocab) : 0xffffffffu;
+#pragma unroll
+    for (int j = threadIdx.x; j < 4096; j += 1024) keys[j] = base + j < n ? clamp_token(tokens[base + j], vocab) : 0xffffffffu;
     __syncthreads();
-    for (int j = wave * 256; j < wave * 256 + 256; j += 4) {
-      const uint4 k = *reinterpret_cast<const uint4*>(&keys[j]);
-      const int at = base + j;
-      before += (k.x < mine || (k.x == mine && at < i)) + (k.y < mine || (k.y == mine && at + 1 < i)) +
-                (k.z < mine || (k.z == mine && at + 2 < i)) + (k.w < mine || (k.w == mine && at + 3 < i));
+    const uint4* k4 = reinterpret_cast<const uint4*>(keys + wave * 256);
+    const int lo = base + wave * 256;
+    if (lo >= n) continue;
+    if (lo + 256 <= first) {
+#pragma unroll 8
+      for (int j = 0; j < 64; ++j) before += (k4[j].x <= mine) + (k4[j].y <= mine) + (k4[j].z <= mine) + (k4[j].w <= mine);
+    } else if (lo >= first + 64) {
+#pragma unroll 8
+      for (int j = 0; j < 64; ++j) before += (k4[j].x < mine) + (k4[j].y < mine) + (k4[j].z < mine) + (k4[j].w < mine);
+    } else {
+#pragma unroll 4
+      for (int j = 0; j < 64; ++j) {
+        const uint4 k = k4[j];
+        const int at = lo + 4 * j;
+        before += (k.x < mine || (k.x == mine && at < i)) + (k.y < mine || (k.y == mine && at + 1 < i)) +
+                  (k.z < mine || (k.z == mine && at + 2 < i)) + (k.w < mine || (k.w == mine && at + 3 < i));
+      }
     }
   }
   part[wave][lane] = before;
   __syncthreads();
   if (wave == 0 && i < n) {
-    const int r = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+    int r = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) r += part[w][lane];
     skey[r] = mine;
     spos[r] = i;
   }
@@ -110,28 +128,44 @@ __global__ __launch_bounds__(256) void embed_count_kernel(const long long* __res
     for (int d = lane; d < 256; d += 64) hist[sg * 256 + d] = cnt[wave][d];
 }
 
-__global__ __launch_bounds__(256) void embed_place_kernel(const long long* __restrict__ tokens, const uint32_t* __restrict__ key, const int* __restrict__ pos,
-                                                          int n, int vocab, int shift, int seg, int nseg, const int* __restrict__ hist,
-                                                          uint32_t* __restrict__ okey, int* __restrict__ opos) {
-  __shared__ int at[4][256], tot[256];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, sg = blockIdx.x * 4 + wave;
-  int run = 0;
-  for (int s = 0; s < nseg; ++s) {
-    if ((s >> 2) == (int)blockIdx.x) at[s & 3][tid] = run;   // this digit's items in the segments before s
-    run += hist[s * 256 + tid];
+__global__ __launch_bounds__(1024) void embed_place_kernel(const long long* __restrict__ tokens, const uint32_t* __restrict__ key, const int* __restrict__ pos,
+                                                           int n, int vocab, int shift, int seg, int nseg, const int* __restrict__ hist,
+                                                           uint32_t* __restrict__ okey, int* __restrict__ opos) {
+  __shared__ int at[16][256], sums[2][4][256];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, first = blockIdx.x * 16, sg = first + wave, d0 = tid & 255, quarter = tid >> 8;
+  int all = 0, pre = 0;   // this digit's items in a quarter of the segments, and in those of them that lie before this workgroup's
+#pragma unroll 8
+  for (int s = nseg * quarter / 4; s < nseg * (quarter + 1) / 4; ++s) {
+    const int h = hist[s * 256 + d0];
+    all += h;
+    pre += s < first ? h : 0;
   }
-  tot[tid] = run;
+  sums[0][quarter][d0] = all;
+  sums[1][quarter][d0] = pre;
+  __syncthreads();
+  if (tid < 256) {
+    all = (sums[0][0][tid] + sums[0][1][tid]) + (sums[0][2][tid] + sums[0][3][tid]);
+    pre = (sums[1][0][tid] + sums[1][1][tid]) + (sums[1][2][tid] + sums[1][3][tid]);
+    at[0][tid] = all;
+  }
   __syncthreads();
   for (int o = 1; o < 256; o <<= 1) {   // inclusive sums over the digits
-    const int v = tid >= o ? tot[tid - o] : 0;
+    const int v = tid < 256 && tid >= o ? at[0][tid - o] : 0;
     __syncthreads();
-    tot[tid] += v;
+    if (tid < 256) at[0][tid] += v;
     __syncthreads();
   }
-  const int less = tot[tid] - run;
+  if (tid < 256) {
+    int run = at[0][tid] - all + pre;
+    int h[16];
 #pragma unroll
-  for (int s = 0; s < 4; ++s)
-    if (blockIdx.x * 4 + s < nseg) at[s][tid] += less;
+    for (int s = 0; s < 16; ++s) h[s] = first + s < nseg ? hist[(first + s) * 256 + tid] : 0;
+#pragma unroll
+    for (int s = 0; s < 16; ++s) {
+      at[s][tid] = run;
+      run += h[s];
+    }
+  }
   __syncthreads();
   volatile int* mine = at[wave];
   const long long e = min((long long)n, (long long)(sg + 1) * seg);
@@ -161,22 +195,31 @@ __global__ __launch_bounds__(256) void embed_place_kernel(const long long* __res
 // A lane's four columns of a block of 256: adjacent where rows are aligned for it, else 64 apart.
 template <int V>
 __device__ __forceinline__ int col_of(int c0, int lane, int k) { return V == 4 ? c0 + lane * 4 + k : c0 + lane + 64 * k; }
+// adds one row's columns; a lane whose columns do not exist reads others (all lanes stay active) and stores nothing
 template <typename T, int V>
 __device__ __forceinline__ void add_row(const typename T::elem* row, int c0, int lane, int W, float* acc) {
   float f[4];
   if constexpr (V == 4) {
-    T::load4(row + c0 + lane * 4, f);
+    T::load4(row + min(c0 + lane * 4, W - 4), f);
   } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) f[k] = c0 + lane + 64 * k < W ? T::load(row + c0 + lane + 64 * k) : 0.f;
+    for (int k = 0; k < 4; ++k) f[k] = T::load(row + min(c0 + lane + 64 * k, W - 1));
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) acc[k] += f[k];
 }
+// 64 positions are fetched at once, a lane each, so that the rows' loads need not wait for one another
 template <typename T, int V>
 __device__ __forceinline__ void add_items(const typename T::elem* dy, long long ldg, const int* spos, int s, int e, int c0, int lane, int W, float* acc) {
-#pragma unroll 8
-  for (int i = s; i < e; ++i) add_row<T, V>(dy + (long long)spos[i] * ldg, c0, lane, W, acc);
+  for (int i = s; i < e; i += 64) {
+    const int m = min(64, e - i), p = lane < m ? spos[i + lane] : 0;
+    int j = 0;
+    for (; j + 8 <= m; j += 8) {   // (by hand: the compiler unrolls no cross-lane reads)
+#pragma unroll
+      for (int u = 0; u < 8; ++u) add_row<T, V>(dy + (long long)__builtin_amdgcn_readlane(p, j + u) * ldg, c0, lane, W, acc);
+    }
+    for (; j < m; ++j) add_row<T, V>(dy + (long long)__builtin_amdgcn_readlane(p, j) * ldg, c0, lane, W, acc);
+  }
 }
 
 // the sum of sorted positions [piece * RUN, + RUN) where they are one run: a wave a block of 256 columns
@@ -185,7 +228,6 @@ __global__ __launch_bounds__(256) void embed_piece_kernel(const typename T::elem
                                                           const int* __restrict__ spos, float* __restrict__ part, int W, int Wp) {
   const int piece = blockIdx.x, lane = threadIdx.x & 63, c0 = (blockIdx.y * 4 + (threadIdx.x >> 6)) * 256;
   if (c0 >= W || skey[(long long)piece * RUN] != skey[(long long)piece * RUN + RUN - 1]) return;
-  if (V == 4 && c0 + lane * 4 >= W) return;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   add_items<T, V>(dy, ldg, spos, piece * RUN, piece * RUN + RUN, c0, lane, W, acc);
 #pragma unroll
@@ -197,7 +239,7 @@ __global__ __launch_bounds__(256) void embed_piece_kernel(const typename T::elem
 template <typename T, int V>
 __device__ __forceinline__ void add_run(const typename T::elem* dy, long long ldg, const int* spos, const float* part, int Wp, int s, int e, int c0, int lane,
                                         int W, float* acc) {
-  const int ps = (s + RUN - 1) / RUN, pe = e / RUN;
+  const int ps = (s + RUN - 1) / RUN, pe = part ? e / RUN : 0;
   if (ps < pe) {
     add_items<T, V>(dy, ldg, spos, s, ps * RUN, c0, lane, W, acc);
 #pragma unroll 8
@@ -217,16 +259,45 @@ __device__ __forceinline__ int first_at_least(const uint32_t* skey, int n, uint3
   return lo;
 }
 
+// dpos[l] in one block of 256 columns, the waves a quarter of the batch each
+template <typename T, int V>
+__device__ __forceinline__ void pos_block(const typename T::elem* dy, long long ldg, float* dpos, int B, int L, int W, int l, int c0, int lane, int wave,
+                                          float* join) {
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  if (l < L) {
+#pragma unroll 8
+    for (int b = wave; b < B; b += 4) add_row<T, V>(dy + ((long long)b * L + l) * ldg, c0, lane, W, acc);
+  }
+  if (wave) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) join[(wave - 1) * 256 + k * 64 + lane] = acc[k];
+  }
+  __syncthreads();
+  if (wave == 0) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int at = k * 64 + lane;
+      if (col_of<V>(c0, lane, k) < W) dpos[(long long)l * W + col_of<V>(c0, lane, k)] = (acc[k] + join[at]) + (join[256 + at] + join[512 + at]);
+    }
+  }
+}
+
 // SHARED: one row of the table a workgroup, its positions split over the four waves (small tables); else 32 rows, 8 a wave, most of them
-// empty.  One block of 256 columns either way.
+// empty.  One block of 256 columns either way.  The first pos_rows * (blocks of columns) workgroups make dpos.
 template <typename T, int V, bool SHARED>
 __global__ __launch_bounds__(256) void embed_rows_kernel(const typename T::elem* __restrict__ dy, long long ldg, const uint32_t* __restrict__ skey,
                                                          const int* __restrict__ spos, const float* __restrict__ part, float* __restrict__ dtable,
-                                                         long long ldd, float scale, int n, int W, int Wp, int vocab, int padding, int accumulate) {
+                                                         long long ldd, float* __restrict__ dpos, float scale, int n, int L, int W, int Wp, int vocab,
+                                                         int pos_rows, int padding, int accumulate) {
   constexpr int ROWS = SHARED ? 1 : 32;
   __shared__ int first[ROWS + 1];
-  __shared__ float join[SHARED ? 3 : 1][SHARED ? 256 : 1];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c0 = blockIdx.y * 256, v0 = blockIdx.x * ROWS;
+  __shared__ float join[3][256];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c0 = blockIdx.y * 256;
+  if ((int)blockIdx.x < pos_rows) {
+    pos_block<T, V>(dy, ldg, dpos, n / L, L, W, blockIdx.x, c0, lane, wave, &join[0][0]);
+    return;
+  }
+  const int v0 = (blockIdx.x - pos_rows) * ROWS;
   if (threadIdx.x <= ROWS) first[threadIdx.x] = first_at_least(skey, n, (uint32_t)(v0 + threadIdx.x));
   __syncthreads();
   const bool lane_ok = V == 1 || c0 + lane * 4 < W;
@@ -239,11 +310,11 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const typename T::elem*
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
     if (!none) {
       if (SHARED) {   // a quarter of the positions each, whole pieces where there are some
-        const int per = ((e - s + 3) / 4 + (e - s > 8 * RUN ? RUN - 1 : 0)) / (e - s > 8 * RUN ? RUN : 1) * (e - s > 8 * RUN ? RUN : 1);
+        const int unit = e - s > 8 * RUN ? RUN : 1, per = ((e - s + 3) / 4 + unit - 1) / unit * unit;
         s = min(e, s + wave * per);
         e = min(e, s + per);
       }
-      if (lane_ok) add_run<T, V>(dy, ldg, spos, part, Wp, s, e, c0, lane, W, acc);
+      add_run<T, V>(dy, ldg, spos, part, Wp, s, e, c0, lane, W, acc);
       if (SHARED) {
         if (wave) {
 #pragma unroll
@@ -273,23 +344,6 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const typename T::elem*
   }
 }
 
-// dpos[l]: a workgroup a row and block of 256 columns, its waves a quarter of the batch each
-template <typename T, int V>
-__global__ __launch_bounds__(256) void embed_pos_kernel(const typename T::elem* __restrict__ dy, long long ldg, float* __restrict__ dpos, int B, int L, int W) {
-  __shared__ float red[4][256];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c0 = blockIdx.x * 256, l = blockIdx.y;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  if (l < L && !(V == 4 && c0 + lane * 4 >= W)) {
-#pragma unroll 8
-    for (int b = wave; b < B; b += 4) add_row<T, V>(dy + ((long long)b * L + l) * ldg, c0, lane, W, acc);
-  }
-#pragma unroll
-  for (int k = 0; k < 4; ++k) red[wave][V == 4 ? lane * 4 + k : lane + 64 * k] = acc[k];
-  __syncthreads();
-  const int c = threadIdx.x;
-  if (c0 + c < W) dpos[(long long)l * W + c0 + c] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
-}
-
 // ------------------------------------------------------------------------------------------------------------- host
 struct Plan {
   int seg, nseg, passes, pieces, Wp;
@@ -302,7 +356,7 @@ Plan plan_of(int n, int W, int vocab) {
   p.nseg = cdiv(n, p.seg);
   p.passes = 1;
   while (p.passes < 4 && ((long long)(vocab - 1) >> (8 * p.passes)) > 0) ++p.passes;
-  p.pieces = n / RUN;
+  p.pieces = n >= 8 * RUN ? n / RUN : 0;   // (fewer positions: even a run of all of them is short)
   p.Wp = (W + 3) / 4 * 4;
   const long long np = ((long long)n + 3) / 4 * 4;
   p.hist = (n > RANK_MAX ? 4 : 2) * np;
@@ -325,6 +379,7 @@ extern "C" int dbir_embedding_fwd(int table_dtype, const void* table, long long 
   const int nv = v4 ? W / 4 : W;
   int lg = 0;
   while (lg < 6 && (1 << lg) < nv) ++lg;
+  DBIR_CHECK_ARG(((long long)n << lg) <= 0xffffff00LL, "dbir_embedding_fwd: too many tokens for one launch");
   const dim3 grid((unsigned)(((((long long)n) << lg) + 255) / 256));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define GO2(TT, TO, V)                                                                                                                        \
@@ -363,10 +418,11 @@ extern "C" int dbir_embedding_bwd(int dtype, const void* dy, long long ldg, cons
                                   long long ws_bytes, void* stream) {
   DBIR_CHECK_ARG(dy && tokens && dtable && ws && (dpos || pos_rows == 0), "dbir_embedding_bwd: null pointer");
   DBIR_CHECK_ARG(n > 0 && n < (1 << 30) && L > 0 && n % L == 0 && W > 0 && vocab > 0 && ldg >= W && ldd >= W, "dbir_embedding_bwd: bad shape");
-  DBIR_CHECK_ARG(pos_rows == 0 || (pos_rows >= L && pos_rows <= 65535), "dbir_embedding_bwd: pos_rows must be 0 or L .. 65535");
+  DBIR_CHECK_ARG(pos_rows == 0 || (pos_rows >= L && pos_rows < (1 << 23)), "dbir_embedding_bwd: pos_rows must be 0 or L .. 2^23");
   DBIR_CHECK_ARG(dtype >= 0 && dtype <= 2, "dbir_embedding_bwd: bad dtype");
   DBIR_CHECK_ARG(dtable != dy, "dbir_embedding_bwd: dtable must not be dy");
-  DBIR_CHECK_ARG(cdiv(W, 1024) <= 65535, "dbir_embedding_bwd: W too large");
+  DBIR_CHECK_ARG(cdiv(W, 256) <= 65535, "dbir_embedding_bwd: W too large");
+  DBIR_CHECK_ARG(vocab <= (1 << 28), "dbir_embedding_bwd: vocab too large");
   const Plan p = plan_of(n, W, vocab);
   DBIR_CHECK_ARG(ws_bytes >= p.total * 4 && (reinterpret_cast<uintptr_t>(ws) & 15) == 0,
                  "dbir_embedding_bwd: the workspace must hold %lld bytes, 16-byte aligned", p.total * 4);
@@ -376,32 +432,30 @@ extern "C" int dbir_embedding_bwd(int dtype, const void* dy, long long ldg, cons
   uint32_t* key[2] = {w, w + 2 * np};
   int* pos[2] = {reinterpret_cast<int*>(w + np), reinterpret_cast<int*>(w + 3 * np)};
   int* hist = reinterpret_cast<int*>(w + p.hist);
-  float* part = reinterpret_cast<float*>(w + p.part);
+  float* part = p.pieces ? reinterpret_cast<float*>(w + p.part) : nullptr;
   int at = 0;
   if (n <= RANK_MAX) {
-    hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)cdiv(n, 64)), dim3(256), 0, s, tokens, n, vocab, key[0], pos[0]);
+    hipLaunchKernelGGL(embed_rank_kernel, dim3((unsigned)cdiv(n, 64)), dim3(1024), 0, s, tokens, n, vocab, key[0], pos[0]);
   } else {
     for (int pass = 0; pass < p.passes; ++pass) {
       const long long* t = pass == 0 ? tokens : nullptr;
-      const dim3 g((unsigned)cdiv(p.nseg, 4));
-      hipLaunchKernelGGL(embed_count_kernel, g, dim3(256), 0, s, t, key[at], n, vocab, 8 * pass, p.seg, p.nseg, hist);
-      hipLaunchKernelGGL(embed_place_kernel, g, dim3(256), 0, s, t, key[at], pos[at], n, vocab, 8 * pass, p.seg, p.nseg, hist, key[at ^ 1], pos[at ^ 1]);
+      const dim3 g((unsigned)cdiv(p.nseg, 16));
+      hipLaunchKernelGGL(embed_count_kernel, dim3((unsigned)cdiv(p.nseg, 4)), dim3(256), 0, s, t, key[at], n, vocab, 8 * pass, p.seg, p.nseg, hist);
+      hipLaunchKernelGGL(embed_place_kernel, g, dim3(1024), 0, s, t, key[at], pos[at], n, vocab, 8 * pass, p.seg, p.nseg, hist, key[at ^ 1], pos[at ^ 1]);
       at ^= 1;
     }
   }
   const bool v4 = W % 4 == 0 && al(dy, ldg, elem4(dtype)) && al(dtable, ldd, 16);
   const bool shared = vocab <= 8 * 1024;   // below, 32 rows a workgroup do not fill the chip
-  const dim3 gp((unsigned)p.pieces, (unsigned)cdiv(W, 1024)), gr((unsigned)(shared ? vocab : cdiv(vocab, 32)), (unsigned)cdiv(W, 256)), gl((unsigned)cdiv(W, 256), (unsigned)pos_rows);
+  const dim3 gp((unsigned)p.pieces, (unsigned)cdiv(W, 1024)), gr((unsigned)((shared ? vocab : cdiv(vocab, 32)) + pos_rows), (unsigned)cdiv(W, 256));
+#define ROWS(T, V, S)                                                                                                                         \
+  hipLaunchKernelGGL((embed_rows_kernel<T, V, S>), gr, dim3(256), 0, s, (const T::elem*)dy, ldg, key[at], pos[at], part, dtable, ldd, dpos, \
+                     scale, n, L, W, p.Wp, vocab, pos_rows, padding_idx, accumulate)
 #define GO2(T, V)                                                                                                                                \
   do {                                                                                                                                           \
     if (p.pieces) hipLaunchKernelGGL((embed_piece_kernel<T, V>), gp, dim3(256), 0, s, (const T::elem*)dy, ldg, key[at], pos[at], part, W, p.Wp);  \
-    if (shared)                                                                                                                                  \
-      hipLaunchKernelGGL((embed_rows_kernel<T, V, true>), gr, dim3(256), 0, s, (const T::elem*)dy, ldg, key[at], pos[at], part, dtable, ldd,      \
-                         scale, n, W, p.Wp, vocab, padding_idx, accumulate);                                                                     \
-    else                                                                                                                                         \
-      hipLaunchKernelGGL((embed_rows_kernel<T, V, false>), gr, dim3(256), 0, s, (const T::elem*)dy, ldg, key[at], pos[at], part, dtable, ldd,     \
-                         scale, n, W, p.Wp, vocab, padding_idx, accumulate);                                                                     \
-    if (pos_rows) hipLaunchKernelGGL((embed_pos_kernel<T, V>), gl, dim3(256), 0, s, (const T::elem*)dy, ldg, dpos, n / L, L, W);                  \
+    if (shared) ROWS(T, V, true);                                                                                                                \
+    else ROWS(T, V, false);                                                                                                                      \
   } while (0)
 #define GO(T)          \
   do {                 \
@@ -413,6 +467,7 @@ extern "C" int dbir_embedding_bwd(int dtype, const void* dy, long long ldg, cons
   else GO(F32T);
 #undef GO
 #undef GO2
+#undef ROWS
   DBIR_CHECK_LAUNCH("dbir_embedding_bwd");
   return DBIR_OK;
 }

@@ -55,6 +55,19 @@ __device__ __forceinline__ void store_vec(typename T::elem* p, const float* f) {
   if constexpr (V == 1) T::store(p, f[0]);
   else *reinterpret_cast<uint4*>(p) = T::pack(f);
 }
+// gamma / beta: 16 bytes at a time where rows are wide (they are aligned then)
+template <int V>
+__device__ __forceinline__ void load_f32(const float* p, int c, bool ok, float* f) {
+  if constexpr (V == 1) {
+    f[0] = ok ? p[c] : 0.f;
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; e += 4) {
+      const float4 v = ok ? *reinterpret_cast<const float4*>(p + c + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+      f[e] = v.x; f[e + 1] = v.y; f[e + 2] = v.z; f[e + 3] = v.w;
+    }
+  }
+}
 template <int LPR>
 __device__ __forceinline__ float row_sum(float v) {
 #pragma unroll
@@ -89,13 +102,10 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const typename T::elem* __r
   int turn = 0;
   float g[VPL][V], b[VPL][V];
 #pragma unroll
-  for (int i = 0; i < VPL; ++i)
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      const bool ok = l + LPR * i < nv;
-      g[i][e] = ok ? gamma[(l + LPR * i) * V + e] : 0.f;
-      b[i][e] = ok ? beta[(l + LPR * i) * V + e] : 0.f;
-    }
+  for (int i = 0; i < VPL; ++i) {
+    load_f32<V>(gamma, (l + LPR * i) * V, l + LPR * i < nv, g[i]);
+    load_f32<V>(beta, (l + LPR * i) * V, l + LPR * i < nv, b[i]);
+  }
   for (int row = blockIdx.x * GROUPS + threadIdx.x / LPR; row < rows; row += step) {   // (LPR = 256: the same for the whole workgroup)
     const typename T::elem* xr = x + (long long)row * ldx;
     float f[VPL][V], s = 0.f, q = 0.f;
@@ -148,12 +158,11 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const typename T::elem* __r
   int turn = 0;
   float g[VPL][V], sg[VPL][V], sb[VPL][V];
 #pragma unroll
-  for (int i = 0; i < VPL; ++i)
+  for (int i = 0; i < VPL; ++i) {
+    load_f32<V>(gamma, (l + LPR * i) * V, l + LPR * i < nv, g[i]);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      g[i][e] = l + LPR * i < nv ? gamma[(l + LPR * i) * V + e] : 0.f;
-      sg[i][e] = sb[i][e] = 0.f;
-    }
+    for (int e = 0; e < V; ++e) sg[i][e] = sb[i][e] = 0.f;
+  }
   for (int row = blockIdx.x * GROUPS + threadIdx.x / LPR; row < rows; row += step) {
     const float2 st = *reinterpret_cast<const float2*>(stats + 2LL * row);
     float xh[VPL][V], d[VPL][V], r[VPL][V], s1 = 0.f, s2 = 0.f;
@@ -230,23 +239,24 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const typename T::elem* __r
 template <typename T>
 __global__ __launch_bounds__(256) void ln_fwd_any_kernel(const typename T::elem* __restrict__ x, long long ldx, typename T::elem* __restrict__ y,
                                                          long long ldy, const float* __restrict__ gamma, const float* __restrict__ beta,
-                                                         float* __restrict__ stats, int C, float eps) {
+                                                         float* __restrict__ stats, int rows, int C, float eps) {
   __shared__ float red[4];
-  const long long row = blockIdx.x;
-  const typename T::elem* xr = x + row * ldx;
-  float s = 0.f;
-  for (int c = threadIdx.x; c < C; c += 256) s += T::load(xr + c);
-  const float mean = block_sum(s, red) / (float)C;
-  s = 0.f;
-  for (int c = threadIdx.x; c < C; c += 256) {
-    const float d = T::load(xr + c) - mean;
-    s += d * d;
-  }
-  const float rstd = 1.f / sqrtf(block_sum(s, red) / (float)C + eps);
-  for (int c = threadIdx.x; c < C; c += 256) T::store(y + row * ldy + c, (T::load(xr + c) - mean) * rstd * gamma[c] + beta[c]);
-  if (threadIdx.x == 0) {
-    stats[2 * row] = mean;
-    stats[2 * row + 1] = rstd;
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const typename T::elem* xr = x + row * ldx;
+    float s = 0.f;
+    for (int c = threadIdx.x; c < C; c += 256) s += T::load(xr + c);
+    const float mean = block_sum(s, red) / (float)C;
+    s = 0.f;
+    for (int c = threadIdx.x; c < C; c += 256) {
+      const float d = T::load(xr + c) - mean;
+      s += d * d;
+    }
+    const float rstd = 1.f / sqrtf(block_sum(s, red) / (float)C + eps);
+    for (int c = threadIdx.x; c < C; c += 256) T::store(y + row * ldy + c, (T::load(xr + c) - mean) * rstd * gamma[c] + beta[c]);
+    if (threadIdx.x == 0) {
+      stats[2 * row] = mean;
+      stats[2 * row + 1] = rstd;
+    }
   }
 }
 
@@ -254,23 +264,24 @@ template <typename T>
 __global__ __launch_bounds__(256) void ln_bwd_any_kernel(const typename T::elem* __restrict__ dy, long long ldg, const typename T::elem* __restrict__ x,
                                                          long long ldx, const typename T::elem* __restrict__ dres, long long ldr,
                                                          typename T::elem* __restrict__ dx, long long ldd, const float* __restrict__ gamma,
-                                                         const float* __restrict__ stats, int C) {
+                                                         const float* __restrict__ stats, int rows, int C) {
   __shared__ float red[4];
-  const long long row = blockIdx.x;
-  const float mean = stats[2 * row], rstd = stats[2 * row + 1];
-  float s1 = 0.f, s2 = 0.f;
-  for (int c = threadIdx.x; c < C; c += 256) {
-    const float a = T::load(dy + row * ldg + c) * gamma[c];
-    s1 += a;
-    s2 += a * ((T::load(x + row * ldx + c) - mean) * rstd);
-  }
-  s1 = block_sum(s1, red) / (float)C;
-  s2 = block_sum(s2, red) / (float)C;
-  for (int c = threadIdx.x; c < C; c += 256) {
-    const float a = T::load(dy + row * ldg + c) * gamma[c], xh = (T::load(x + row * ldx + c) - mean) * rstd;
-    float d = rstd * (a - s1 - xh * s2);
-    if (dres) d += T::load(dres + row * ldr + c);
-    T::store(dx + row * ldd + c, d);
+  for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
+    const float mean = stats[2 * row], rstd = stats[2 * row + 1];
+    float s1 = 0.f, s2 = 0.f;
+    for (int c = threadIdx.x; c < C; c += 256) {
+      const float a = T::load(dy + row * ldg + c) * gamma[c];
+      s1 += a;
+      s2 += a * ((T::load(x + row * ldx + c) - mean) * rstd);
+    }
+    s1 = block_sum(s1, red) / (float)C;
+    s2 = block_sum(s2, red) / (float)C;
+    for (int c = threadIdx.x; c < C; c += 256) {
+      const float a = T::load(dy + row * ldg + c) * gamma[c], xh = (T::load(x + row * ldx + c) - mean) * rstd;
+      float d = rstd * (a - s1 - xh * s2);
+      if (dres) d += T::load(dres + row * ldr + c);
+      T::store(dx + row * ldd + c, d);
+    }
   }
 }
 
@@ -327,6 +338,7 @@ Shape shape_of(int dtype, int C, bool wide) {
   return nv <= 8 ? Shape{v, 8, 1} : nv <= 32 ? Shape{v, 32, 1} : nv <= 64 ? Shape{v, 32, 2} : nv <= 128 ? Shape{v, 64, 2} : nv <= 192 ? Shape{v, 64, 3} :
          nv <= 320 ? Shape{v, 64, 5} : nv <= 512 ? Shape{v, 256, 2} : nv <= 1024 ? Shape{v, 256, 4} : Shape{0, 0, 0};
 }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 bool is_wide(int dtype, int C, const void* p, long long ld) {
   const int v = dtype == DBIR_F32 ? 4 : 8;
   return C % v == 0 && ld % v == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
@@ -362,7 +374,8 @@ void launch_fwd(const Shape& sh, const void* x, long long ldx, void* y, long lon
                 float eps, hipStream_t s) {
   typedef typename T::elem E;
   if (!sh.v) {
-    hipLaunchKernelGGL(ln_fwd_any_kernel<T>, dim3((unsigned)rows), dim3(256), 0, s, (const E*)x, ldx, (E*)y, ldy, gamma, beta, stats, C, eps);
+    hipLaunchKernelGGL(ln_fwd_any_kernel<T>, dim3((unsigned)(rows < 65536 ? rows : 65536)), dim3(256), 0, s, (const E*)x, ldx, (E*)y, ldy, gamma, beta, stats, rows, C,
+                       eps);
     return;
   }
   const int n = cdiv(rows, 256 / sh.lpr);
@@ -378,8 +391,8 @@ void launch_bwd(const Shape& sh, int n, const void* dy, long long ldg, const voi
                 const float* gamma, const float* stats, float* ws, int rows, int C, hipStream_t s) {
   typedef typename T::elem E;
   if (!sh.v) {
-    hipLaunchKernelGGL(ln_bwd_any_kernel<T>, dim3((unsigned)rows), dim3(256), 0, s, (const E*)dy, ldg, (const E*)x, ldx, (const E*)dres, ldr, (E*)dx, ldd,
-                       gamma, stats, C);
+    hipLaunchKernelGGL(ln_bwd_any_kernel<T>, dim3((unsigned)(rows < 65536 ? rows : 65536)), dim3(256), 0, s, (const E*)dy, ldg, (const E*)x, ldx,
+                       (const E*)dres, ldr, (E*)dx, ldd, gamma, stats, rows, C);
     hipLaunchKernelGGL(ln_cols_any_kernel<T>, dim3((unsigned)cdiv(C, 256), (unsigned)n), dim3(256), 0, s, (const E*)dy, ldg, (const E*)x, ldx, stats, ws,
                        rows, C, cdiv(rows, n));
     return;
@@ -413,7 +426,7 @@ extern "C" int dbir_layernorm_fwd(int dtype, const void* x, long long ldx, void*
   DBIR_CHECK_ARG(dtype >= DBIR_F16 && dtype <= DBIR_F32, "dbir_layernorm_fwd: bad dtype %d", dtype);
   DBIR_CHECK_ARG((reinterpret_cast<uintptr_t>(stats) & 7) == 0, "dbir_layernorm_fwd: stats must be 8-byte aligned");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const Shape sh = shape_of(dtype, C, is_wide(dtype, C, x, ldx) && is_wide(dtype, C, y, ldy));
+  const Shape sh = shape_of(dtype, C, is_wide(dtype, C, x, ldx) && is_wide(dtype, C, y, ldy) && aligned16(gamma) && aligned16(beta));
   if (dtype == DBIR_F16) launch_fwd<F16T>(sh, x, ldx, y, ldy, gamma, beta, stats, rows, C, eps, s);
   else if (dtype == DBIR_BF16) launch_fwd<BF16T>(sh, x, ldx, y, ldy, gamma, beta, stats, rows, C, eps, s);
   else launch_fwd<F32T>(sh, x, ldx, y, ldy, gamma, beta, stats, rows, C, eps, s);
@@ -429,7 +442,7 @@ extern "C" int dbir_layernorm_bwd(int dtype, const void* dy, long long ldg, cons
   DBIR_CHECK_ARG(dx != x && dx != dy && dx != dres, "dbir_layernorm_bwd: dx must not be an input");
   DBIR_CHECK_ARG(dtype >= DBIR_F16 && dtype <= DBIR_F32, "dbir_layernorm_bwd: bad dtype %d", dtype);
   DBIR_CHECK_ARG(((reinterpret_cast<uintptr_t>(stats) & 7) | (reinterpret_cast<uintptr_t>(ws) & 3)) == 0, "dbir_layernorm_bwd: stats must be 8-byte aligned");
-  const bool wide = is_wide(dtype, C, dy, ldg) && is_wide(dtype, C, x, ldx) && is_wide(dtype, C, dx, ldd) && (!dres || is_wide(dtype, C, dres, ldr));
+  const bool wide = aligned16(gamma) && is_wide(dtype, C, dy, ldg) && is_wide(dtype, C, x, ldx) && is_wide(dtype, C, dx, ldd) && (!dres || is_wide(dtype, C, dres, ldr));
   const Shape sh = shape_of(dtype, C, wide);
   const int n = bwd_parts(dtype, rows, C, wide);
   DBIR_CHECK_ARG(ws_bytes >= 8LL * C * n, "dbir_layernorm_bwd: the workspace must hold %lld bytes", 8LL * C * n);

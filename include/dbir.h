@@ -325,7 +325,7 @@ int dbir_layernorm_bwd(int dtype, const void* dy, long long lddy, const void* x,
  *   for n tokens (int64, clamped to [0, vocab)); table and out f16 / bf16 / f32.
  *   Backward: dtable f32 [vocab, W] = scale times the sum of dy over the positions of each token, zeros where there are none or the token is
  *   padding_idx (-1: none); accumulate: added to dtable, rows without a position untouched.  dpos f32 [pos_rows, W] (pos_rows 0, or
- *   L .. 65535): sum of dy over the batch for l < L, zeros behind.  ws: dbir_embedding_bwd_ws bytes, 16-byte aligned. */
+ *   L .. 2^23): sum of dy over the batch for l < L, zeros behind.  ws: dbir_embedding_bwd_ws bytes, 16-byte aligned. */
 int dbir_embedding_fwd(int table_dtype, const void* table, long long ldt, const long long* tokens, const float* pos, long long ldpos,
                        int out_dtype, void* out, long long ldo, float scale, int n, int L, int W, int vocab, void* stream);
 int dbir_embedding_bwd_ws(int n, int W, int vocab, long long* bytes);

@@ -197,7 +197,7 @@ def test_norm_and_embedding_refusals(lib):
         a[i] = v
         assert lib.dbir_embedding_bwd(*a) == 1, (i, v)
     a = list(eb)
-    a[6], a[12] = p, 70000
+    a[6], a[12] = p, 1 << 23
     assert lib.dbir_embedding_bwd(*a) == 1
 
 
