@@ -13,6 +13,9 @@
 // 8 (j >> 2), and the A operand follows that order by reading the row-major tile through two transposing LDS reads of four rows.
 #include <math.h>
 
+#include <type_traits>
+#include <stdlib.h>
+
 #include "common.h"
 
 namespace {
@@ -28,7 +31,7 @@ struct Args {
   long long qs[3], ks[3], vs[3], os[3], gs[3], dqs[3], dks[3], dvs[3];  // batch, row, head strides in elements
   float* lse;             // [B, H, Lq]
   const int *q_len, *kv_len;
-  float *nl2, *nd;        // [B * H, Lqp]: -lse * log2(e) and -D, -inf and 0 behind the last row
+  float *nl2, *nd;        // [B * H, Lqp], from the dq kernel for the other: -lse * log2(e) and -D; -inf and 0 behind the last row
   float *gmax, *vmax;     // f16: per 64 rows the largest row norm of dout / v
   float *part, *part_row; // with several splits: their sums [split][head][row][64] (dk, dv: [128]) and a number per row
   int splits;
@@ -36,13 +39,13 @@ struct Args {
   float scale;
 };
 
-typedef __attribute__((address_space(3))) void* lds_ptr;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((address_space(3))) s16x4* lds_tr;
 
-// A tile is 64 rows of 128 bytes whose 16-byte chunks are permuted by the row: eight consecutive rows put one chunk into eight
-// different places (row reads, 16 bytes a lane) and four consecutive rows put a pair of chunks into disjoint places (transposing reads).
-__device__ __forceinline__ int swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1); }
+// A tile is 64 rows of 128 bytes whose 16-byte chunks are permuted by the row, for 256 bytes a cycle from LDS: of sixteen consecutive rows the even
+// and the odd ones put one chunk into eight different places each (row reads, 16 bytes a lane), and of four consecutive rows two of a
+// kind put four adjacent chunks into disjoint halves (transposing reads).
+__device__ __forceinline__ int swz(int row) { return (((row >> 1) & 1) << 2) | ((row >> 2) & 3); }
 
 // workgroups are dealt to the 8 XCDs in turn: give each XCD a contiguous range of work so that a head's rows stay in one L2
 __device__ __forceinline__ int xcd_range(int w, int n) {
@@ -50,16 +53,33 @@ __device__ __forceinline__ int xcd_range(int w, int n) {
   return x * per + (x < rest ? x : rest) + i;
 }
 
-// 64 rows [row0, row0 + 64) of a head into LDS, straight from memory; rows at or behind `n` arrive as zeros (the descriptor ends there)
+// Loads straight into LDS (lane l's bytes at `to` + l * size), written out so that the compiler does not know of them: it would wait for every load in
+// flight before each read of LDS.  No register is written; tile_ready() waits before the tile is read.
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+__device__ __forceinline__ u32x4 buffer_of(const void* p, int bytes) {   // reads at or behind `bytes` give zeros
+  const uint64_t at = reinterpret_cast<uint64_t>(p);
+  return u32x4{(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at), (uint32_t)__builtin_amdgcn_readfirstlane((int)((uint32_t)(at >> 32) & 0xffffu)),
+               (uint32_t)__builtin_amdgcn_readfirstlane(bytes), 0x00020000u};
+}
+__device__ __forceinline__ uint32_t lds_at(const void* p) {
+  return (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)p);
+}
+__device__ __forceinline__ void load_lds16(uint32_t to, u32x4 buf, int off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(buf) : "memory");
+}
+__device__ __forceinline__ void load_lds4(uint32_t to, u32x4 buf, int off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(to), "v"(off), "s"(buf) : "memory");
+}
+
+// 64 rows [row0, row0 + 64) of a head into LDS; rows at or behind `n` arrive as zeros (the buffer ends there)
 __device__ __forceinline__ void stage_tile(char* tile, const u16* base, long long ld, int row0, int n, int wave, int lane) {
   const int left = n - row0, rows = left < 0 ? 0 : (left > TILE ? TILE : left);
-  const __amdgpu_buffer_rsrc_t srd = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<u16*>(base + (long long)row0 * ld), 0, rows ? (int)((rows - 1) * ld * 2 + HD * 2) : 0, 0x00020000);
+  const u32x4 buf = buffer_of(base + (long long)row0 * ld, rows ? (int)((rows - 1) * ld * 2 + HD * 2) : 0);
+  const uint32_t to = lds_at(tile);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int piece = wave + 4 * i, row = piece * 8 + (lane >> 3);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(srd, (lds_ptr)(tile + piece * 1024), 16,
-                                             (int)(row * ld * 2) + (((lane & 7) ^ swz(lane >> 3)) << 4), 0, 0, 0);
+    load_lds16(to + piece * 1024, buf, (int)(row * ld * 2) + (((lane & 7) ^ swz(row)) << 4));
   }
 }
 
@@ -74,8 +94,9 @@ template <typename T>
 __device__ __forceinline__ typename T::vec8 cols_frag(const char* tile, int k0, int n0, int lane) {
   const int hi = lane >> 5, g = (lane >> 4) & 1, i = lane & 15;
   const int row = 4 * hi + (i >> 2), chunk = (n0 >> 3) + 2 * g + ((i & 3) >> 1);
-  const char* p = tile + (k0 + row) * 128 + ((chunk ^ swz(row)) << 4) + (i & 1) * 8;
-  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr)p), b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr)(p + 8 * 128));
+  const char* p = tile + (k0 + row) * 128 + (i & 1) * 8;   // (k0 is a multiple of 16)
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr)(p + ((chunk ^ swz(row)) << 4)));
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_tr)(p + 8 * 128 + ((chunk ^ swz(row + 8)) << 4)));
   typedef __attribute__((ext_vector_type(8))) short s16x8;
   const s16x8 v = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
   return __builtin_bit_cast(typename T::vec8, v);
@@ -140,30 +161,38 @@ __device__ __forceinline__ void tile_ready() {
 }
 
 // ---------------------------------------------------------------------------------------------------------------- forward
-// 128 queries a workgroup, 32 a wave; keys in tiles of 64, double buffered.  With few workgroups the keys are split over several
+// 128 QB queries a workgroup, 32 QB a wave; keys in tiles of 64, double buffered.  With few workgroups the keys are split over several
 // (host rule): each leaves its normalised sum and lse, attn_fwd_join_kernel weighs them.
-template <typename T>
+// The exponent's reference m need not be the running maximum, only near it: a tile is first taken with the m there is, and only if a lane's sum
+// of 32 comes out above 2^13 (p must stay in f16) it is taken again for the new maximum.  That saves the maximum and the rescaling of the output
+// sums, 54 of 170 vector instructions, in all but the first, the masked and such rare tiles.
+template <typename T, int QB>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Args a) {
+  constexpr int ROWS = 128 * QB;
   __shared__ __attribute__((aligned(16))) char lds[4 * TILE_BYTES];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
-  const int nqb = (a.Lq + 127) >> 7, ws = xcd_range(blockIdx.x, gridDim.x), split = ws % a.splits, w = ws / a.splits;
+  const int nqb = (a.Lq + ROWS - 1) / ROWS, ws = xcd_range(blockIdx.x, gridDim.x), split = ws % a.splits, w = ws / a.splits;
   const int bh = w / nqb, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
   const int qb = a.causal ? nqb - 1 - w % nqb : w % nqb;   // (long rows first)
   const int nk = clamp_len(a.kv_len, b, a.Lk), nq = clamp_len(a.q_len, b, a.Lq), off = a.Lk - a.Lq;
-  const int w0 = qb * 128 + wave * 32, row = w0 + (lane & 31);
-  const bool q_ok = row < nq;
-  int kend = qb * 128 < nq ? nk : 0;
-  if (a.causal) kend = min(kend, min(qb * 128 + 128, nq) + off);
+  const int w0 = qb * ROWS + wave * 32 * QB, row0 = w0 + (lane & 31);
+  int kend = qb * ROWS < nq ? nk : 0;
+  if (a.causal) kend = min(kend, min(qb * ROWS + ROWS, nq) + off);
   const int full = a.causal ? min(nk, w0 + off + 1) : nk;                   // keys that every row of this wave sees
-  const int mine = a.causal ? min(nk, row + off + 1) : nk;                  // keys that this lane's row sees
-  const int wend = a.causal ? min(nk, w0 + 32 + off) : nk;                  // keys that some row of this wave sees
+  const int wend = a.causal ? min(nk, w0 + 32 * QB + off) : nk;             // keys that some row of this wave sees
   const u16* kp = a.k + b * a.ks[0] + hk * a.ks[2];
   const u16* vp = a.v + b * a.vs[0] + hk * a.vs[2];
-  typename T::vec8 qf[4];
-  load_rows<T>(qf, a.q + b * a.qs[0] + (long long)(q_ok ? row : 0) * a.qs[1] + h * a.qs[2], q_ok, hi);
+  typename T::vec8 qf[QB][4];
+  f32x16 acc[QB][2];
+  float m[QB], l[QB];   // the exponent's reference (times c) and this lane's part of the sum
+#pragma unroll
+  for (int i = 0; i < QB; ++i) {
+    const int row = row0 + 32 * i;
+    load_rows<T>(qf[i], a.q + b * a.qs[0] + (long long)(row < nq ? row : 0) * a.qs[1] + h * a.qs[2], row < nq, hi);
+    acc[i][0] = acc[i][1] = splat(0.f);
+    m[i] = l[i] = 0.f;
+  }
   const float c = a.scale * LOG2E;
-  f32x16 acc[2] = {splat(0.f), splat(0.f)};
-  float m = -INFINITY, l = 0.f;   // running maximum (times c) and sum
   int t0, t1;
   split_range(kend > 0 ? (kend + TILE - 1) / TILE : 0, split, a.splits, t0, t1);
   auto stage = [&](int t) {
@@ -171,81 +200,143 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Args a) {
     stage_tile(p, kp, a.ks[1], t * TILE, nk, wave, lane);
     stage_tile(p + TILE_BYTES, vp, a.vs[1], t * TILE, nk, wave, lane);
   };
-  if (t0 < t1) stage(t0);
-  for (int t = t0; t < t1; ++t) {
-    const int key0 = t * TILE;
-    const char *kt = lds + (t & 1) * 2 * TILE_BYTES, *vt = kt + TILE_BYTES;
+  auto enter = [&](int t) {   // every wave, once a tile
     tile_ready();
     if (t + 1 < t1) stage(t + 1);
-    if (key0 >= wend || w0 >= nq) continue;
-    f32x16 s[2] = {splat(0.f), splat(0.f)};
+  };
+  auto score = [&](const char* kt, int kb, f32x16* s) {
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+    for (int i = 0; i < QB; ++i) s[i] = splat(0.f);
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) s[kb] = T::mfma32(rows_frag<T>(kt, kb * 32, ks, lane), qf[ks], s[kb]);
-    if (key0 + TILE > full) {
+    for (int ks = 0; ks < 4; ++ks) {
+      const typename T::vec8 kf = rows_frag<T>(kt, kb * 32, ks, lane);
+#pragma unroll
+      for (int i = 0; i < QB; ++i) s[i] = T::mfma32(kf, qf[i][ks], s[i]);
+    }
+  };
+  auto prob = [&](f32x16& s, float ref) {   // s -> p, their sum over this lane's 16 keys
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, -ref));
+      sum += s[r];
+    }
+    return sum;
+  };
+  if (t0 < t1) stage(t0);
+  bool entered = false;
+  const int hot = w0 < nq ? min(t1, full / TILE) : 0;   // tiles before this are seen whole by every row of the wave
+  for (int t = t0; t < t1; ++t) {
+    if (!entered) enter(t);
+    entered = false;
+    if (w0 >= nq) continue;
+    const char *kt = lds + (t & 1) * 2 * TILE_BYTES, *vt = kt + TILE_BYTES;
+#pragma unroll 1
+    for (int kb = 0; kb < 2; ++kb) {   // the reference becomes the maximum
+      const int key0 = t * TILE + kb * 32;
+      if (key0 >= wend) break;
+      const bool first = t == t0 && kb == 0;
+      f32x16 s[QB];
+      score(kt, kb, s);
+#pragma unroll
+      for (int i = 0; i < QB; ++i) {
+        const int end = (a.causal ? min(nk, row0 + 32 * i + off + 1) : nk) - key0;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          if (row_of(r, hi) >= end) s[i][r] = -INFINITY;
+          mx = fmaxf(mx, s[i][r]);
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
+        const float to = first ? (mx == -INFINITY ? 0.f : mx) : fmaxf(m[i], mx);   // (a row sees the first keys or none)
+        const float al = first ? 0.f : __builtin_amdgcn_exp2f(m[i] - to);
+        m[i] = to;
+        l[i] = l[i] * al + prob(s[i], to);
+#pragma unroll
+        for (int d = 0; d < 2; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[i][d][r] *= al;
+      }
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+        for (int d = 0; d < 2; ++d) {
+          const typename T::vec8 vf = cols_frag<T>(vt, kb * 32 + hf * 16, d * 32, lane);
+#pragma unroll
+          for (int i = 0; i < QB; ++i) acc[i][d] = T::mfma32(vf, pack_frag<T>(s[i], hf), acc[i][d]);
+        }
+    }
+    for (; t + 1 < hot; ++t) {   // the reference stays
+      enter(t + 1);
+      const char *kt = lds + ((t + 1) & 1) * 2 * TILE_BYTES, *vt = kt + TILE_BYTES;
+      typename T::vec8 pf[2][2][QB];
+      float sum[QB], top = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+        f32x16 s[QB];
+        score(kt, kb, s);
+#pragma unroll
+        for (int i = 0; i < QB; ++i) {
+          const float x = prob(s[i], m[i]);
+          sum[i] = kb ? sum[i] + x : x;
+          pf[kb][0][i] = pack_frag<T>(s[i], 0);
+          pf[kb][1][i] = pack_frag<T>(s[i], 1);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < QB; ++i) top = sum[i] <= 8192.f ? top : INFINITY;
+      if (!__all(top == 0.f)) {   // the scores have grown beyond it: this tile once more, with the maximum
+        entered = true;
+        break;
+      }
+#pragma unroll
+      for (int i = 0; i < QB; ++i) l[i] += sum[i];
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (key0 + kb * 32 + row_of(r, hi) >= mine) s[kb][r] = -INFINITY;
+        for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+          for (int d = 0; d < 2; ++d) {
+            const typename T::vec8 vf = cols_frag<T>(vt, kb * 32 + hf * 16, d * 32, lane);
+#pragma unroll
+            for (int i = 0; i < QB; ++i) acc[i][d] = T::mfma32(vf, pf[kb][hf][i], acc[i][d]);
+          }
     }
-    float mx = s[0][0];
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
-    const float mn = fmaxf(m, mx), mu = mn == -INFINITY ? 0.f : mn, al = __builtin_amdgcn_exp2f(m - mu);
-    m = mn;
-    float sum = 0.f;
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[kb][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][r], c, -mu));
-        sum += s[kb][r];
-      }
-    l = l * al + sum + __shfl_xor(sum, 32, 64);
-#pragma unroll
-    for (int d = 0; d < 2; ++d)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[d][r] *= al;
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const typename T::vec8 pf = pack_frag<T>(s[kb], hf);
-#pragma unroll
-        for (int d = 0; d < 2; ++d) acc[d] = T::mfma32(cols_frag<T>(vt, kb * 32 + hf * 16, d * 32, lane), pf, acc[d]);
-      }
   }
-  if (row < a.Lq) {
-    const bool some = q_ok && l != 0.f;   // (a NaN stays one)
-    const float inv = some ? 1.f / l : 0.f, lse = some ? (m + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
-    const long long at = (long long)bh * a.Lq + row, pat = (long long)split * a.B * a.H * a.Lq + at;
-    if (a.splits == 1) store_cols<T>(a.o + b * a.os[0] + (long long)row * a.os[1] + h * a.os[2], acc, inv, hi);
-    else store_cols_f32(a.part + pat * HD, acc, inv, hi);
-    if (hi == 0) (a.splits == 1 ? a.lse + at : a.part_row + pat)[0] = lse;
+#pragma unroll
+  for (int i = 0; i < QB; ++i) {
+    const int row = row0 + 32 * i;
+    const float sum = l[i] + __shfl_xor(l[i], 32, 64);
+    if (row < a.Lq) {
+      const bool some = row < nq && sum != 0.f;   // (a NaN stays one)
+      const float inv = some ? 1.f / sum : 0.f, lse = some ? (m[i] + __builtin_amdgcn_logf(sum)) * LN2 : -INFINITY;
+      const long long at = (long long)bh * a.Lq + row, pat = (long long)split * a.B * a.H * a.Lq + at;
+      if (a.splits == 1) store_cols<T>(a.o + b * a.os[0] + (long long)row * a.os[1] + h * a.os[2], acc[i], inv, hi);
+      else store_cols_f32(a.part + pat * HD, acc[i], inv, hi);
+      if (hi == 0) (a.splits == 1 ? a.lse + at : a.part_row + pat)[0] = lse;
+    }
   }
 }
 
-// 16 rows a workgroup, 16 lanes a row, 4 columns a lane
+// A wave a row: 16 lanes of 4 columns, four of them share the splits.
 template <typename T>
 __global__ __launch_bounds__(256) void attn_fwd_join_kernel(const Args a) {
-  const long long rows = (long long)a.B * a.H * a.Lq, at = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const long long rows = (long long)a.B * a.H * a.Lq, at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (at >= rows) return;
-  const int c = (threadIdx.x & 15) * 4;
-  float m = -INFINITY;
-  bool nan = false;
-  for (int s = 0; s < a.splits; ++s) {
+  const int lane = threadIdx.x & 63, c = (lane & 15) * 4, s0 = lane >> 4;
+  float m = -INFINITY, nan = 0.f;
+  for (int s = lane; s < a.splits; s += 64) {
     const float l = a.part_row[s * rows + at];
     m = fmaxf(m, l);
-    nan |= l != l;
+    nan = l != l ? l : nan;
   }
-  float o[4] = {0.f, 0.f, 0.f, 0.f}, sum = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float w = m == -INFINITY && !nan ? 0.f : __builtin_amdgcn_exp2f((a.part_row[s * rows + at] - m) * LOG2E);
+  m = wave_max(m);
+  nan = wave_sum(nan);   // (0, or NaN where a split has one)
+  const float mu = m == -INFINITY ? 0.f : m;
+  float o[4] = {0.f, 0.f, 0.f, 0.f}, sum = nan;
+#pragma unroll 4
+  for (int s = s0; s < a.splits; s += 4) {
+    const float w = __builtin_amdgcn_exp2f((a.part_row[s * rows + at] - mu) * LOG2E);
     const float4 v = *reinterpret_cast<const float4*>(a.part + (s * rows + at) * HD + c);
     o[0] = __builtin_fmaf(w, v.x, o[0]);
     o[1] = __builtin_fmaf(w, v.y, o[1]);
@@ -253,11 +344,18 @@ __global__ __launch_bounds__(256) void attn_fwd_join_kernel(const Args a) {
     o[3] = __builtin_fmaf(w, v.w, o[3]);
     sum += w;
   }
+#pragma unroll
+  for (int d = 16; d < 64; d <<= 1) {
+    sum += __shfl_xor(sum, d, 64);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] += __shfl_xor(o[i], d, 64);
+  }
+  if (s0) return;
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
   const int row = (int)(at % a.Lq), bh = (int)(at / a.Lq), b = bh / a.H, h = bh % a.H;
   *reinterpret_cast<uint2*>(a.o + b * a.os[0] + (long long)row * a.os[1] + h * a.os[2] + c) =
       make_uint2(T::pack2(o[0] * inv, o[1] * inv), T::pack2(o[2] * inv, o[3] * inv));
-  if (c == 0) a.lse[at] = sum != 0.f ? m + __builtin_amdgcn_logf(sum) * LN2 : -INFINITY;
+  if (c == 0) a.lse[at] = sum != 0.f ? mu + __builtin_amdgcn_logf(sum) * LN2 : -INFINITY;
 }
 
 // the f32 sums of the splits -> 16 bits; WIDTH 64: dq (and the corrections of D), 128: dk and dv
@@ -288,115 +386,85 @@ __global__ __launch_bounds__(256) void attn_bwd_join_kernel(const Args a) {
 
 
 // ---------------------------------------------------------------------------------------------------------------- backward
-// D and the negated statistics of 64 rows, 8 lanes a row; f16 also the largest norms (scale_exp below).
+// f16: p and ds are operands of 11 bits between 2^-14 and 65504, and ds may be far below (4096 keys, a gradient of 1e-3: 1e-6) or, with
+// a loss scale, above.  Both are formed times 2^e, which the result is divided by: |ds| <= 2 max|do| max|v| must stay under 2^15,
+// p under 2^14.  A power of two rounds nothing.  bf16 has the exponents of f32: e = 0.
+__device__ __forceinline__ float exponent_for(float x) {   // x: max|do| max|v|
+  const int ex = (int)((__builtin_bit_cast(uint32_t, x) >> 23) & 255) - 126, e = 14 - ex;   // x < 2^ex
+  return ex > 100 ? 0.f : (float)(e > 14 ? 14 : e);
+}
+// the square of the largest norm of rows [row0, row0 + n) of a head, over 256 threads (8 lanes a row); each thread has a part of it
 template <typename T>
-__global__ __launch_bounds__(256) void attn_bwd_rows_kernel(const Args a, int nqb, int f16) {
-  __shared__ float mx[4];
-  const int tid = threadIdx.x, bh = blockIdx.y, sub = tid & 7, blk = blockIdx.x;
+__device__ __forceinline__ float norm2_part(const u16* base, long long ld, int row0, int n, int tid) {
   float top = 0.f;
+  for (int r = row0 + (tid >> 3); r < row0 + n; r += 32) {
+    float x[8], s = 0.f;
+    unpack8<T>(*reinterpret_cast<const uint4*>(base + (long long)r * ld + (tid & 7) * 8), x);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s += x[e] * x[e];
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+    top = fmaxf(top, s);
+  }
+  return top;
+}
+__device__ __forceinline__ float block_max(float v, float* red, int tid) {
+  v = wave_max(v);
+  __syncthreads();
+  if ((tid & 63) == 0) red[tid >> 6] = v;
+  __syncthreads();
+  return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+// the largest norm of every 64 rows of dout (blocks below nqb) and v
+__global__ __launch_bounds__(256) void attn_bwd_norms_kernel(const Args a, int nqb) {
+  __shared__ float red[4];
+  const int tid = threadIdx.x, bh = blockIdx.y, blk = blockIdx.x;
+  float top;
   if (blk < nqb) {
-    const int b = bh / a.H, h = bh % a.H, nq = clamp_len(a.q_len, b, a.Lq);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = blk * 64 + i * 32 + (tid >> 3);
-      float d = 0.f, n = 0.f;
-      const float lse = row < nq ? a.lse[(long long)bh * a.Lq + row] : -INFINITY;
-      if (row < nq) {
-        float x[8], y[8];
-        unpack8<T>(*reinterpret_cast<const uint4*>(a.dout + b * a.gs[0] + (long long)row * a.gs[1] + h * a.gs[2] + sub * 8), x);
-        unpack8<T>(*reinterpret_cast<const uint4*>(a.o_in + b * a.os[0] + (long long)row * a.os[1] + h * a.os[2] + sub * 8), y);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          d += x[e] * y[e];
-          n += x[e] * x[e];
-        }
-      }
-#pragma unroll
-      for (int o = 4; o > 0; o >>= 1) {
-        d += __shfl_xor(d, o, 64);
-        n += __shfl_xor(n, o, 64);
-      }
-      top = fmaxf(top, n);
-      if (sub == 0) {
-        const bool some = lse != -INFINITY;   // an empty row has no probabilities
-        a.nl2[(long long)bh * a.Lqp + row] = some ? -lse * LOG2E : -INFINITY;
-        a.nd[(long long)bh * a.Lqp + row] = some ? -d : 0.f;
-      }
-    }
+    const int b = bh / a.H, nq = clamp_len(a.q_len, b, a.Lq);
+    top = norm2_part<F16>(a.dout + b * a.gs[0] + (bh % a.H) * a.gs[2], a.gs[1], blk * 64, min(64, nq - blk * 64), tid);
   } else {
     if (bh >= a.B * a.Hkv) return;
-    const int b = bh / a.Hkv, h = bh % a.Hkv, nk = clamp_len(a.kv_len, b, a.Lk);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int row = (blk - nqb) * 64 + i * 32 + (tid >> 3);
-      float n = 0.f;
-      if (row < nk) {
-        float x[8];
-        unpack8<T>(*reinterpret_cast<const uint4*>(a.v + b * a.vs[0] + (long long)row * a.vs[1] + h * a.vs[2] + sub * 8), x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) n += x[e] * x[e];
-      }
-#pragma unroll
-      for (int o = 4; o > 0; o >>= 1) n += __shfl_xor(n, o, 64);
-      top = fmaxf(top, n);
-    }
+    const int b = bh / a.Hkv, nk = clamp_len(a.kv_len, b, a.Lk);
+    top = norm2_part<F16>(a.v + b * a.vs[0] + (bh % a.Hkv) * a.vs[2], a.vs[1], (blk - nqb) * 64, min(64, nk - (blk - nqb) * 64), tid);
   }
-  if (!f16) return;
-  top = wave_max(top);
-  if ((tid & 63) == 0) mx[tid >> 6] = top;
-  __syncthreads();
+  top = sqrtf(block_max(top, red, tid));
   if (tid == 0) {
-    top = sqrtf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
     if (blk < nqb) a.gmax[(long long)bh * nqb + blk] = top;
     else a.vmax[(long long)bh * (gridDim.x - nqb) + blk - nqb] = top;
   }
 }
-
-// f16: p and ds are operands of 11 bits between 2^-14 and 65504, and ds may be far below (4096 keys, a gradient of 1e-3: 1e-6) or, with
-// a loss scale, above.  Both are formed times 2^e, which the result is divided by: |ds| <= 2 max|do| max|v| must stay under 2^15,
-// p under 2^14.  A power of two rounds nothing.  bf16 has the exponents of f32: e = 0.
 template <typename T>
-__device__ __forceinline__ float scale_exp(const Args& a, int b, int hk, int nqb, int nkb, int tid, float* red);
+__device__ __forceinline__ float scale_exp(const Args& a, int b, int hk, int tid, float* red);
 template <>
-__device__ __forceinline__ float scale_exp<BF16>(const Args&, int, int, int, int, int, float*) { return 0.f; }
+__device__ __forceinline__ float scale_exp<BF16>(const Args&, int, int, int, float*) { return 0.f; }
 template <>
-__device__ __forceinline__ float scale_exp<F16>(const Args& a, int b, int hk, int nqb, int nkb, int tid, float* red) {
-  const int grp = a.H / a.Hkv;
+__device__ __forceinline__ float scale_exp<F16>(const Args& a, int b, int hk, int tid, float* red) {   // from the blocks' norms
+  const int grp = a.H / a.Hkv, nqb = a.Lqp / 64, nkb = (a.Lk + 63) >> 6;
   const float* g = a.gmax + (long long)(b * a.H + hk * grp) * nqb;   // the group's heads are adjacent
   const float* v = a.vmax + (long long)(b * a.Hkv + hk) * nkb;
   float x = 0.f, y = 0.f;
   for (int i = tid; i < grp * nqb; i += 256) x = fmaxf(x, g[i]);
   for (int i = tid; i < nkb; i += 256) y = fmaxf(y, v[i]);
-  x = wave_max(x);
-  y = wave_max(y);
-  if ((tid & 63) == 0) {
-    red[tid >> 6] = x;
-    red[4 + (tid >> 6)] = y;
-  }
-  __syncthreads();
-  x = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])) * fmaxf(fmaxf(red[4], red[5]), fmaxf(red[6], red[7]));
-  const int ex = (int)((__builtin_bit_cast(uint32_t, x) >> 23) & 255) - 126;   // x < 2^ex
-  const int e = 14 - ex;
-  return ex > 100 ? 0.f : (float)(e > 14 ? 14 : e);
+  x = block_max(x, red, tid);
+  return exponent_for(x * block_max(y, red, tid));
 }
 
 // dk, dv: 128 keys a workgroup, 32 a wave (their k, v operands and sums stay in registers); queries in tiles of 64, double buffered,
 // over all heads that share these keys; with few workgroups these rounds are split over several (host rule).
-template <typename T>
-__global__ __launch_bounds__(256, 2) void attn_bwd_kv_kernel(const Args a) {
-  __shared__ __attribute__((aligned(16))) char lds[2 * (2 * TILE_BYTES + 512)];
-  __shared__ float red[8];
+constexpr int KV_LDS = 2 * (2 * TILE_BYTES + 512);
+template <typename T, bool CAUSAL>
+__device__ __forceinline__ void kv_part(const Args& a, char* lds, int b, int hk, int k0, int split, float e) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
-  const int nkb = (a.Lk + 127) >> 7, ws = xcd_range(blockIdx.x, gridDim.x), split = ws % a.splits, w = ws / a.splits;
-  const int bh = w / nkb, b = bh / a.Hkv, hk = bh % a.Hkv, grp = a.H / a.Hkv, k0 = (w % nkb) * 128;
+  const int bh = b * a.Hkv + hk, grp = a.H / a.Hkv;
   const int nk = clamp_len(a.kv_len, b, a.Lk), nq = clamp_len(a.q_len, b, a.Lq), off = a.Lk - a.Lq;
   const int key = k0 + wave * 32 + (lane & 31);
   const bool k_ok = key < nk;
   typename T::vec8 kf[4], vf[4];
   load_rows<T>(kf, a.k + b * a.ks[0] + (long long)(k_ok ? key : 0) * a.ks[1] + hk * a.ks[2], k_ok, hi);
   load_rows<T>(vf, a.v + b * a.vs[0] + (long long)(k_ok ? key : 0) * a.vs[1] + hk * a.vs[2], k_ok, hi);
-  const float c = a.scale * LOG2E, e = scale_exp<T>(a, b, hk, a.Lqp / 64, (a.Lk + 63) >> 6, tid, red);
-  const int qt0 = a.causal ? max(0, k0 - off) / TILE : 0, qt1 = k0 < nk ? (nq + TILE - 1) / TILE : 0, nt = max(0, qt1 - qt0);
+  const float c = a.scale * LOG2E;
+  const int qt0 = CAUSAL ? max(0, k0 - off) / TILE : 0, qt1 = k0 < nk ? (nq + TILE - 1) / TILE : 0, nt = max(0, qt1 - qt0);
   f32x16 dk[2] = {splat(0.f), splat(0.f)}, dv[2] = {splat(0.f), splat(0.f)};
   auto stage = [&](int it) {
     const int h = hk * grp + it / nt, q0 = (qt0 + it % nt) * TILE;
@@ -405,58 +473,68 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_kv_kernel(const Args a) {
     stage_tile(p + TILE_BYTES, a.dout + b * a.gs[0] + h * a.gs[2], a.gs[1], q0, nq, wave, lane);
     if (wave < 2) {
       const float* st = (wave ? a.nd : a.nl2) + (long long)(b * a.H + h) * a.Lqp + q0;
-      const __amdgpu_buffer_rsrc_t srd = __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(st), 0, 256, 0x00020000);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(srd, (lds_ptr)(p + 2 * TILE_BYTES + wave * 256), 4, lane * 4, 0, 0, 0);
+      load_lds4(lds_at(p + 2 * TILE_BYTES + wave * 256), buffer_of(st, 256), lane * 4);
     }
   };
   int it0, it1;
   split_range(nt * grp, split, a.splits, it0, it1);
   if (it0 < it1) stage(it0);
-  for (int it = it0; it < it1; ++it) {
-    const char *qt = lds + (it & 1) * (2 * TILE_BYTES + 512), *gt = qt + TILE_BYTES;
+  auto half = [&](auto masked, const char* qt, int q0, int sb) {
+    const char* gt = qt + TILE_BYTES;
     const float* st = reinterpret_cast<const float*>(gt + TILE_BYTES);
-    tile_ready();
-    if (it + 1 < it1) stage(it + 1);
-    if (k0 + wave * 32 >= nk) continue;
-    const int q0 = (qt0 + it % nt) * TILE;
+    f32x16 s = splat(e / c), dp;
 #pragma unroll
-    for (int sb = 0; sb < 2; ++sb) {
-      if (a.causal && q0 + sb * 32 + 31 + off < k0 + wave * 32) continue;   // no row of these sees a key of this wave
-      f32x16 s = splat(e / c), dp;
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(st + 64 + sb * 32 + 8 * g + 4 * hi);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(st + 64 + sb * 32 + 8 * g + 4 * hi);
+      for (int r = 0; r < 4; ++r) dp[4 * g + r] = v[r];
+    }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) dp[4 * g + r] = v[r];
-      }
+    for (int ks = 0; ks < 4; ++ks) {
+      s = T::mfma32(rows_frag<T>(qt, sb * 32, ks, lane), kf[ks], s);
+      dp = T::mfma32(rows_frag<T>(gt, sb * 32, ks, lane), vf[ks], dp);
+    }
 #pragma unroll
-      for (int ks = 0; ks < 4; ++ks) {
-        s = T::mfma32(rows_frag<T>(qt, sb * 32, ks, lane), kf[ks], s);
-        dp = T::mfma32(rows_frag<T>(gt, sb * 32, ks, lane), vf[ks], dp);
-      }
+    for (int g = 0; g < 4; ++g) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(st + sb * 32 + 8 * g + 4 * hi);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 v = *reinterpret_cast<const f32x4*>(st + sb * 32 + 8 * g + 4 * hi);
+      for (int r = 0; r < 4; ++r) s[4 * g + r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + r], c, v[r]));
+    }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[4 * g + r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * g + r], c, v[r]));
-      }
+    for (int r = 0; r < 16; ++r) dp[r] *= s[r];
+    if constexpr (masked) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) dp[r] *= s[r];
-      if (a.causal && q0 + sb * 32 + off < k0 + wave * 32 + 31) {
+      for (int r = 0; r < 16; ++r)
+        if (q0 + sb * 32 + row_of(r, hi) + off < key) s[r] = dp[r] = 0.f;
+    }
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (q0 + sb * 32 + row_of(r, hi) + off < key) s[r] = dp[r] = 0.f;
-      }
+    for (int hf = 0; hf < 2; ++hf) {
+      const typename T::vec8 pf = pack_frag<T>(s, hf), df = pack_frag<T>(dp, hf);
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const typename T::vec8 pf = pack_frag<T>(s, hf), df = pack_frag<T>(dp, hf);
-#pragma unroll
-        for (int d = 0; d < 2; ++d) {
-          dv[d] = T::mfma32(cols_frag<T>(gt, sb * 32 + hf * 16, d * 32, lane), pf, dv[d]);
-          dk[d] = T::mfma32(cols_frag<T>(qt, sb * 32 + hf * 16, d * 32, lane), df, dk[d]);
-        }
+      for (int d = 0; d < 2; ++d) {
+        dv[d] = T::mfma32(cols_frag<T>(gt, sb * 32 + hf * 16, d * 32, lane), pf, dv[d]);
+        dk[d] = T::mfma32(cols_frag<T>(qt, sb * 32 + hf * 16, d * 32, lane), df, dk[d]);
       }
     }
+  };
+  // tiles of queries from here on see every key of the wave (CAUSAL; else all do): loops of their own for the two kinds
+  const int hot = !CAUSAL ? 0 : (max(0, k0 + wave * 32 + 31 - off) + TILE - 1) / TILE - qt0;
+  for (int it = it0, q = nt ? it0 % nt : 0; it < it1;) {
+    for (; it < it1 && q < hot; ++it, ++q) {
+      tile_ready();
+      if (it + 1 < it1) stage(it + 1);
+      if (k0 + wave * 32 >= nk) continue;
+#pragma unroll 1
+      for (int sb = 0; sb < 2; ++sb) half(std::true_type(), lds + (it & 1) * (2 * TILE_BYTES + 512), (qt0 + q) * TILE, sb);
+    }
+    for (; it < it1 && q < nt; ++it, ++q) {
+      tile_ready();
+      if (it + 1 < it1) stage(it + 1);
+      if (k0 + wave * 32 >= nk) continue;
+#pragma unroll 1   // (two in flight do not fit the registers)
+      for (int sb = 0; sb < 2; ++sb) half(std::false_type(), lds + (it & 1) * (2 * TILE_BYTES + 512), 0, sb);
+    }
+    q = 0;
   }
   if (key < a.Lk) {
     const float un = k_ok ? __builtin_amdgcn_exp2f(-e) : 0.f;
@@ -472,18 +550,21 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_kv_kernel(const Args a) {
     }
   }
 }
+template <typename T, bool CAUSAL>
+__global__ __launch_bounds__(256, 2) void attn_bwd_kv_kernel(const Args a) {
+  __shared__ __attribute__((aligned(16))) char lds[KV_LDS];
+  __shared__ float red[4];
+  const int nkb = (a.Lk + 127) >> 7, ws = xcd_range(blockIdx.x, gridDim.x), w = ws / a.splits, bh = w / nkb, b = bh / a.Hkv, hk = bh % a.Hkv;
+  kv_part<T, CAUSAL>(a, lds, b, hk, (w % nkb) * 128, ws % a.splits, scale_exp<T>(a, b, hk, threadIdx.x, red));
+}
 
 // dq: 128 queries a workgroup, 32 a wave; keys in tiles of 64, double buffered.  D = do . o comes from the ROUNDED o, and where one key has
 // most of a row, dp - D is far below D.  The exact D makes sum_j ds_ij zero, so the sum of the ds that are formed with the rounded one is its error:
 // it corrects D for the dk kernel, and rows of up to two tiles (few keys: where it matters most) are gone through once more with the corrected one.
 template <typename T>
-__global__ __launch_bounds__(256, 2) void attn_bwd_q_kernel(const Args a) {
-  __shared__ __attribute__((aligned(16))) char lds[4 * TILE_BYTES];
-  __shared__ float red[8];
+__device__ __forceinline__ void q_part(const Args& a, char* lds, int b, int h, int qb, int split, float e) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
-  const int nqb = (a.Lq + 127) >> 7, ws = xcd_range(blockIdx.x, gridDim.x), split = ws % a.splits, w = ws / a.splits;
-  const int bh = w / nqb, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
-  const int qb = a.causal ? nqb - 1 - w % nqb : w % nqb;
+  const int bh = b * a.H + h, hk = h / (a.H / a.Hkv);
   const int nk = clamp_len(a.kv_len, b, a.Lk), nq = clamp_len(a.q_len, b, a.Lq), off = a.Lk - a.Lq;
   const int w0 = qb * 128 + wave * 32, row = w0 + (lane & 31);
   const bool q_ok = row < nq;
@@ -496,9 +577,29 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_q_kernel(const Args a) {
   typename T::vec8 qf[4], gf[4];
   load_rows<T>(qf, a.q + b * a.qs[0] + (long long)(q_ok ? row : 0) * a.qs[1] + h * a.qs[2], q_ok, hi);
   load_rows<T>(gf, a.dout + b * a.gs[0] + (long long)(q_ok ? row : 0) * a.gs[1] + h * a.gs[2], q_ok, hi);
-  const float c = a.scale * LOG2E, e = scale_exp<T>(a, b, hk, a.Lqp / 64, (a.Lk + 63) >> 6, tid, red), un = __builtin_amdgcn_exp2f(-e);
-  const float nl2 = q_ok ? a.nl2[(long long)bh * a.Lqp + row] + e : -INFINITY;
-  float nd = q_ok ? a.nd[(long long)bh * a.Lqp + row] : 0.f, sum = 0.f;
+  const float c = a.scale * LOG2E, un = __builtin_amdgcn_exp2f(-e);
+  const float lse = q_ok ? a.lse[(long long)bh * a.Lq + row] : -INFINITY;
+  float nd = 0.f, nl2 = lse != -INFINITY ? -lse * LOG2E : -INFINITY, sum = 0.f;   // (an empty row has no probabilities)
+  {
+    typename T::vec8 of[4];
+    load_rows<T>(of, a.o_in + b * a.os[0] + (long long)(q_ok ? row : 0) * a.os[1] + h * a.os[2], q_ok, hi);
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      float x[8], y[8];
+      unpack8<T>(__builtin_bit_cast(uint4, of[ks]), x);
+      unpack8<T>(__builtin_bit_cast(uint4, gf[ks]), y);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) nd -= x[i] * y[i];
+    }
+    nd += __shfl_xor(nd, 32, 64);
+    if (nl2 == -INFINITY) nd = 0.f;
+  }
+  float* const to_nd = a.nd + (long long)bh * a.Lqp + row;
+  if (hi == 0 && split == 0 && row < a.Lqp) {
+    a.nl2[(long long)bh * a.Lqp + row] = nl2;
+    *to_nd = nd;
+  }
+  nl2 += e;
   f32x16 acc[2] = {splat(0.f), splat(0.f)};
   const int nt = kend > 0 ? (kend + TILE - 1) / TILE : 0;
   const bool few = nt <= 2;
@@ -510,7 +611,11 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_q_kernel(const Args a) {
     stage_tile(p, kp, a.ks[1], t * TILE, nk, wave, lane);
     stage_tile(p + TILE_BYTES, vp, a.vs[1], t * TILE, nk, wave, lane);
   };
-  auto ds_of = [&](const char* kt, int key0, int kb) {   // 2^e ds of 32 keys (rows) and the wave's 32 queries
+  if (t0 < t1) stage(t0);
+  if (few && t1 == 2) stage(1);
+  if (few && t1) tile_ready();
+  float fix = 0.f;
+  auto ds_of = [&](auto masked, const char* kt, int key0, int kb) {   // 2^e ds of 32 keys (rows) and the wave's 32 queries
     f32x16 s = splat(0.f), dp = splat(nd);
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
@@ -519,7 +624,7 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_q_kernel(const Args a) {
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r) dp[r] *= __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, nl2));
-    if (key0 + kb * 32 + 32 > full) {
+    if constexpr (masked) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
         if (key0 + kb * 32 + row_of(r, hi) >= mine) dp[r] = 0.f;
@@ -528,36 +633,40 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_q_kernel(const Args a) {
     for (int r = 0; r < 16; ++r) sum += dp[r];
     return dp;
   };
-  if (t0 < t1) stage(t0);
-  if (few && t1) {
-    if (t1 == 2) stage(1);
-    tile_ready();
-    for (int t = 0; t < t1; ++t)
+  auto add_half = [&](const f32x16& ds, const char* kt, int kb) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-        if (t * TILE + kb * 32 < wend && w0 < nq) ds_of(lds + t * 2 * TILE_BYTES, t * TILE, kb);
-    sum = (sum + __shfl_xor(sum, 32, 64)) * un;
-    nd -= sum;
-  }
-  const float fix = sum;
-  for (int t = t0; t < t1; ++t) {
-    const int key0 = t * TILE;
+    for (int hf = 0; hf < 2; ++hf) {
+      const typename T::vec8 df = pack_frag<T>(ds, hf);
+#pragma unroll
+      for (int d = 0; d < 2; ++d) acc[d] = T::mfma32(cols_frag<T>(kt, kb * 32 + hf * 16, d * 32, lane), df, acc[d]);
+    }
+  };
+  int t = few ? -t1 : t0;
+  const int hot = few || w0 >= nq ? t : min(t1, full / TILE);   // tiles before this are seen whole by every row of the wave
+  for (; t < hot; ++t) {
+    tile_ready();
+    if (t + 1 < t1) stage(t + 1);
     const char* kt = lds + (t & 1) * 2 * TILE_BYTES;
+#pragma unroll 1
+    for (int kb = 0; kb < 2; ++kb) add_half(ds_of(std::false_type(), kt, 0, kb), kt, kb);
+  }
+#pragma unroll 1
+  for (; t < t1; ++t) {   // few: the tiles once for the sum (t < 0), once more for dq
+    const int key0 = (t < 0 ? t + t1 : t) * TILE;
+    const char* kt = lds + ((t < 0 ? t + t1 : t) & 1) * 2 * TILE_BYTES;
     if (!few) {
       tile_ready();
       if (t + 1 < t1) stage(t + 1);
+    } else if (t == 0) {
+      fix = (sum + __shfl_xor(sum, 32, 64)) * un;
+      nd -= fix;
     }
     if (w0 >= nq) continue;
-#pragma unroll
+#pragma unroll 1
     for (int kb = 0; kb < 2; ++kb) {
-      if (key0 + kb * 32 >= wend) continue;
-      const f32x16 ds = ds_of(kt, key0, kb);
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        const typename T::vec8 df = pack_frag<T>(ds, hf);
-#pragma unroll
-        for (int d = 0; d < 2; ++d) acc[d] = T::mfma32(cols_frag<T>(kt, kb * 32 + hf * 16, d * 32, lane), df, acc[d]);
-      }
+      if (key0 + kb * 32 >= wend) break;
+      const f32x16 ds = ds_of(std::true_type(), kt, key0, kb);
+      if (t >= 0) add_half(ds, kt, kb);
     }
   }
   sum = q_ok ? (few ? fix : (sum + __shfl_xor(sum, 32, 64)) * un) : 0.f;
@@ -567,12 +676,41 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_q_kernel(const Args a) {
     const long long at = (long long)bh * a.Lq + row, pat = (long long)split * a.B * a.H * a.Lq + at;
     if (a.splits == 1) {
       store_cols<T>(a.dq + b * a.dqs[0] + (long long)row * a.dqs[1] + h * a.dqs[2], acc, q_ok ? un * a.scale : 0.f, hi);
-      if (q_ok && hi == 0) a.nd[(long long)bh * a.Lqp + row] = nd;
+      if (q_ok && hi == 0) *to_nd = nd;
     } else {
       store_cols_f32(a.part + pat * HD, acc, q_ok ? un * a.scale : 0.f, hi);
       if (hi == 0) a.part_row[pat] = sum;
     }
   }
+}
+template <typename T>
+__global__ __launch_bounds__(256, 2) void attn_bwd_q_kernel(const Args a) {
+  __shared__ __attribute__((aligned(16))) char lds[4 * TILE_BYTES];
+  __shared__ float red[4];
+  const int nqb = (a.Lq + 127) >> 7, ws = xcd_range(blockIdx.x, gridDim.x), w = ws / a.splits, bh = w / nqb, b = bh / a.H, h = bh % a.H;
+  q_part<T>(a, lds, b, h, a.causal ? nqb - 1 - w % nqb : w % nqb, ws % a.splits, scale_exp<T>(a, b, h / (a.H / a.Hkv), threadIdx.x, red));
+}
+
+// Up to 128 queries and keys: all of a key head in one workgroup and one launch.
+template <typename T, bool CAUSAL>
+__global__ __launch_bounds__(256, 2) void attn_bwd_small_kernel(const Args a) {
+  __shared__ __attribute__((aligned(16))) char lds[KV_LDS];
+  __shared__ float red[4];
+  const int tid = threadIdx.x, b = blockIdx.x / a.Hkv, hk = blockIdx.x % a.Hkv, grp = a.H / a.Hkv;
+  float e = 0.f;
+  if (std::is_same<T, F16>::value) {
+    float x = 0.f;
+    for (int h = hk * grp; h < hk * grp + grp; ++h)
+      x = fmaxf(x, norm2_part<T>(a.dout + b * a.gs[0] + h * a.gs[2], a.gs[1], 0, clamp_len(a.q_len, b, a.Lq), tid));
+    x = block_max(x, red, tid);
+    e = exponent_for(sqrtf(x) * sqrtf(block_max(norm2_part<T>(a.v + b * a.vs[0] + hk * a.vs[2], a.vs[1], 0, clamp_len(a.kv_len, b, a.Lk), tid), red, tid)));
+  }
+  for (int h = hk * grp; h < hk * grp + grp; ++h) {
+    q_part<T>(a, lds, b, h, 0, 0, e);
+    __threadfence_block();   // its nl2 and nd, for the next part; the tiles in LDS are done with
+    __syncthreads();
+  }
+  kv_part<T, CAUSAL>(a, lds, b, hk, 0, 0, e);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
@@ -648,17 +786,21 @@ int splits_of(long long groups, long long tiles) {
 }
 struct Plan {
   int fwd, q, kv;             // splits
+  int fwd_qb;                 // 32 queries a wave, or 64
+  bool small;                 // backward in one launch
   long long lqp, rows_floats; // padded queries; nl2 | nd | gmax | vmax
   long long part_floats;      // the largest of the splits' sums, dq's first
 };
 Plan plan_of(int dtype, int B, int H, int Hkv, int Lq, int Lk) {
   Plan p;
   const long long bh = (long long)B * H, bk = (long long)B * Hkv;
+  p.fwd_qb = getenv("XQB") ? atoi(getenv("XQB")) : bh * cdiv(Lq, 256) >= 256 ? 2 : 1;
+  p.small = Lq <= 128 && Lk <= 128 && H / Hkv <= 4;
   p.fwd = p.q = splits_of(bh * cdiv(Lq, 128), cdiv(Lk, TILE));
   p.kv = splits_of(bk * cdiv(Lk, 128), (long long)cdiv(Lq, TILE) * (H / Hkv));
   p.lqp = ((long long)Lq + 63) / 64 * 64;
   p.rows_floats = (bh * p.lqp * 2 + (dtype == DBIR_F16 ? bh * (p.lqp / 64) + bk * ((Lk + 63) / 64) : 0) + 3) / 4 * 4;
-  const long long nq = p.q > 1 ? p.q * bh * Lq * (HD + 1) : 0, nk = p.kv > 1 ? p.kv * bk * Lk * 128 : 0;
+  const long long nq = p.q > 1 && !p.small ? p.q * bh * Lq * (HD + 1) : 0, nk = p.kv > 1 && !p.small ? p.kv * bk * Lk * 128 : 0;
   p.part_floats = nq > nk ? nq : nk;
   return p;
 }
@@ -679,6 +821,16 @@ extern "C" int dbir_attention_bwd_ws(int dtype, int B, int H, int Hkv, int Lq, i
   return DBIR_OK;
 }
 
+namespace {
+template <typename T>
+void launch_fwd(const Args& a, const Plan& p, hipStream_t s) {
+  const dim3 grid((unsigned)(cdiv(a.Lq, 128 * p.fwd_qb) * a.B * a.H * p.fwd));
+  if (p.fwd_qb == 2) hipLaunchKernelGGL((attn_fwd_kernel<T, 2>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((attn_fwd_kernel<T, 1>), grid, dim3(256), 0, s, a);
+  if (p.fwd > 1) hipLaunchKernelGGL(attn_fwd_join_kernel<T>, dim3((unsigned)cdiv((long long)a.B * a.H * a.Lq, 4)), dim3(256), 0, s, a);
+}
+}  // namespace
+
 extern "C" int dbir_attention_fwd(const dbir_attn_desc* d, void* stream) {
   const char* name = "dbir_attention_fwd";
   if (int rc = check_desc(d, name, false)) return rc;
@@ -690,15 +842,9 @@ extern "C" int dbir_attention_fwd(const dbir_attn_desc* d, void* stream) {
   a.splits = p.fwd;
   a.part = reinterpret_cast<float*>(d->ws);
   a.part_row = a.part + p.fwd * rows * HD;
-  const dim3 grid((unsigned)(cdiv(d->Lq, 128) * d->B * d->H * p.fwd)), gj((unsigned)cdiv(rows, 16));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (d->dtype == DBIR_F16) {
-    hipLaunchKernelGGL(attn_fwd_kernel<F16>, grid, dim3(256), 0, s, a);
-    if (p.fwd > 1) hipLaunchKernelGGL(attn_fwd_join_kernel<F16>, gj, dim3(256), 0, s, a);
-  } else {
-    hipLaunchKernelGGL(attn_fwd_kernel<BF16>, grid, dim3(256), 0, s, a);
-    if (p.fwd > 1) hipLaunchKernelGGL(attn_fwd_join_kernel<BF16>, gj, dim3(256), 0, s, a);
-  }
+  if (d->dtype == DBIR_F16) launch_fwd<F16>(a, p, s);
+  else launch_fwd<BF16>(a, p, s);
   DBIR_CHECK_LAUNCH(name);
   return DBIR_OK;
 }
@@ -707,14 +853,25 @@ namespace {
 template <typename T>
 void launch_bwd(Args a, const Plan& p, int f16, hipStream_t s) {
   const long long bh = (long long)a.B * a.H, bk = (long long)a.B * a.Hkv, nq = bh * a.Lq, nk = bk * a.Lk;
-  const int nqb = a.Lqp / 64, nkb = cdiv(a.Lk, 64);
-  hipLaunchKernelGGL(attn_bwd_rows_kernel<T>, dim3((unsigned)(nqb + (f16 ? nkb : 0)), (unsigned)bh), dim3(256), 0, s, a, nqb, f16);
+  if (p.small) {
+    const dim3 g((unsigned)bk);
+    a.splits = 1;
+    if (a.causal) hipLaunchKernelGGL((attn_bwd_small_kernel<T, true>), g, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((attn_bwd_small_kernel<T, false>), g, dim3(256), 0, s, a);
+    return;
+  }
+  if (f16) {
+    const int nqb = a.Lqp / 64, nkb = cdiv(a.Lk, 64);
+    hipLaunchKernelGGL(attn_bwd_norms_kernel, dim3((unsigned)(nqb + nkb), (unsigned)bh), dim3(256), 0, s, a, nqb);
+  }
   a.splits = p.q;
   a.part_row = a.part + p.q * nq * HD;
   hipLaunchKernelGGL(attn_bwd_q_kernel<T>, dim3((unsigned)(cdiv(a.Lq, 128) * bh * p.q)), dim3(256), 0, s, a);
   if (p.q > 1) hipLaunchKernelGGL((attn_bwd_join_kernel<T, 64>), dim3((unsigned)cdiv(nq, 16)), dim3(256), 0, s, a);
   a.splits = p.kv;
-  hipLaunchKernelGGL(attn_bwd_kv_kernel<T>, dim3((unsigned)(cdiv(a.Lk, 128) * bk * p.kv)), dim3(256), 0, s, a);
+  const dim3 gk((unsigned)(cdiv(a.Lk, 128) * bk * p.kv));
+  if (a.causal) hipLaunchKernelGGL((attn_bwd_kv_kernel<T, true>), gk, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((attn_bwd_kv_kernel<T, false>), gk, dim3(256), 0, s, a);
   if (p.kv > 1) hipLaunchKernelGGL((attn_bwd_join_kernel<T, 128>), dim3((unsigned)cdiv(nk, 8)), dim3(256), 0, s, a);
 }
 }  // namespace

@@ -694,13 +694,13 @@ def _train_device(what: str, first: T, *others) -> int:
 
 
 def _train_call(name: str, dev: int, *args) -> None:
-    """The C entry on the current stream of the tensors' device."""
+    """The C entry on the current stream of the tensors' device (its raw handle: _stream() costs as much as a launch)."""
     fn = getattr(native.lib(), name)
     if dev == torch.cuda.current_device():
-        rc = fn(*args, _stream())
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, _stream())
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     if rc:
         native.check(rc, name)
 
@@ -710,6 +710,10 @@ def _ws_bytes(name: str, *args) -> int:
     n = ctypes.c_longlong()
     native.check(getattr(native.lib(), name)(*args, ctypes.byref(n)), name)
     return n.value
+
+
+def _dense_like(x: T) -> T:
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
 
 def _row_ld(t: T, what: str) -> int:
@@ -803,7 +807,7 @@ def layernorm_fwd(x: T, gamma: T, beta: T, eps: float = 1e-5, out: Optional[T] =
     gamma / beta f32 [C]."""
     dev = _train_device("layernorm_fwd", x, gamma, beta, out)
     if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        out = _dense_like(x)
     shape, dt = x.shape, _DT3.get(x.dtype)
     C = shape[-1]
     if dt is None or out.dtype != x.dtype or gamma.dtype != torch.float32 or beta.dtype != torch.float32:
@@ -821,7 +825,7 @@ def layernorm_bwd(dy: T, x: T, gamma: T, stats: T, dres: Optional[T] = None, dx:
     norm (a residual connection) is added to dx."""
     dev = _train_device("layernorm_bwd", x, dy, gamma, stats, dres, dx)
     if dx is None:
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dx = _dense_like(x)
     shape, dt = x.shape, _DT3.get(x.dtype)
     C = shape[-1]
     if dt is None or dy.dtype != x.dtype or dx.dtype != x.dtype or (dres is not None and dres.dtype != x.dtype) or gamma.dtype != torch.float32 \

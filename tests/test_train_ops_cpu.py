@@ -27,7 +27,7 @@ def no_launch(monkeypatch):
             return call
 
     monkeypatch.setattr(ops, "_gpu", lambda *ts: None)
-    monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: 0, raising=False)
     monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
     ops._ws_bytes.cache_clear()
     monkeypatch.setattr(native, "_lib", Lib())
