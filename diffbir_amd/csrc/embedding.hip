@@ -40,35 +40,66 @@ constexpr int RANK_MAX = 16384;  // up to here the sort is one launch that count
 __device__ __forceinline__ uint32_t clamp_token(long long t, int vocab) { return (uint32_t)(t < 0 ? 0 : (t >= vocab ? vocab - 1 : t)); }
 
 // ------------------------------------------------------------------------------------------------------------- forward
-// lpr lanes (a power of two) a row, V elements a lane and step
+// lpr lanes (a power of two) a row, V elements a lane and step; a lane group takes FWD_ROWS rows at once: their loads are in flight together, and
+// with positions they are rows of one position (rows `gap` = L apart), which is read once for all of them.
+constexpr int FWD_ROWS = 4;
 template <typename TT, typename TO, int V>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const typename TT::elem* __restrict__ table, long long ldt, const long long* __restrict__ tokens,
                                                         const float* __restrict__ pos, long long ldp, typename TO::elem* __restrict__ out, long long ldo,
-                                                        float scale, int n, int L, int W, int vocab, int lpr_log) {
-  const long long id = (long long)blockIdx.x * 256 + threadIdx.x, row = id >> lpr_log;
-  if (row >= n) return;
+                                                        float scale, int n, int gap, int W, int vocab, int lpr_log) {
+  const long long id = (long long)blockIdx.x * 256 + threadIdx.x, set = id >> lpr_log;
+  const long long row0 = set / gap * gap * FWD_ROWS + set % gap;
+  if (row0 >= n) return;
   const int lpr = 1 << lpr_log;
-  const typename TT::elem* t = table + (long long)clamp_token(tokens[row], vocab) * ldt;
-  const float* p = pos ? pos + (row % L) * ldp : nullptr;
-#pragma unroll 4
-  for (int c = ((int)id & (lpr - 1)) * V; c < W; c += lpr * V) {
-    if constexpr (V == 4) {
-      float f[4], q[4] = {0.f, 0.f, 0.f, 0.f};
-      TT::load4(t + c, f);
-      if (p) F32T::load4(p + c, q);
+  const typename TT::elem* t[FWD_ROWS];
+  bool same = true;   // one token in all of them (padding)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f[e] = __builtin_fmaf(f[e], scale, q[e]);
-      TO::store4(out + row * ldo + c, f);
+  for (int r = 0; r < FWD_ROWS; ++r) {   // (rows that do not exist read the first one's token and store nothing)
+    const long long row = row0 + (long long)r * gap;
+    t[r] = table + (long long)clamp_token(tokens[row < n ? row : row0], vocab) * ldt;
+    same &= t[r] == t[0];
+  }
+  const float* p = pos ? pos + (row0 % gap) * ldp : nullptr;
+#pragma unroll 2
+  for (int c = ((int)id & (lpr - 1)) * V; c < W; c += lpr * V) {
+    float f[FWD_ROWS][V], q[V];
+    if constexpr (V == 4) TT::load4(t[0] + c, f[0]);
+    else f[0][0] = TT::load(t[0] + c);
+    if (same) {
+#pragma unroll
+      for (int r = 1; r < FWD_ROWS; ++r)
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[r][e] = f[0][e];
     } else {
-      TO::store(out + row * ldo + c, __builtin_fmaf(TT::load(t + c), scale, p ? p[c] : 0.f));
+#pragma unroll
+      for (int r = 1; r < FWD_ROWS; ++r) {
+        if constexpr (V == 4) TT::load4(t[r] + c, f[r]);
+        else f[r][0] = TT::load(t[r] + c);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) q[e] = 0.f;
+    if (p) {
+      if constexpr (V == 4) F32T::load4(p + c, q);
+      else q[0] = p[c];
+    }
+#pragma unroll
+    for (int r = 0; r < FWD_ROWS; ++r) {
+      const long long row = row0 + (long long)r * gap;
+#pragma unroll
+      for (int e = 0; e < V; ++e) f[r][e] = __builtin_fmaf(f[r][e], scale, q[e]);
+      if (row < n) {
+        if constexpr (V == 4) TO::store4(out + row * ldo + c, f[r]);
+        else TO::store(out + row * ldo + c, f[r][0]);
+      }
     }
   }
 }
 
 // ------------------------------------------------------------------------------------------------------------- sort
-// Rank of each token among all: 64 tokens a workgroup, 16 waves that compare them with 256 of every 4096 tokens each.  Of equal tokens the
-// earlier goes first: all that lie before the workgroup's count up to equality, all behind it only below it, and only a wave's own stretch looks
-// at places.  Two instructions a pair: n^2 / (64 lanes x 1024 SIMDs) of them take less than a radix sort's launches up to RANK_MAX.
+// Rank of each token among all: 64 tokens a workgroup, 16 waves that compare them with a sixteenth of every 4096 tokens each.  Of equal tokens the
+// earlier goes first: all that lie before the workgroup's count up to equality, all behind it only below it, and only among its own 64 places are
+// compared.  Two instructions a pair: n^2 / (64 lanes x 1024 SIMDs) of them take less than a radix sort's launches up to RANK_MAX.
 __global__ __launch_bounds__(1024) void embed_rank_kernel(const long long* __restrict__ tokens, int n, int vocab, uint32_t* __restrict__ skey,
                                                           int* __restrict__ spos) {
   __shared__ __attribute__((aligned(16))) uint32_t keys[4096];
@@ -81,24 +112,21 @@ __global__ __launch_bounds__(1024) void embed_rank_kernel(const long long* __res
 #pragma unroll
     for (int j = threadIdx.x; j < 4096; j += 1024) keys[j] = base + j < n ? clamp_token(tokens[base + j], vocab) : 0xffffffffu;
     __syncthreads();
-    const uint4* k4 = reinterpret_cast<const uint4*>(keys + wave * 256);
-    const int lo = base + wave * 256;
+    const int per = (min(n - base, 4096) + 63) / 64, off = wave * per * 4, lo = base + off;   // quads of keys a wave
+    const uint4* k4 = reinterpret_cast<const uint4*>(keys + off);
     if (lo >= n) continue;
-    if (lo + 256 <= first) {
+    const int j0 = max(0, min(per, (first - lo) / 4)), j1 = max(j0, min(per, (first + 64 - lo + 3) / 4));
 #pragma unroll 8
-      for (int j = 0; j < 64; ++j) before += (k4[j].x <= mine) + (k4[j].y <= mine) + (k4[j].z <= mine) + (k4[j].w <= mine);
-    } else if (lo >= first + 64) {
-#pragma unroll 8
-      for (int j = 0; j < 64; ++j) before += (k4[j].x < mine) + (k4[j].y < mine) + (k4[j].z < mine) + (k4[j].w < mine);
-    } else {
+    for (int j = 0; j < j0; ++j) before += (k4[j].x <= mine) + (k4[j].y <= mine) + (k4[j].z <= mine) + (k4[j].w <= mine);
 #pragma unroll 4
-      for (int j = 0; j < 64; ++j) {
-        const uint4 k = k4[j];
-        const int at = lo + 4 * j;
-        before += (k.x < mine || (k.x == mine && at < i)) + (k.y < mine || (k.y == mine && at + 1 < i)) +
-                  (k.z < mine || (k.z == mine && at + 2 < i)) + (k.w < mine || (k.w == mine && at + 3 < i));
-      }
+    for (int j = j0; j < j1; ++j) {
+      const uint4 k = k4[j];
+      const int at = lo + 4 * j;
+      before += (k.x < mine || (k.x == mine && at < i)) + (k.y < mine || (k.y == mine && at + 1 < i)) +
+                (k.z < mine || (k.z == mine && at + 2 < i)) + (k.w < mine || (k.w == mine && at + 3 < i));
     }
+#pragma unroll 8
+    for (int j = j1; j < per; ++j) before += (k4[j].x < mine) + (k4[j].y < mine) + (k4[j].z < mine) + (k4[j].w < mine);
   }
   part[wave][lane] = before;
   __syncthreads();
@@ -134,11 +162,13 @@ __global__ __launch_bounds__(1024) void embed_place_kernel(const long long* __re
   __shared__ int at[16][256], sums[2][4][256];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, first = blockIdx.x * 16, sg = first + wave, d0 = tid & 255, quarter = tid >> 8;
   int all = 0, pre = 0;   // this digit's items in a quarter of the segments, and in those of them that lie before this workgroup's
-#pragma unroll 8
-  for (int s = nseg * quarter / 4; s < nseg * (quarter + 1) / 4; ++s) {
-    const int h = hist[s * 256 + d0];
-    all += h;
-    pre += s < first ? h : 0;
+  for (int s0 = nseg * quarter / 4, s1 = nseg * (quarter + 1) / 4; s0 < s1; s0 += 16) {
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      const int s = s0 + u, h = hist[min(s, nseg - 1) * 256 + d0];
+      all += s < s1 ? h : 0;
+      pre += s < s1 && s < first ? h : 0;
+    }
   }
   sums[0][quarter][d0] = all;
   sums[1][quarter][d0] = pre;
@@ -146,17 +176,21 @@ __global__ __launch_bounds__(1024) void embed_place_kernel(const long long* __re
   if (tid < 256) {
     all = (sums[0][0][tid] + sums[0][1][tid]) + (sums[0][2][tid] + sums[0][3][tid]);
     pre = (sums[1][0][tid] + sums[1][1][tid]) + (sums[1][2][tid] + sums[1][3][tid]);
-    at[0][tid] = all;
   }
   __syncthreads();
-  for (int o = 1; o < 256; o <<= 1) {   // inclusive sums over the digits
-    const int v = tid < 256 && tid >= o ? at[0][tid - o] : 0;
-    __syncthreads();
-    if (tid < 256) at[0][tid] += v;
-    __syncthreads();
-  }
+  int run = all;   // inclusive sums over the digits: within a wave, then the waves before
   if (tid < 256) {
-    int run = at[0][tid] - all + pre;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int v = __shfl_up(run, o, 64);
+      run += lane >= o ? v : 0;
+    }
+    if (lane == 63) sums[0][0][wave] = run;
+  }
+  __syncthreads();
+  if (tid < 256) {
+    run += pre - all;
+    for (int w = 0; w < wave; ++w) run += sums[0][0][w];
     int h[16];
 #pragma unroll
     for (int s = 0; s < 16; ++s) h[s] = first + s < nseg ? hist[(first + s) * 256 + tid] : 0;
@@ -169,10 +203,19 @@ __global__ __launch_bounds__(1024) void embed_place_kernel(const long long* __re
   __syncthreads();
   volatile int* mine = at[wave];
   const long long e = min((long long)n, (long long)(sg + 1) * seg);
+  uint32_t next_k = 0;
+  int next_p = 0;
+  auto fetch = [&](long long i) {   // the next 64 items, while these are placed
+    next_k = i < e ? (tokens ? clamp_token(tokens[i], vocab) : key[i]) : 0;
+    next_p = i < e ? (tokens ? (int)i : pos[i]) : 0;
+  };
+  if ((long long)sg * seg < e) fetch((long long)sg * seg + lane);
   for (long long i0 = (long long)sg * seg; i0 < e; i0 += 64) {
     const long long i = i0 + lane;
     const bool ok = i < e;
-    const uint32_t k = ok ? (tokens ? clamp_token(tokens[i], vocab) : key[i]) : 0;
+    const uint32_t k = next_k;
+    const int p = next_p;
+    if (i0 + 64 < e) fetch(i + 64);
     const int d = (k >> shift) & 255;
     unsigned long long same = __ballot(ok);
 #pragma unroll
@@ -186,7 +229,7 @@ __global__ __launch_bounds__(1024) void embed_place_kernel(const long long* __re
       if (r == 0) mine[d] = to + __popcll(same);   // the first of a digit moves it on for the next 64
       __builtin_amdgcn_wave_barrier();
       okey[to] = k;
-      opos[to] = tokens ? (int)i : pos[i];
+      opos[to] = p;
     }
   }
 }
@@ -235,7 +278,7 @@ __global__ __launch_bounds__(256) void embed_piece_kernel(const typename T::elem
     if (col_of<V>(c0, lane, k) < W) part[(long long)piece * Wp + col_of<V>(c0, lane, k)] = acc[k];
 }
 
-// the sum of sorted positions [s, e) of one token: single ones up to the first whole piece, pieces, single ones again
+// the sum of sorted positions [s, e) of one token: single ones up to the first whole piece, pieces (where there are any), single ones again
 template <typename T, int V>
 __device__ __forceinline__ void add_run(const typename T::elem* dy, long long ldg, const int* spos, const float* part, int Wp, int s, int e, int c0, int lane,
                                         int W, float* acc) {
@@ -259,75 +302,56 @@ __device__ __forceinline__ int first_at_least(const uint32_t* skey, int n, uint3
   return lo;
 }
 
-// dpos[l] in one block of 256 columns, the waves a quarter of the batch each
-template <typename T, int V>
-__device__ __forceinline__ void pos_block(const typename T::elem* dy, long long ldg, float* dpos, int B, int L, int W, int l, int c0, int lane, int wave,
-                                          float* join) {
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  if (l < L) {
-#pragma unroll 8
-    for (int b = wave; b < B; b += 4) add_row<T, V>(dy + ((long long)b * L + l) * ldg, c0, lane, W, acc);
-  }
+// sums the waves' columns into wave 0's
+template <int NW>
+__device__ __forceinline__ void join_waves(float* acc, float (*join)[256], int lane, int wave) {
   if (wave) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) join[(wave - 1) * 256 + k * 64 + lane] = acc[k];
+    for (int k = 0; k < 4; ++k) join[wave - 1][k * 64 + lane] = acc[k];
   }
   __syncthreads();
   if (wave == 0) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int at = k * 64 + lane;
-      if (col_of<V>(c0, lane, k) < W) dpos[(long long)l * W + col_of<V>(c0, lane, k)] = (acc[k] + join[at]) + (join[256 + at] + join[512 + at]);
-    }
+    for (int w = 0; w < NW - 1; ++w)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) acc[k] += join[w][k * 64 + lane];
   }
 }
 
-// SHARED: one row of the table a workgroup, its positions split over the four waves (small tables); else 32 rows, 8 a wave, most of them
-// empty.  One block of 256 columns either way.  The first pos_rows * (blocks of columns) workgroups make dpos.
-template <typename T, int V, bool SHARED>
-__global__ __launch_bounds__(256) void embed_rows_kernel(const typename T::elem* __restrict__ dy, long long ldg, const uint32_t* __restrict__ skey,
-                                                         const int* __restrict__ spos, const float* __restrict__ part, float* __restrict__ dtable,
-                                                         long long ldd, float* __restrict__ dpos, float scale, int n, int L, int W, int Wp, int vocab,
-                                                         int pos_rows, int padding, int accumulate) {
-  constexpr int ROWS = SHARED ? 1 : 32;
+// NW = 4: one row of the table a workgroup, its positions split over the waves (small tables); NW = 16: 128 rows, 8 a wave, most of them empty,
+// and runs of more than RUN positions split over the waves.  One block of 256 columns either way.  The first pos_rows * (blocks of columns)
+// workgroups make dpos[l], the waves a part of the batch each.  Blocks of columns are adjacent workgroups, so that a long run's all start early.
+template <typename T, int V, int NW>
+__global__ __launch_bounds__(NW * 64) void embed_rows_kernel(const typename T::elem* __restrict__ dy, long long ldg, const uint32_t* __restrict__ skey,
+                                                             const int* __restrict__ spos, const float* __restrict__ part, float* __restrict__ dtable,
+                                                             long long ldd, float* __restrict__ dpos, float scale, int n, int L, int W, int Wp, int vocab,
+                                                             int pos_rows, int padding, int accumulate) {
+  constexpr int ROWS = NW == 4 ? 1 : NW * 8, LONG = NW == 4 ? 0 : RUN;
   __shared__ int first[ROWS + 1];
-  __shared__ float join[3][256];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c0 = blockIdx.y * 256;
-  if ((int)blockIdx.x < pos_rows) {
-    pos_block<T, V>(dy, ldg, dpos, n / L, L, W, blockIdx.x, c0, lane, wave, &join[0][0]);
+  __shared__ float join[NW - 1][256];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ncb = (W + 255) / 256, c0 = (int)(blockIdx.x % ncb) * 256;
+  const int blk = (int)(blockIdx.x / ncb);
+  if (blk < pos_rows) {
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    if (blk < L) {
+#pragma unroll 8
+      for (int b = wave; b < n / L; b += NW) add_row<T, V>(dy + ((long long)b * L + blk) * ldg, c0, lane, W, acc);
+    }
+    join_waves<NW>(acc, join, lane, wave);
+    if (wave == 0) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (col_of<V>(c0, lane, k) < W) dpos[(long long)blk * W + col_of<V>(c0, lane, k)] = acc[k];
+    }
     return;
   }
-  const int v0 = (blockIdx.x - pos_rows) * ROWS;
-  if (threadIdx.x <= ROWS) first[threadIdx.x] = first_at_least(skey, n, (uint32_t)(v0 + threadIdx.x));
+  const int v0 = (blk - pos_rows) * ROWS;
+  if ((int)threadIdx.x <= ROWS) first[threadIdx.x] = first_at_least(skey, n, (uint32_t)(v0 + threadIdx.x));
   __syncthreads();
-  const bool lane_ok = V == 1 || c0 + lane * 4 < W;
-  for (int r = SHARED ? 0 : wave * 8; r < (SHARED ? 1 : wave * 8 + 8); ++r) {
-    const int v = v0 + r;
-    if (v >= vocab) return;
-    int s = __builtin_amdgcn_readfirstlane(first[r]), e = __builtin_amdgcn_readfirstlane(first[r + 1]);
-    const bool none = s == e || v == padding;
-    if (none && accumulate) continue;
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
-    if (!none) {
-      if (SHARED) {   // a quarter of the positions each, whole pieces where there are some
-        const int unit = e - s > 8 * RUN ? RUN : 1, per = ((e - s + 3) / 4 + unit - 1) / unit * unit;
-        s = min(e, s + wave * per);
-        e = min(e, s + per);
-      }
-      add_run<T, V>(dy, ldg, spos, part, Wp, s, e, c0, lane, W, acc);
-      if (SHARED) {
-        if (wave) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) join[wave - 1][k * 64 + lane] = acc[k];
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < 4; ++k) acc[k] = (acc[k] + join[0][k * 64 + lane]) + (join[1][k * 64 + lane] + join[2][k * 64 + lane]);
-      }
-    }
-    if ((SHARED && wave) || !lane_ok) continue;
+  auto write = [&](int v, const float* acc) {
     float* d = dtable + (long long)v * ldd;
     if constexpr (V == 4) {
+      if (c0 + lane * 4 >= W) return;
       float f[4] = {0.f, 0.f, 0.f, 0.f};
       if (accumulate) F32T::load4(d + c0 + lane * 4, f);
 #pragma unroll
@@ -341,6 +365,30 @@ __global__ __launch_bounds__(256) void embed_rows_kernel(const typename T::elem*
           *p = __builtin_fmaf(acc[k], scale, accumulate ? *p : 0.f);
         }
     }
+  };
+#pragma unroll
+  for (int r0 = 0; r0 < ROWS; r0 += 64) {   // long runs: a part of the positions a wave, whole pieces where that gives each one
+    const int r = r0 + lane;
+    unsigned long long todo = __ballot(r < ROWS && first[min(r + 1, ROWS)] - first[min(r, ROWS)] > LONG && v0 + r != padding);
+    while (todo) {
+      const int at = r0 + __builtin_ctzll(todo), s0 = __builtin_amdgcn_readfirstlane(first[at]), e0 = __builtin_amdgcn_readfirstlane(first[at + 1]);
+      todo &= todo - 1;
+      const int unit = e0 - s0 > 2 * NW * RUN ? RUN : 1, per = ((e0 - s0 + NW - 1) / NW + unit - 1) / unit * unit;
+      const int s = min(e0, s0 + wave * per), e = min(e0, s + per);
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      add_run<T, V>(dy, ldg, spos, part, Wp, s, e, c0, lane, W, acc);
+      join_waves<NW>(acc, join, lane, wave);
+      if (wave == 0) write(v0 + at, acc);
+      __syncthreads();
+    }
+  }
+  for (int r = NW == 4 ? wave : wave * 8; r < (NW == 4 ? 1 : wave * 8 + 8); ++r) {
+    const int v = v0 + r, s = __builtin_amdgcn_readfirstlane(first[r]), e = __builtin_amdgcn_readfirstlane(first[r + 1]);
+    const bool none = s == e || v == padding;
+    if (v >= vocab || (none && accumulate) || (!none && e - s > LONG)) continue;
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    if (!none) add_items<T, V>(dy, ldg, spos, s, e, c0, lane, W, acc);
+    write(v, acc);
   }
 }
 
@@ -373,18 +421,21 @@ extern "C" int dbir_embedding_fwd(int table_dtype, const void* table, long long 
                                   int out_dtype, void* out, long long ldo, float scale, int n, int L, int W, int vocab, void* stream) {
   DBIR_CHECK_ARG(table && tokens && out, "dbir_embedding_fwd: null pointer");
   DBIR_CHECK_ARG(n > 0 && n < (1 << 30) && L > 0 && W > 0 && vocab > 0 && ldt >= W && ldo >= W && (!pos || ldp >= W), "dbir_embedding_fwd: bad shape");
+  DBIR_CHECK_ARG(n % L == 0, "dbir_embedding_fwd: n must be a multiple of L");
   DBIR_CHECK_ARG(table_dtype >= 0 && table_dtype <= 2 && out_dtype >= 0 && out_dtype <= 2, "dbir_embedding_fwd: bad dtype");
   DBIR_CHECK_ARG(out != table && out != (const void*)pos, "dbir_embedding_fwd: out must not be an input");
   const bool v4 = W % 4 == 0 && al(table, ldt, elem4(table_dtype)) && al(out, ldo, elem4(out_dtype)) && (!pos || al(pos, ldp, 16));
   const int nv = v4 ? W / 4 : W;
   int lg = 0;
   while (lg < 6 && (1 << lg) < nv) ++lg;
-  DBIR_CHECK_ARG(((long long)n << lg) <= 0xffffff00LL, "dbir_embedding_fwd: too many tokens for one launch");
-  const dim3 grid((unsigned)(((((long long)n) << lg) + 255) / 256));
+  const int gap = pos ? L : 1;
+  const long long sets = (long long)cdiv(n, (long long)gap * FWD_ROWS) * gap;
+  DBIR_CHECK_ARG((sets << lg) <= 0xffffff00LL, "dbir_embedding_fwd: too many tokens for one launch");
+  const dim3 grid((unsigned)(((sets << lg) + 255) / 256));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
 #define GO2(TT, TO, V)                                                                                                                        \
   hipLaunchKernelGGL((embed_fwd_kernel<TT, TO, V>), grid, dim3(256), 0, s, (const TT::elem*)table, ldt, tokens, pos, ldp, (TO::elem*)out, ldo, \
-                     scale, n, L, W, vocab, lg)
+                     scale, n, gap, W, vocab, lg)
 #define GO(TT, TO)          \
   do {                      \
     if (v4) GO2(TT, TO, 4); \
@@ -421,8 +472,7 @@ extern "C" int dbir_embedding_bwd(int dtype, const void* dy, long long ldg, cons
   DBIR_CHECK_ARG(pos_rows == 0 || (pos_rows >= L && pos_rows < (1 << 23)), "dbir_embedding_bwd: pos_rows must be 0 or L .. 2^23");
   DBIR_CHECK_ARG(dtype >= 0 && dtype <= 2, "dbir_embedding_bwd: bad dtype");
   DBIR_CHECK_ARG(dtable != dy, "dbir_embedding_bwd: dtable must not be dy");
-  DBIR_CHECK_ARG(cdiv(W, 256) <= 65535, "dbir_embedding_bwd: W too large");
-  DBIR_CHECK_ARG(vocab <= (1 << 28), "dbir_embedding_bwd: vocab too large");
+  DBIR_CHECK_ARG(cdiv(W, 1024) <= 65535, "dbir_embedding_bwd: W too large");
   const Plan p = plan_of(n, W, vocab);
   DBIR_CHECK_ARG(ws_bytes >= p.total * 4 && (reinterpret_cast<uintptr_t>(ws) & 15) == 0,
                  "dbir_embedding_bwd: the workspace must hold %lld bytes, 16-byte aligned", p.total * 4);
@@ -446,16 +496,18 @@ extern "C" int dbir_embedding_bwd(int dtype, const void* dy, long long ldg, cons
     }
   }
   const bool v4 = W % 4 == 0 && al(dy, ldg, elem4(dtype)) && al(dtable, ldd, 16);
-  const bool shared = vocab <= 8 * 1024;   // below, 32 rows a workgroup do not fill the chip
-  const dim3 gp((unsigned)p.pieces, (unsigned)cdiv(W, 1024)), gr((unsigned)((shared ? vocab : cdiv(vocab, 32)) + pos_rows), (unsigned)cdiv(W, 256));
+  const bool small = vocab <= 8 * 1024;   // 128 rows a workgroup would not fill the chip
+  const long long groups = (small ? vocab : cdiv(vocab, 128)) + (long long)pos_rows;
+  DBIR_CHECK_ARG(groups * cdiv(W, 256) < (1 << 22), "dbir_embedding_bwd: table too large for one launch");
+  const dim3 gp((unsigned)p.pieces, (unsigned)cdiv(W, 1024)), gr((unsigned)(groups * cdiv(W, 256)));
 #define ROWS(T, V, S)                                                                                                                         \
-  hipLaunchKernelGGL((embed_rows_kernel<T, V, S>), gr, dim3(256), 0, s, (const T::elem*)dy, ldg, key[at], pos[at], part, dtable, ldd, dpos, \
+  hipLaunchKernelGGL((embed_rows_kernel<T, V, S>), gr, dim3(S * 64), 0, s, (const T::elem*)dy, ldg, key[at], pos[at], part, dtable, ldd, dpos, \
                      scale, n, L, W, p.Wp, vocab, pos_rows, padding_idx, accumulate)
 #define GO2(T, V)                                                                                                                                \
   do {                                                                                                                                           \
     if (p.pieces) hipLaunchKernelGGL((embed_piece_kernel<T, V>), gp, dim3(256), 0, s, (const T::elem*)dy, ldg, key[at], pos[at], part, W, p.Wp);  \
-    if (shared) ROWS(T, V, true);                                                                                                                \
-    else ROWS(T, V, false);                                                                                                                      \
+    if (small) ROWS(T, V, 4);                                                                                                                    \
+    else ROWS(T, V, 16);                                                                                                                         \
   } while (0)
 #define GO(T)          \
   do {                 \

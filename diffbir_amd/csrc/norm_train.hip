@@ -55,6 +55,17 @@ __device__ __forceinline__ void store_vec(typename T::elem* p, const float* f) {
   if constexpr (V == 1) T::store(p, f[0]);
   else *reinterpret_cast<uint4*>(p) = T::pack(f);
 }
+// a vector as it lies in memory
+template <typename T, int V>
+struct Raw {
+  typedef uint4 type;
+  static __device__ __forceinline__ void unpack(const uint4& v, float* f) { T::unpack(v, f); }
+};
+template <typename T>
+struct Raw<T, 1> {
+  typedef typename T::elem type;
+  static __device__ __forceinline__ void unpack(const type& v, float* f) { f[0] = T::load(&v); }
+};
 // gamma / beta: 16 bytes at a time where rows are wide (they are aligned then)
 template <int V>
 __device__ __forceinline__ void load_f32(const float* p, int c, bool ok, float* f) {
@@ -163,21 +174,34 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const typename T::elem* __r
 #pragma unroll
     for (int e = 0; e < V; ++e) sg[i][e] = sb[i][e] = 0.f;
   }
-  for (int row = blockIdx.x * GROUPS + threadIdx.x / LPR; row < rows; row += step) {
-    const float2 st = *reinterpret_cast<const float2*>(stats + 2LL * row);
+  typename Raw<T, V>::type rx[VPL], rd[VPL], rr[VPL];   // the next row, in flight while this one is summed
+  float2 st_next;
+  auto fetch = [&](int row) {
+    st_next = *reinterpret_cast<const float2*>(stats + 2LL * row);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      const int c = min(l + LPR * i, nv - 1) * V;   // (lanes without a column read the last one and drop it)
+      rx[i] = *reinterpret_cast<const typename Raw<T, V>::type*>(x + (long long)row * ldx + c);
+      rd[i] = *reinterpret_cast<const typename Raw<T, V>::type*>(dy + (long long)row * ldg + c);
+      if (dres) rr[i] = *reinterpret_cast<const typename Raw<T, V>::type*>(dres + (long long)row * ldr + c);
+    }
+  };
+  int row = blockIdx.x * GROUPS + threadIdx.x / LPR;
+  if (row < rows) fetch(row);
+  for (; row < rows; row += step) {
+    const float2 st = st_next;
     float xh[VPL][V], d[VPL][V], r[VPL][V], s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      const int c = (l + LPR * i) * V;
-      if (l + LPR * i < nv) {
-        load_vec<T, V>(x + (long long)row * ldx + c, xh[i]);
-        load_vec<T, V>(dy + (long long)row * ldg + c, d[i]);
-        if (dres) load_vec<T, V>(dres + (long long)row * ldr + c, r[i]);
-      } else {
+      Raw<T, V>::unpack(rx[i], xh[i]);
+      Raw<T, V>::unpack(rd[i], d[i]);
+      if (dres) Raw<T, V>::unpack(rr[i], r[i]);
+      if (l + LPR * i >= nv) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) xh[i][e] = d[i][e] = 0.f;
+        for (int e = 0; e < V; ++e) d[i][e] = 0.f;
       }
     }
+    if (row + step < rows) fetch(row + step);
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
 #pragma unroll
