@@ -14,7 +14,6 @@
 #include <math.h>
 
 #include <type_traits>
-#include <stdlib.h>
 
 #include "common.h"
 
@@ -161,37 +160,32 @@ __device__ __forceinline__ void tile_ready() {
 }
 
 // ---------------------------------------------------------------------------------------------------------------- forward
-// 128 QB queries a workgroup, 32 QB a wave; keys in tiles of 64, double buffered.  With few workgroups the keys are split over several
+// 128 queries a workgroup, 32 a wave; keys in tiles of 64, double buffered.  With few workgroups the keys are split over several
 // (host rule): each leaves its normalised sum and lse, attn_fwd_join_kernel weighs them.
 // The exponent's reference m need not be the running maximum, only near it: a tile is first taken with the m there is, and only if a lane's sum
 // of 32 comes out above 2^13 (p must stay in f16) it is taken again for the new maximum.  That saves the maximum and the rescaling of the output
 // sums, 54 of 170 vector instructions, in all but the first, the masked and such rare tiles.
-template <typename T, int QB>
+template <typename T>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Args a) {
-  constexpr int ROWS = 128 * QB;
   __shared__ __attribute__((aligned(16))) char lds[4 * TILE_BYTES];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
-  const int nqb = (a.Lq + ROWS - 1) / ROWS, ws = xcd_range(blockIdx.x, gridDim.x), split = ws % a.splits, w = ws / a.splits;
+  const int nqb = (a.Lq + 127) >> 7, ws = xcd_range(blockIdx.x, gridDim.x), split = ws % a.splits, w = ws / a.splits;
   const int bh = w / nqb, b = bh / a.H, h = bh % a.H, hk = h / (a.H / a.Hkv);
   const int qb = a.causal ? nqb - 1 - w % nqb : w % nqb;   // (long rows first)
   const int nk = clamp_len(a.kv_len, b, a.Lk), nq = clamp_len(a.q_len, b, a.Lq), off = a.Lk - a.Lq;
-  const int w0 = qb * ROWS + wave * 32 * QB, row0 = w0 + (lane & 31);
-  int kend = qb * ROWS < nq ? nk : 0;
-  if (a.causal) kend = min(kend, min(qb * ROWS + ROWS, nq) + off);
-  const int full = a.causal ? min(nk, w0 + off + 1) : nk;                   // keys that every row of this wave sees
-  const int wend = a.causal ? min(nk, w0 + 32 * QB + off) : nk;             // keys that some row of this wave sees
+  const int w0 = qb * 128 + wave * 32, row = w0 + (lane & 31);
+  const bool q_ok = row < nq;
+  int kend = qb * 128 < nq ? nk : 0;
+  if (a.causal) kend = min(kend, min(qb * 128 + 128, nq) + off);
+  const int full = a.causal ? min(nk, w0 + off + 1) : nk;      // keys that every row of this wave sees
+  const int wend = a.causal ? min(nk, w0 + 32 + off) : nk;     // keys that some row of this wave sees
+  const int mine = a.causal ? min(nk, row + off + 1) : nk;     // keys that this lane's row sees
   const u16* kp = a.k + b * a.ks[0] + hk * a.ks[2];
   const u16* vp = a.v + b * a.vs[0] + hk * a.vs[2];
-  typename T::vec8 qf[QB][4];
-  f32x16 acc[QB][2];
-  float m[QB], l[QB];   // the exponent's reference (times c) and this lane's part of the sum
-#pragma unroll
-  for (int i = 0; i < QB; ++i) {
-    const int row = row0 + 32 * i;
-    load_rows<T>(qf[i], a.q + b * a.qs[0] + (long long)(row < nq ? row : 0) * a.qs[1] + h * a.qs[2], row < nq, hi);
-    acc[i][0] = acc[i][1] = splat(0.f);
-    m[i] = l[i] = 0.f;
-  }
+  typename T::vec8 qf[4];
+  load_rows<T>(qf, a.q + b * a.qs[0] + (long long)(q_ok ? row : 0) * a.qs[1] + h * a.qs[2], q_ok, hi);
+  f32x16 acc[2] = {splat(0.f), splat(0.f)};
+  float m = 0.f, l = 0.f;   // the exponent's reference (times c) and this lane's part of the sum
   const float c = a.scale * LOG2E;
   int t0, t1;
   split_range(kend > 0 ? (kend + TILE - 1) / TILE : 0, split, a.splits, t0, t1);
@@ -204,15 +198,11 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Args a) {
     tile_ready();
     if (t + 1 < t1) stage(t + 1);
   };
-  auto score = [&](const char* kt, int kb, f32x16* s) {
+  auto score = [&](const char* kt, int kb) {
+    f32x16 s = splat(0.f);
 #pragma unroll
-    for (int i = 0; i < QB; ++i) s[i] = splat(0.f);
-#pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      const typename T::vec8 kf = rows_frag<T>(kt, kb * 32, ks, lane);
-#pragma unroll
-      for (int i = 0; i < QB; ++i) s[i] = T::mfma32(kf, qf[i][ks], s[i]);
-    }
+    for (int ks = 0; ks < 4; ++ks) s = T::mfma32(rows_frag<T>(kt, kb * 32, ks, lane), qf[ks], s);
+    return s;
   };
   auto prob = [&](f32x16& s, float ref) {   // s -> p, their sum over this lane's 16 keys
     float sum = 0.f;
@@ -236,85 +226,62 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Args a) {
       const int key0 = t * TILE + kb * 32;
       if (key0 >= wend) break;
       const bool first = t == t0 && kb == 0;
-      f32x16 s[QB];
-      score(kt, kb, s);
+      f32x16 s = score(kt, kb);
+      float mx = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < QB; ++i) {
-        const int end = (a.causal ? min(nk, row0 + 32 * i + off + 1) : nk) - key0;
-        float mx = -INFINITY;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          if (row_of(r, hi) >= end) s[i][r] = -INFINITY;
-          mx = fmaxf(mx, s[i][r]);
-        }
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
-        const float to = first ? (mx == -INFINITY ? 0.f : mx) : fmaxf(m[i], mx);   // (a row sees the first keys or none)
-        const float al = first ? 0.f : __builtin_amdgcn_exp2f(m[i] - to);
-        m[i] = to;
-        l[i] = l[i] * al + prob(s[i], to);
-#pragma unroll
-        for (int d = 0; d < 2; ++d)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) acc[i][d][r] *= al;
+      for (int r = 0; r < 16; ++r) {
+        if (row_of(r, hi) >= mine - key0) s[r] = -INFINITY;
+        mx = fmaxf(mx, s[r]);
       }
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * c;
+      const float to = first ? (mx == -INFINITY ? 0.f : mx) : fmaxf(m, mx);   // (a row sees the first keys or none)
+      const float al = first ? 0.f : __builtin_amdgcn_exp2f(m - to);
+      m = to;
+      l = l * al + prob(s, to);
 #pragma unroll
-      for (int hf = 0; hf < 2; ++hf)
+      for (int d = 0; d < 2; ++d)
 #pragma unroll
-        for (int d = 0; d < 2; ++d) {
-          const typename T::vec8 vf = cols_frag<T>(vt, kb * 32 + hf * 16, d * 32, lane);
+        for (int r = 0; r < 16; ++r) acc[d][r] *= al;
 #pragma unroll
-          for (int i = 0; i < QB; ++i) acc[i][d] = T::mfma32(vf, pack_frag<T>(s[i], hf), acc[i][d]);
-        }
+      for (int hf = 0; hf < 2; ++hf) {
+        const typename T::vec8 pf = pack_frag<T>(s, hf);
+#pragma unroll
+        for (int d = 0; d < 2; ++d) acc[d] = T::mfma32(cols_frag<T>(vt, kb * 32 + hf * 16, d * 32, lane), pf, acc[d]);
+      }
     }
     for (; t + 1 < hot; ++t) {   // the reference stays
       enter(t + 1);
-      const char *kt = lds + ((t + 1) & 1) * 2 * TILE_BYTES, *vt = kt + TILE_BYTES;
-      typename T::vec8 pf[2][2][QB];
-      float sum[QB], top = 0.f;
+      const char *kn = lds + ((t + 1) & 1) * 2 * TILE_BYTES, *vn = kn + TILE_BYTES;
+      typename T::vec8 pf[2][2];
+      float sum = 0.f;
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
-        f32x16 s[QB];
-        score(kt, kb, s);
-#pragma unroll
-        for (int i = 0; i < QB; ++i) {
-          const float x = prob(s[i], m[i]);
-          sum[i] = kb ? sum[i] + x : x;
-          pf[kb][0][i] = pack_frag<T>(s[i], 0);
-          pf[kb][1][i] = pack_frag<T>(s[i], 1);
-        }
+        f32x16 s = score(kn, kb);
+        sum += prob(s, m);
+        pf[kb][0] = pack_frag<T>(s, 0);
+        pf[kb][1] = pack_frag<T>(s, 1);
       }
-#pragma unroll
-      for (int i = 0; i < QB; ++i) top = sum[i] <= 8192.f ? top : INFINITY;
-      if (!__all(top == 0.f)) {   // the scores have grown beyond it: this tile once more, with the maximum
+      if (!__all(sum <= 8192.f)) {   // the scores have grown beyond it: this tile once more, with the maximum
         entered = true;
         break;
       }
-#pragma unroll
-      for (int i = 0; i < QB; ++i) l[i] += sum[i];
+      l += sum;
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-          for (int d = 0; d < 2; ++d) {
-            const typename T::vec8 vf = cols_frag<T>(vt, kb * 32 + hf * 16, d * 32, lane);
-#pragma unroll
-            for (int i = 0; i < QB; ++i) acc[i][d] = T::mfma32(vf, pf[kb][hf][i], acc[i][d]);
-          }
+          for (int d = 0; d < 2; ++d) acc[d] = T::mfma32(cols_frag<T>(vn, kb * 32 + hf * 16, d * 32, lane), pf[kb][hf], acc[d]);
     }
   }
-#pragma unroll
-  for (int i = 0; i < QB; ++i) {
-    const int row = row0 + 32 * i;
-    const float sum = l[i] + __shfl_xor(l[i], 32, 64);
-    if (row < a.Lq) {
-      const bool some = row < nq && sum != 0.f;   // (a NaN stays one)
-      const float inv = some ? 1.f / sum : 0.f, lse = some ? (m[i] + __builtin_amdgcn_logf(sum)) * LN2 : -INFINITY;
-      const long long at = (long long)bh * a.Lq + row, pat = (long long)split * a.B * a.H * a.Lq + at;
-      if (a.splits == 1) store_cols<T>(a.o + b * a.os[0] + (long long)row * a.os[1] + h * a.os[2], acc[i], inv, hi);
-      else store_cols_f32(a.part + pat * HD, acc[i], inv, hi);
-      if (hi == 0) (a.splits == 1 ? a.lse + at : a.part_row + pat)[0] = lse;
-    }
+  l += __shfl_xor(l, 32, 64);
+  if (row < a.Lq) {
+    const bool some = q_ok && l != 0.f;   // (a NaN stays one)
+    const float inv = some ? 1.f / l : 0.f, lse = some ? (m + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
+    const long long at = (long long)bh * a.Lq + row, pat = (long long)split * a.B * a.H * a.Lq + at;
+    if (a.splits == 1) store_cols<T>(a.o + b * a.os[0] + (long long)row * a.os[1] + h * a.os[2], acc, inv, hi);
+    else store_cols_f32(a.part + pat * HD, acc, inv, hi);
+    if (hi == 0) (a.splits == 1 ? a.lse + at : a.part_row + pat)[0] = lse;
   }
 }
 
@@ -786,7 +753,6 @@ int splits_of(long long groups, long long tiles) {
 }
 struct Plan {
   int fwd, q, kv;             // splits
-  int fwd_qb;                 // 32 queries a wave, or 64
   bool small;                 // backward in one launch
   long long lqp, rows_floats; // padded queries; nl2 | nd | gmax | vmax
   long long part_floats;      // the largest of the splits' sums, dq's first
@@ -794,7 +760,6 @@ struct Plan {
 Plan plan_of(int dtype, int B, int H, int Hkv, int Lq, int Lk) {
   Plan p;
   const long long bh = (long long)B * H, bk = (long long)B * Hkv;
-  p.fwd_qb = getenv("XQB") ? atoi(getenv("XQB")) : bh * cdiv(Lq, 256) >= 256 ? 2 : 1;
   p.small = Lq <= 128 && Lk <= 128 && H / Hkv <= 4;
   p.fwd = p.q = splits_of(bh * cdiv(Lq, 128), cdiv(Lk, TILE));
   p.kv = splits_of(bk * cdiv(Lk, 128), (long long)cdiv(Lq, TILE) * (H / Hkv));
@@ -824,9 +789,7 @@ extern "C" int dbir_attention_bwd_ws(int dtype, int B, int H, int Hkv, int Lq, i
 namespace {
 template <typename T>
 void launch_fwd(const Args& a, const Plan& p, hipStream_t s) {
-  const dim3 grid((unsigned)(cdiv(a.Lq, 128 * p.fwd_qb) * a.B * a.H * p.fwd));
-  if (p.fwd_qb == 2) hipLaunchKernelGGL((attn_fwd_kernel<T, 2>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((attn_fwd_kernel<T, 1>), grid, dim3(256), 0, s, a);
+  hipLaunchKernelGGL(attn_fwd_kernel<T>, dim3((unsigned)(cdiv(a.Lq, 128) * a.B * a.H * p.fwd)), dim3(256), 0, s, a);
   if (p.fwd > 1) hipLaunchKernelGGL(attn_fwd_join_kernel<T>, dim3((unsigned)cdiv((long long)a.B * a.H * a.Lq, 4)), dim3(256), 0, s, a);
 }
 }  // namespace

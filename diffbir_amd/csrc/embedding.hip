@@ -40,21 +40,20 @@ constexpr int RANK_MAX = 16384;  // up to here the sort is one launch that count
 __device__ __forceinline__ uint32_t clamp_token(long long t, int vocab) { return (uint32_t)(t < 0 ? 0 : (t >= vocab ? vocab - 1 : t)); }
 
 // ------------------------------------------------------------------------------------------------------------- forward
-// lpr lanes (a power of two) a row, V elements a lane and step; a lane group takes FWD_ROWS rows at once: their loads are in flight together, and
+// lpr lanes (a power of two) a row, V elements a lane and step; a lane group takes R rows at once: their loads are in flight together, and
 // with positions they are rows of one position (rows `gap` = L apart), which is read once for all of them.
-constexpr int FWD_ROWS = 4;
-template <typename TT, typename TO, int V>
+template <typename TT, typename TO, int V, int R>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const typename TT::elem* __restrict__ table, long long ldt, const long long* __restrict__ tokens,
                                                         const float* __restrict__ pos, long long ldp, typename TO::elem* __restrict__ out, long long ldo,
                                                         float scale, int n, int gap, int W, int vocab, int lpr_log) {
   const long long id = (long long)blockIdx.x * 256 + threadIdx.x, set = id >> lpr_log;
-  const long long row0 = set / gap * gap * FWD_ROWS + set % gap;
+  const long long row0 = set / gap * gap * R + set % gap;
   if (row0 >= n) return;
   const int lpr = 1 << lpr_log;
-  const typename TT::elem* t[FWD_ROWS];
+  const typename TT::elem* t[R];
   bool same = true;   // one token in all of them (padding)
 #pragma unroll
-  for (int r = 0; r < FWD_ROWS; ++r) {   // (rows that do not exist read the first one's token and store nothing)
+  for (int r = 0; r < R; ++r) {   // (rows that do not exist read the first one's token and store nothing)
     const long long row = row0 + (long long)r * gap;
     t[r] = table + (long long)clamp_token(tokens[row < n ? row : row0], vocab) * ldt;
     same &= t[r] == t[0];
@@ -62,17 +61,17 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const typename TT::elem*
   const float* p = pos ? pos + (row0 % gap) * ldp : nullptr;
 #pragma unroll 2
   for (int c = ((int)id & (lpr - 1)) * V; c < W; c += lpr * V) {
-    float f[FWD_ROWS][V], q[V];
+    float f[R][V], q[V];
     if constexpr (V == 4) TT::load4(t[0] + c, f[0]);
     else f[0][0] = TT::load(t[0] + c);
     if (same) {
 #pragma unroll
-      for (int r = 1; r < FWD_ROWS; ++r)
+      for (int r = 1; r < R; ++r)
 #pragma unroll
         for (int e = 0; e < V; ++e) f[r][e] = f[0][e];
     } else {
 #pragma unroll
-      for (int r = 1; r < FWD_ROWS; ++r) {
+      for (int r = 1; r < R; ++r) {
         if constexpr (V == 4) TT::load4(t[r] + c, f[r]);
         else f[r][0] = TT::load(t[r] + c);
       }
@@ -84,7 +83,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const typename TT::elem*
       else q[0] = p[c];
     }
 #pragma unroll
-    for (int r = 0; r < FWD_ROWS; ++r) {
+    for (int r = 0; r < R; ++r) {
       const long long row = row0 + (long long)r * gap;
 #pragma unroll
       for (int e = 0; e < V; ++e) f[r][e] = __builtin_fmaf(f[r][e], scale, q[e]);
@@ -292,12 +291,24 @@ __device__ __forceinline__ void add_run(const typename T::elem* dy, long long ld
     add_items<T, V>(dy, ldg, spos, s, e, c0, lane, W, acc);
   }
 }
-__device__ __forceinline__ int first_at_least(const uint32_t* skey, int n, uint32_t v) {   // the first sorted position whose token is at least v
-  int lo = 0, hi = n;
+// the first sorted position in [lo, hi) whose token is at least v (hi if none): by one lane, halving, or by a wave, in 64ths
+__device__ __forceinline__ int first_at_least(const uint32_t* skey, int lo, int hi, uint32_t v) {
   while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
+    const int mid = lo + ((hi - lo) >> 1);
     if (skey[mid] < v) lo = mid + 1;
     else hi = mid;
+  }
+  return lo;
+}
+__device__ __forceinline__ int first_at_least_wave(const uint32_t* skey, int hi, uint32_t v, int lane) {
+  int lo = 0;
+  while (lo < hi) {
+    const int step = (hi - lo + 63) / 64;
+    const long long at = lo + (long long)lane * step;
+    const int less = __popcll(__ballot(at < hi && skey[at < hi ? at : lo] < v));   // of 64 samples, the first `less` are below
+    if (less == 0) return lo;
+    hi = min((long long)hi, lo + (long long)less * step);
+    lo += (less - 1) * step + 1;
   }
   return lo;
 }
@@ -318,7 +329,7 @@ __device__ __forceinline__ void join_waves(float* acc, float (*join)[256], int l
   }
 }
 
-// NW = 4: one row of the table a workgroup, its positions split over the waves (small tables); NW = 16: 128 rows, 8 a wave, most of them empty,
+// NW = 4: one row of the table a workgroup, its positions split over the waves (small tables); NW = 8: 64 rows, 8 a wave, most of them empty,
 // and runs of more than RUN positions split over the waves.  One block of 256 columns either way.  The first pos_rows * (blocks of columns)
 // workgroups make dpos[l], the waves a part of the batch each.  Blocks of columns are adjacent workgroups, so that a long run's all start early.
 template <typename T, int V, int NW>
@@ -346,8 +357,16 @@ __global__ __launch_bounds__(NW * 64) void embed_rows_kernel(const typename T::e
     return;
   }
   const int v0 = (blk - pos_rows) * ROWS;
-  if ((int)threadIdx.x <= ROWS) first[threadIdx.x] = first_at_least(skey, n, (uint32_t)(v0 + threadIdx.x));
+  if (wave < 2) {   // this workgroup's positions, and within them each row's
+    const int at = first_at_least_wave(skey, n, (uint32_t)(v0 + wave * ROWS), lane);
+    if (lane == 0) first[wave * ROWS] = at;
+  }
   __syncthreads();
+  if (ROWS > 1) {
+    const int lo = first[0], hi = first[ROWS], r = (int)threadIdx.x;
+    if (r > 0 && r < ROWS) first[r] = lo == hi ? lo : first_at_least(skey, lo, hi, (uint32_t)(v0 + r));
+    __syncthreads();
+  }
   auto write = [&](int v, const float* acc) {
     float* d = dtable + (long long)v * ldd;
     if constexpr (V == 4) {
@@ -429,12 +448,18 @@ extern "C" int dbir_embedding_fwd(int table_dtype, const void* table, long long 
   int lg = 0;
   while (lg < 6 && (1 << lg) < nv) ++lg;
   const int gap = pos ? L : 1;
-  const long long sets = (long long)cdiv(n, (long long)gap * FWD_ROWS) * gap;
+  const int R = ((long long)n << lg) >= 64 * 8192 ? 4 : 1;   // one row a group while that gives fewer than eight waves a SIMD
+  const long long sets = (long long)cdiv(n, (long long)gap * R) * gap;
   DBIR_CHECK_ARG((sets << lg) <= 0xffffff00LL, "dbir_embedding_fwd: too many tokens for one launch");
   const dim3 grid((unsigned)(((sets << lg) + 255) / 256));
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-#define GO2(TT, TO, V)                                                                                                                        \
-  hipLaunchKernelGGL((embed_fwd_kernel<TT, TO, V>), grid, dim3(256), 0, s, (const TT::elem*)table, ldt, tokens, pos, ldp, (TO::elem*)out, ldo, \
+#define GO2(TT, TO, V)             \
+  do {                             \
+    if (R == 4) GO3(TT, TO, V, 4); \
+    else GO3(TT, TO, V, 1);        \
+  } while (0)
+#define GO3(TT, TO, V, R)                                                                                                                        \
+  hipLaunchKernelGGL((embed_fwd_kernel<TT, TO, V, R>), grid, dim3(256), 0, s, (const TT::elem*)table, ldt, tokens, pos, ldp, (TO::elem*)out, ldo, \
                      scale, n, gap, W, vocab, lg)
 #define GO(TT, TO)          \
   do {                      \
@@ -454,6 +479,7 @@ extern "C" int dbir_embedding_fwd(int table_dtype, const void* table, long long 
   }
 #undef GO
 #undef GO2
+#undef GO3
   DBIR_CHECK_LAUNCH("dbir_embedding_fwd");
   return DBIR_OK;
 }
@@ -496,9 +522,9 @@ extern "C" int dbir_embedding_bwd(int dtype, const void* dy, long long ldg, cons
     }
   }
   const bool v4 = W % 4 == 0 && al(dy, ldg, elem4(dtype)) && al(dtable, ldd, 16);
-  const bool small = vocab <= 8 * 1024;   // 128 rows a workgroup would not fill the chip
-  const long long groups = (small ? vocab : cdiv(vocab, 128)) + (long long)pos_rows;
-  DBIR_CHECK_ARG(groups * cdiv(W, 256) < (1 << 22), "dbir_embedding_bwd: table too large for one launch");
+  const bool small = vocab <= 8 * 1024;   // 64 rows a workgroup would not fill the chip
+  const long long groups = (small ? vocab : cdiv(vocab, 64)) + (long long)pos_rows;
+  DBIR_CHECK_ARG(groups * cdiv(W, 256) < (1 << 23), "dbir_embedding_bwd: table too large for one launch");
   const dim3 gp((unsigned)p.pieces, (unsigned)cdiv(W, 1024)), gr((unsigned)(groups * cdiv(W, 256)));
 #define ROWS(T, V, S)                                                                                                                         \
   hipLaunchKernelGGL((embed_rows_kernel<T, V, S>), gr, dim3(S * 64), 0, s, (const T::elem*)dy, ldg, key[at], pos[at], part, dtable, ldd, dpos, \
@@ -507,7 +533,7 @@ extern "C" int dbir_embedding_bwd(int dtype, const void* dy, long long ldg, cons
   do {                                                                                                                                           \
     if (p.pieces) hipLaunchKernelGGL((embed_piece_kernel<T, V>), gp, dim3(256), 0, s, (const T::elem*)dy, ldg, key[at], pos[at], part, W, p.Wp);  \
     if (small) ROWS(T, V, 4);                                                                                                                    \
-    else ROWS(T, V, 16);                                                                                                                         \
+    else ROWS(T, V, 8);                                                                                                                          \
   } while (0)
 #define GO(T)          \
   do {                 \
