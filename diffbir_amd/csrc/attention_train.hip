@@ -651,7 +651,7 @@ __device__ __forceinline__ void q_part(const Args& a, char* lds, int b, int h, i
   }
 }
 template <typename T>
-__global__ __launch_bounds__(256, 2) void attn_bwd_q_kernel(const Args a) {
+__global__ __launch_bounds__(256, 3) void attn_bwd_q_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char lds[4 * TILE_BYTES];
   __shared__ float red[4];
   const int nqb = (a.Lq + 127) >> 7, ws = xcd_range(blockIdx.x, gridDim.x), w = ws / a.splits, bh = w / nqb, b = bh / a.H, h = bh % a.H;

@@ -43,7 +43,7 @@ __device__ __forceinline__ float block_sum(float v, float* red) {   // 256 threa
 }
 
 // Rows held in registers: LPR lanes a row, VPL vectors of V elements a lane (V = 16 bytes' worth, or 1 where the rows are not aligned for
-// that), vector v = lane + LPR i.  A group goes through rows `step` apart with gamma (beta) and the column sums in its registers.
+// that), vector v = lane + LPR i.  A group goes through rows `step` apart, backwards with gamma and the column sums in its registers.
 // Every byte is read once: the bound is memory (figures at the host rule below).
 template <typename T, int V>
 __device__ __forceinline__ void load_vec(const typename T::elem* p, float* f) {
@@ -111,12 +111,6 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const typename T::elem* __r
   __shared__ float red[2][8];
   const int l = threadIdx.x % LPR, nv = C / V, step = gridDim.x * GROUPS;
   int turn = 0;
-  float g[VPL][V], b[VPL][V];
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    load_f32<V>(gamma, (l + LPR * i) * V, l + LPR * i < nv, g[i]);
-    load_f32<V>(beta, (l + LPR * i) * V, l + LPR * i < nv, b[i]);
-  }
   for (int row = blockIdx.x * GROUPS + threadIdx.x / LPR; row < rows; row += step) {   // (LPR = 256: the same for the whole workgroup)
     const typename T::elem* xr = x + (long long)row * ldx;
     float f[VPL][V], s = 0.f, q = 0.f;
@@ -147,8 +141,11 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const typename T::elem* __r
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
       if (l + LPR * i < nv) {
+        float g[V], b[V];   // (from the cache: held in registers they cost more waves than they save)
+        load_f32<V>(gamma, (l + LPR * i) * V, true, g);
+        load_f32<V>(beta, (l + LPR * i) * V, true, b);
 #pragma unroll
-        for (int e = 0; e < V; ++e) f[i][e] = __builtin_fmaf(f[i][e] * rstd, g[i][e], b[i][e]);
+        for (int e = 0; e < V; ++e) f[i][e] = __builtin_fmaf(f[i][e] * rstd, g[e], b[e]);
         store_vec<T, V>(y + (long long)row * ldy + (l + LPR * i) * V, f[i]);
       }
     if (l == 0) *reinterpret_cast<float2*>(stats + 2LL * row) = make_float2(mean, rstd);
@@ -356,8 +353,9 @@ int any_chunks(int rows, int C) {   // partial rows: about 2048 workgroups over 
 struct Shape {
   int v, lpr, vpl;   // v = 0: too wide for registers
 };
-Shape shape_of(int dtype, int C, bool wide) {
+Shape shape_of(int dtype, int C, bool wide, bool fwd) {
   const int v = wide ? (dtype == DBIR_F32 ? 4 : 8) : 1, nv = C / v;
+  if (wide && fwd && nv > 32 && nv <= 160) return nv <= 40 ? Shape{v, 8, 5} : nv <= 80 ? Shape{v, 16, 5} : Shape{v, 32, 5};   // (no column sums to hold)
   if (!wide) return nv <= 256 ? Shape{1, 64, 4} : nv <= 2048 ? Shape{1, 256, 8} : nv <= 4096 ? Shape{1, 256, 16} : Shape{0, 0, 0};
   return nv <= 8 ? Shape{v, 8, 1} : nv <= 32 ? Shape{v, 32, 1} : nv <= 64 ? Shape{v, 32, 2} : nv <= 128 ? Shape{v, 64, 2} : nv <= 192 ? Shape{v, 64, 3} :
          nv <= 320 ? Shape{v, 64, 5} : nv <= 512 ? Shape{v, 256, 2} : nv <= 1024 ? Shape{v, 256, 4} : Shape{0, 0, 0};
@@ -373,7 +371,7 @@ int bwd_groups(int rows, const Shape& sh) {
   return n < 512 ? n : 512;
 }
 int bwd_parts(int dtype, int rows, int C, bool wide) {
-  const Shape sh = shape_of(dtype, C, wide);
+  const Shape sh = shape_of(dtype, C, wide, false);
   return sh.v ? bwd_groups(rows, sh) : any_chunks(rows, C);
 }
 
@@ -406,7 +404,10 @@ void launch_fwd(const Shape& sh, const void* x, long long ldx, void* y, long lon
   const dim3 grid((unsigned)(n < 2048 ? n : 2048));
 #define GO(TT, V, LPR, VPL) \
   hipLaunchKernelGGL((ln_fwd_kernel<TT, V, LPR, VPL>), grid, dim3(256), 0, s, (const E*)x, ldx, (E*)y, ldy, gamma, beta, stats, rows, C, eps)
-  EACH_SHAPE(GO, T);
+  if (sh.v > 1 && sh.lpr == 8 && sh.vpl == 5) GO(T, T::wide, 8, 5);
+  else if (sh.v > 1 && sh.lpr == 16) GO(T, T::wide, 16, 5);
+  else if (sh.v > 1 && sh.lpr == 32 && sh.vpl == 5) GO(T, T::wide, 32, 5);
+  else EACH_SHAPE(GO, T);
 #undef GO
 }
 
@@ -450,7 +451,7 @@ extern "C" int dbir_layernorm_fwd(int dtype, const void* x, long long ldx, void*
   DBIR_CHECK_ARG(dtype >= DBIR_F16 && dtype <= DBIR_F32, "dbir_layernorm_fwd: bad dtype %d", dtype);
   DBIR_CHECK_ARG((reinterpret_cast<uintptr_t>(stats) & 7) == 0, "dbir_layernorm_fwd: stats must be 8-byte aligned");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const Shape sh = shape_of(dtype, C, is_wide(dtype, C, x, ldx) && is_wide(dtype, C, y, ldy) && aligned16(gamma) && aligned16(beta));
+  const Shape sh = shape_of(dtype, C, is_wide(dtype, C, x, ldx) && is_wide(dtype, C, y, ldy) && aligned16(gamma) && aligned16(beta), true);
   if (dtype == DBIR_F16) launch_fwd<F16T>(sh, x, ldx, y, ldy, gamma, beta, stats, rows, C, eps, s);
   else if (dtype == DBIR_BF16) launch_fwd<BF16T>(sh, x, ldx, y, ldy, gamma, beta, stats, rows, C, eps, s);
   else launch_fwd<F32T>(sh, x, ldx, y, ldy, gamma, beta, stats, rows, C, eps, s);
@@ -467,7 +468,7 @@ extern "C" int dbir_layernorm_bwd(int dtype, const void* dy, long long ldg, cons
   DBIR_CHECK_ARG(dtype >= DBIR_F16 && dtype <= DBIR_F32, "dbir_layernorm_bwd: bad dtype %d", dtype);
   DBIR_CHECK_ARG(((reinterpret_cast<uintptr_t>(stats) & 7) | (reinterpret_cast<uintptr_t>(ws) & 3)) == 0, "dbir_layernorm_bwd: stats must be 8-byte aligned");
   const bool wide = aligned16(gamma) && is_wide(dtype, C, dy, ldg) && is_wide(dtype, C, x, ldx) && is_wide(dtype, C, dx, ldd) && (!dres || is_wide(dtype, C, dres, ldr));
-  const Shape sh = shape_of(dtype, C, wide);
+  const Shape sh = shape_of(dtype, C, wide, false);
   const int n = bwd_parts(dtype, rows, C, wide);
   DBIR_CHECK_ARG(ws_bytes >= 8LL * C * n, "dbir_layernorm_bwd: the workspace must hold %lld bytes", 8LL * C * n);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
