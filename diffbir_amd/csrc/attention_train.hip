@@ -526,9 +526,10 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_kv_kernel(const Args a) {
 }
 
 // dq: 128 queries a workgroup, 32 a wave; keys in tiles of 64, double buffered.  D = do . o comes from the ROUNDED o, and where one key has
-// most of a row, dp - D is far below D.  The exact D makes sum_j ds_ij zero, so the sum of the ds that are formed with the rounded one is its error:
-// it corrects D for the dk kernel, and rows of up to two tiles (few keys: where it matters most) are gone through once more with the corrected one.
-template <typename T>
+// most of a row, dp - D is far below D.  The exact D makes sum_j ds_ij zero, so the sum of the ds that are formed with the rounded one is its error,
+// delta: it corrects D for the dk kernel.  For dq, EXACT (up to 512 keys, where the error shows) also sums p_ij k_j, a third more products, and
+// subtracts delta times that; else rows of up to two tiles are gone through once more with the corrected D.
+template <typename T, bool EXACT>
 __device__ __forceinline__ void q_part(const Args& a, char* lds, int b, int h, int qb, int split, float e) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
   const int bh = b * a.H + h, hk = h / (a.H / a.Hkv);
@@ -567,9 +568,9 @@ __device__ __forceinline__ void q_part(const Args& a, char* lds, int b, int h, i
     *to_nd = nd;
   }
   nl2 += e;
-  f32x16 acc[2] = {splat(0.f), splat(0.f)};
+  f32x16 acc[2] = {splat(0.f), splat(0.f)}, accp[2] = {splat(0.f), splat(0.f)};   // (accp: EXACT)
   const int nt = kend > 0 ? (kend + TILE - 1) / TILE : 0;
-  const bool few = nt <= 2;
+  const bool few = !EXACT && nt <= 2;
   int t0, t1;
   split_range(nt, split, a.splits, t0, t1);
   if (few) t0 = 0, t1 = split == 0 ? nt : 0;   // (the first split alone)
@@ -582,7 +583,7 @@ __device__ __forceinline__ void q_part(const Args& a, char* lds, int b, int h, i
   if (few && t1 == 2) stage(1);
   if (few && t1) tile_ready();
   float fix = 0.f;
-  auto ds_of = [&](auto masked, const char* kt, int key0, int kb) {   // 2^e ds of 32 keys (rows) and the wave's 32 queries
+  auto add_half = [&](auto masked, const char* kt, int key0, int kb, bool to_dq) {   // 32 keys (rows of s) and the wave's 32 queries
     f32x16 s = splat(0.f), dp = splat(nd);
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
@@ -590,22 +591,29 @@ __device__ __forceinline__ void q_part(const Args& a, char* lds, int b, int h, i
       dp = T::mfma32(rows_frag<T>(kt + TILE_BYTES, kb * 32, ks, lane), gf[ks], dp);
     }
 #pragma unroll
-    for (int r = 0; r < 16; ++r) dp[r] *= __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, nl2));
+    for (int r = 0; r < 16; ++r) {
+      s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], c, nl2));   // 2^e p
+      dp[r] *= s[r];                                                 // 2^e ds
+    }
     if constexpr (masked) {
 #pragma unroll
       for (int r = 0; r < 16; ++r)
-        if (key0 + kb * 32 + row_of(r, hi) >= mine) dp[r] = 0.f;
+        if (key0 + kb * 32 + row_of(r, hi) >= mine) s[r] = dp[r] = 0.f;
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r) sum += dp[r];
-    return dp;
-  };
-  auto add_half = [&](const f32x16& ds, const char* kt, int kb) {
+    if (!to_dq) return;
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
-      const typename T::vec8 df = pack_frag<T>(ds, hf);
+      const typename T::vec8 df = pack_frag<T>(dp, hf);
+      typename T::vec8 pf;
+      if constexpr (EXACT) pf = pack_frag<T>(s, hf);
 #pragma unroll
-      for (int d = 0; d < 2; ++d) acc[d] = T::mfma32(cols_frag<T>(kt, kb * 32 + hf * 16, d * 32, lane), df, acc[d]);
+      for (int d = 0; d < 2; ++d) {
+        const typename T::vec8 kc = cols_frag<T>(kt, kb * 32 + hf * 16, d * 32, lane);
+        acc[d] = T::mfma32(kc, df, acc[d]);
+        if constexpr (EXACT) accp[d] = T::mfma32(kc, pf, accp[d]);
+      }
     }
   };
   int t = few ? -t1 : t0;
@@ -615,7 +623,7 @@ __device__ __forceinline__ void q_part(const Args& a, char* lds, int b, int h, i
     if (t + 1 < t1) stage(t + 1);
     const char* kt = lds + (t & 1) * 2 * TILE_BYTES;
 #pragma unroll 1
-    for (int kb = 0; kb < 2; ++kb) add_half(ds_of(std::false_type(), kt, 0, kb), kt, kb);
+    for (int kb = 0; kb < 2; ++kb) add_half(std::false_type(), kt, 0, kb, true);
   }
 #pragma unroll 1
   for (; t < t1; ++t) {   // few: the tiles once for the sum (t < 0), once more for dq
@@ -632,12 +640,17 @@ __device__ __forceinline__ void q_part(const Args& a, char* lds, int b, int h, i
 #pragma unroll 1
     for (int kb = 0; kb < 2; ++kb) {
       if (key0 + kb * 32 >= wend) break;
-      const f32x16 ds = ds_of(std::true_type(), kt, key0, kb);
-      if (t >= 0) add_half(ds, kt, kb);
+      add_half(std::true_type(), kt, key0, kb, t >= 0);
     }
   }
   sum = q_ok ? (few ? fix : (sum + __shfl_xor(sum, 32, 64)) * un) : 0.f;
   if (!few) nd -= sum;
+  if constexpr (EXACT) {
+#pragma unroll
+    for (int d = 0; d < 2; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[d][r] = __builtin_fmaf(-sum, accp[d][r], acc[d][r]);
+  }
   if (row < a.Lq) {
     if (!q_ok) acc[0] = acc[1] = splat(0.f);
     const long long at = (long long)bh * a.Lq + row, pat = (long long)split * a.B * a.H * a.Lq + at;
@@ -650,12 +663,12 @@ __device__ __forceinline__ void q_part(const Args& a, char* lds, int b, int h, i
     }
   }
 }
-template <typename T>
-__global__ __launch_bounds__(256, 3) void attn_bwd_q_kernel(const Args a) {
+template <typename T, bool EXACT>
+__global__ __launch_bounds__(256, EXACT ? 2 : 3) void attn_bwd_q_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char lds[4 * TILE_BYTES];
   __shared__ float red[4];
   const int nqb = (a.Lq + 127) >> 7, ws = xcd_range(blockIdx.x, gridDim.x), w = ws / a.splits, bh = w / nqb, b = bh / a.H, h = bh % a.H;
-  q_part<T>(a, lds, b, h, a.causal ? nqb - 1 - w % nqb : w % nqb, ws % a.splits, scale_exp<T>(a, b, h / (a.H / a.Hkv), threadIdx.x, red));
+  q_part<T, EXACT>(a, lds, b, h, a.causal ? nqb - 1 - w % nqb : w % nqb, ws % a.splits, scale_exp<T>(a, b, h / (a.H / a.Hkv), threadIdx.x, red));
 }
 
 // Up to 128 queries and keys: all of a key head in one workgroup and one launch.
@@ -673,7 +686,7 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_small_kernel(const Args a) {
     e = exponent_for(sqrtf(x) * sqrtf(block_max(norm2_part<T>(a.v + b * a.vs[0] + hk * a.vs[2], a.vs[1], 0, clamp_len(a.kv_len, b, a.Lk), tid), red, tid)));
   }
   for (int h = hk * grp; h < hk * grp + grp; ++h) {
-    q_part<T>(a, lds, b, h, 0, 0, e);
+    q_part<T, true>(a, lds, b, h, 0, 0, e);
     __threadfence_block();   // its nl2 and nd, for the next part; the tiles in LDS are done with
     __syncthreads();
   }
@@ -753,7 +766,7 @@ int splits_of(long long groups, long long tiles) {
 }
 struct Plan {
   int fwd, q, kv;             // splits
-  bool small;                 // backward in one launch
+  bool small, exact;          // backward in one launch; dq with the exact D
   long long lqp, rows_floats; // padded queries; nl2 | nd | gmax | vmax
   long long part_floats;      // the largest of the splits' sums, dq's first
 };
@@ -761,7 +774,9 @@ Plan plan_of(int dtype, int B, int H, int Hkv, int Lq, int Lk) {
   Plan p;
   const long long bh = (long long)B * H, bk = (long long)B * Hkv;
   p.small = Lq <= 128 && Lk <= 128 && H / Hkv <= 4;
-  p.fwd = p.q = splits_of(bh * cdiv(Lq, 128), cdiv(Lk, TILE));
+  p.exact = Lk <= 512;
+  p.fwd = splits_of(bh * cdiv(Lq, 128), cdiv(Lk, TILE));
+  p.q = p.exact ? 1 : p.fwd;   // (the correction needs all keys of a row)
   p.kv = splits_of(bk * cdiv(Lk, 128), (long long)cdiv(Lq, TILE) * (H / Hkv));
   p.lqp = ((long long)Lq + 63) / 64 * 64;
   p.rows_floats = (bh * p.lqp * 2 + (dtype == DBIR_F16 ? bh * (p.lqp / 64) + bk * ((Lk + 63) / 64) : 0) + 3) / 4 * 4;
@@ -829,7 +844,9 @@ void launch_bwd(Args a, const Plan& p, int f16, hipStream_t s) {
   }
   a.splits = p.q;
   a.part_row = a.part + p.q * nq * HD;
-  hipLaunchKernelGGL(attn_bwd_q_kernel<T>, dim3((unsigned)(cdiv(a.Lq, 128) * bh * p.q)), dim3(256), 0, s, a);
+  const dim3 gq((unsigned)(cdiv(a.Lq, 128) * bh * p.q));
+  if (p.exact) hipLaunchKernelGGL((attn_bwd_q_kernel<T, true>), gq, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((attn_bwd_q_kernel<T, false>), gq, dim3(256), 0, s, a);
   if (p.q > 1) hipLaunchKernelGGL((attn_bwd_join_kernel<T, 64>), dim3((unsigned)cdiv(nq, 16)), dim3(256), 0, s, a);
   a.splits = p.kv;
   const dim3 gk((unsigned)(cdiv(a.Lk, 128) * bk * p.kv));
