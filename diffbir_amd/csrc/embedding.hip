@@ -260,16 +260,25 @@ __device__ __forceinline__ void add_items(const typename T::elem* dy, long long 
 #pragma unroll
       for (int u = 0; u < 8; ++u) add_row<T, V>(dy + (long long)__builtin_amdgcn_readlane(p, j + u) * ldg, c0, lane, W, acc);
     }
-    for (; j < m; ++j) add_row<T, V>(dy + (long long)__builtin_amdgcn_readlane(p, j) * ldg, c0, lane, W, acc);
+    if (j < m) {   // the last up to seven, in flight together too: the rest of the eight read the last one and add nothing
+#pragma unroll
+      for (int u = 0; u < 7; ++u) {
+        float f[4] = {0.f, 0.f, 0.f, 0.f};
+        add_row<T, V>(dy + (long long)__builtin_amdgcn_readlane(p, min(j + u, m - 1)) * ldg, c0, lane, W, f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[k] += j + u < m ? f[k] : 0.f;
+      }
+    }
   }
 }
 
 // the sum of sorted positions [piece * RUN, + RUN) where they are one run: a wave a block of 256 columns
 template <typename T, int V>
 __global__ __launch_bounds__(256) void embed_piece_kernel(const typename T::elem* __restrict__ dy, long long ldg, const uint32_t* __restrict__ skey,
-                                                          const int* __restrict__ spos, float* __restrict__ part, int W, int Wp) {
+                                                          const int* __restrict__ spos, float* __restrict__ part, int W, int Wp, int padding) {
   const int piece = blockIdx.x, lane = threadIdx.x & 63, c0 = (blockIdx.y * 4 + (threadIdx.x >> 6)) * 256;
-  if (c0 >= W || skey[(long long)piece * RUN] != skey[(long long)piece * RUN + RUN - 1]) return;
+  const uint32_t token = skey[(long long)piece * RUN];
+  if (c0 >= W || token != skey[(long long)piece * RUN + RUN - 1] || token == (uint32_t)padding) return;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
   add_items<T, V>(dy, ldg, spos, piece * RUN, piece * RUN + RUN, c0, lane, W, acc);
 #pragma unroll
@@ -401,7 +410,7 @@ __global__ __launch_bounds__(NW * 64) void embed_rows_kernel(const typename T::e
       __syncthreads();
     }
   }
-  for (int r = NW == 4 ? wave : wave * 8; r < (NW == 4 ? 1 : wave * 8 + 8); ++r) {
+  for (int r = wave; r < ROWS; r += NW) {   // (in turn: frequent tokens are neighbours)
     const int v = v0 + r, s = __builtin_amdgcn_readfirstlane(first[r]), e = __builtin_amdgcn_readfirstlane(first[r + 1]);
     const bool none = s == e || v == padding;
     if (v >= vocab || (none && accumulate) || (!none && e - s > LONG)) continue;
@@ -522,7 +531,8 @@ extern "C" int dbir_embedding_bwd(int dtype, const void* dy, long long ldg, cons
     }
   }
   const bool v4 = W % 4 == 0 && al(dy, ldg, elem4(dtype)) && al(dtable, ldd, 16);
-  const bool small = vocab <= 8 * 1024;   // 64 rows a workgroup would not fill the chip
+  // a row a workgroup where most rows have positions (4096 rows of 1024, 4096 positions: 35.5 against 52.9 us; 154 positions: 18.2 against 15.5)
+  const bool small = vocab <= 8 * 1024 && vocab <= n;
   const long long groups = (small ? vocab : cdiv(vocab, 64)) + (long long)pos_rows;
   DBIR_CHECK_ARG(groups * cdiv(W, 256) < (1 << 23), "dbir_embedding_bwd: table too large for one launch");
   const dim3 gp((unsigned)p.pieces, (unsigned)cdiv(W, 1024)), gr((unsigned)(groups * cdiv(W, 256)));
@@ -531,7 +541,7 @@ extern "C" int dbir_embedding_bwd(int dtype, const void* dy, long long ldg, cons
                      scale, n, L, W, p.Wp, vocab, pos_rows, padding_idx, accumulate)
 #define GO2(T, V)                                                                                                                                \
   do {                                                                                                                                           \
-    if (p.pieces) hipLaunchKernelGGL((embed_piece_kernel<T, V>), gp, dim3(256), 0, s, (const T::elem*)dy, ldg, key[at], pos[at], part, W, p.Wp);  \
+    if (p.pieces) hipLaunchKernelGGL((embed_piece_kernel<T, V>), gp, dim3(256), 0, s, (const T::elem*)dy, ldg, key[at], pos[at], part, W, p.Wp, padding_idx); \
     if (small) ROWS(T, V, 4);                                                                                                                    \
     else ROWS(T, V, 8);                                                                                                                          \
   } while (0)

@@ -448,6 +448,7 @@ extern "C" int dbir_layernorm_fwd(int dtype, const void* x, long long ldx, void*
   DBIR_CHECK_ARG(x && y && gamma && beta && stats, "dbir_layernorm_fwd: null pointer");
   DBIR_CHECK_ARG(rows > 0 && rows <= (1 << 30) && C > 0 && ldx >= C && ldy >= C, "dbir_layernorm_fwd: bad rows / C / ld");
   DBIR_CHECK_ARG(x != y, "dbir_layernorm_fwd: y must not be x");
+  DBIR_CHECK_ARG(eps >= 0.f, "dbir_layernorm_fwd: eps must not be negative");
   DBIR_CHECK_ARG(dtype >= DBIR_F16 && dtype <= DBIR_F32, "dbir_layernorm_fwd: bad dtype %d", dtype);
   DBIR_CHECK_ARG((reinterpret_cast<uintptr_t>(stats) & 7) == 0, "dbir_layernorm_fwd: stats must be 8-byte aligned");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);

@@ -749,7 +749,7 @@ def attention_fwd(q: T, k: T, v: T, scale: float, causal: bool = False, q_len: O
     that sees no key gives zeros and lse = -inf."""
     dev = _train_device("attention_fwd", q, k, v, out, q_len, kv_len)
     if out is None:
-        out = torch.empty_like(q)
+        out = _dense_like(q)
     qs, ks, dt = q.shape, k.shape, q.dtype
     if len(qs) != 4 or len(ks) != 4 or qs[3] != 64 or ks[3] != 64 or ks[0] != qs[0] or v.shape != ks or out.shape != qs:
         raise ValueError(f"attention_fwd: q, out must be [B, Lq, H, 64] and k, v [B, Lk, Hkv, 64], got {[tuple(t.shape) for t in (q, out, k, v)]}")
@@ -775,11 +775,11 @@ def attention_bwd(dout: T, q: T, k: T, v: T, out: T, lse: T, scale: float, causa
     are recomputed.  dk / dv are sums over the query heads that share them; rows behind a length get zeros."""
     dev = _train_device("attention_bwd", q, k, v, dout, out, lse, q_len, kv_len, dq, dk, dv)
     if dq is None:
-        dq = torch.empty_like(q)
+        dq = _dense_like(q)
     if dk is None:
-        dk = torch.empty_like(k)
+        dk = _dense_like(k)
     if dv is None:
-        dv = torch.empty_like(v)
+        dv = _dense_like(v)
     qs, ks, dt = q.shape, k.shape, q.dtype
     if len(qs) != 4 or len(ks) != 4 or qs[3] != 64 or ks[3] != 64 or ks[0] != qs[0] or not (v.shape == dk.shape == dv.shape == ks) or \
             not (out.shape == dout.shape == dq.shape == qs):
@@ -815,6 +815,8 @@ def layernorm_fwd(x: T, gamma: T, beta: T, eps: float = 1e-5, out: Optional[T] =
     if out.shape != shape or gamma.shape != (C,) or beta.shape != (C,) or not gamma.is_contiguous() or not beta.is_contiguous():
         raise ValueError("layernorm_fwd: out must have the shape of x, gamma and beta be contiguous of its last dimension")
     stats = torch.empty(shape[:-1] + (2,), dtype=torch.float32, device=x.device)
+    if stats.numel() >= 1 << 31 or C >= 1 << 31:
+        raise ValueError("layernorm_fwd: more than 2^30 rows or 2^31 columns")
     _train_call("dbir_layernorm_fwd", dev, dt, x.data_ptr(), _row_ld(x, "layernorm_fwd: x"), out.data_ptr(), _row_ld(out, "layernorm_fwd: out"),
                 gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(), stats.numel() >> 1, C, eps)
     return out, stats
@@ -853,6 +855,8 @@ def embedding(tokens: T, table: T, scale: float = 1.0, pos: Optional[T] = None, 
     if tokens.dtype != torch.int64 or not ts or not tokens.is_contiguous() or table.dim() != 2:
         raise ValueError("embedding: tokens must be contiguous int64 [..., L], table [vocab, W]")
     (vocab, W), L = table.shape, ts[-1]
+    if tokens.numel() >= 1 << 30 or vocab >= 1 << 31:
+        raise ValueError("embedding: more than 2^30 tokens or 2^31 rows")
     if pos is not None and (pos.dtype != torch.float32 or pos.dim() != 2 or pos.shape[0] < L or pos.shape[1] != W):
         raise ValueError(f"embedding: pos must be f32 [>= {L}, {W}]")
     if out is None:
@@ -881,6 +885,8 @@ def embedding_bwd(dy: T, tokens: T, vocab: int, scale: float = 1.0, pos_rows: in
     if vocab <= 0 or (padding_idx is not None and not 0 <= padding_idx < vocab):
         raise ValueError("embedding_bwd: padding_idx must be a row of the table")
     W, L, n = ds[-1], ts[-1], tokens.numel()
+    if n >= 1 << 30 or vocab >= 1 << 31 or not 0 <= pos_rows < 1 << 23:
+        raise ValueError("embedding_bwd: more than 2^30 tokens, 2^31 rows or 2^23 positions")
     if out is None:
         if accumulate:
             raise ValueError("embedding_bwd: accumulate needs `out`")

@@ -93,7 +93,7 @@ def test_embedding_refusals(no_launch):
     dy = torch.zeros(2, 3, 8)
     for args, kw in [((dy[:1], tok, 5), {}), ((dy, tok, 0), {}), ((dy, tok, 5), dict(padding_idx=5)), ((dy, tok, 5), dict(padding_idx=-1)),
                      ((dy, tok, 5), dict(accumulate=True)), ((dy, tok, 5), dict(out=torch.zeros(5, 8).half())), ((dy, tok, 5), dict(out=torch.zeros(4, 8))),
-                     ((dy.double(), tok, 5), {})]:
+                     ((dy.double(), tok, 5), {}), ((dy, tok, 5), dict(pos_rows=1 << 23)), ((dy, tok, 5), dict(pos_rows=-1)), ((dy, tok, 1 << 31), {})]:
         with pytest.raises((ValueError, TypeError)):
             ops.embedding_bwd(*args, **kw)
     assert no_launch == []
@@ -177,7 +177,7 @@ def test_packed_descriptor_is_the_struct():
 def test_norm_and_embedding_refusals(lib):
     p, r, t, big = 1 << 20, 2 << 20, 3 << 20, 1 << 30
     fwd = [0, p, 8, r, 8, p, p, p, 4, 8, 1e-5, None]
-    for i, v in [(0, 3), (0, -1), (1, None), (2, 7), (3, None), (3, p), (4, 7), (5, None), (7, None), (8, 0), (9, 0)]:
+    for i, v in [(0, 3), (0, -1), (1, None), (2, 7), (3, None), (3, p), (4, 7), (5, None), (7, None), (8, 0), (9, 0), (10, -1.0), (10, float("nan"))]:
         a = list(fwd)
         a[i] = v
         assert lib.dbir_layernorm_fwd(*a) == 1, (i, v)

@@ -248,6 +248,30 @@ def test_attention_train_far_rows():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("Lq,Lk", [(100, 100), (100, 700)])
+def test_attention_train_broadcast_keys(Lq, Lk, dtype):
+    """Keys and values shared by a batch (expanded): their gradient is the sum over the samples of what is returned."""
+    q, k, v, do = attn_inputs(3, 2, 2, Lq, Lk, dtype, 22)
+    k, v = k[:1].expand(3, -1, -1, -1), v[:1].expand(3, -1, -1, -1)
+    attn_check(q, k, v, do)
+
+
+def test_attention_train_lengths_out_of_range_and_nan():
+    """Lengths below 0 or beyond the tensor count as 0 and as the whole; a NaN in a visible place reaches its row, and no other sample."""
+    q, k, v, do = attn_inputs(3, 2, 2, 90, 130, F16, 23)
+    bad, good = (torch.tensor(t, dtype=torch.int32, device=DEV) for t in ((-5, 1000, 70), (0, 130, 70)))
+    out, lse = ops.attention_fwd(q, k, v, 0.125, kv_len=bad)
+    for a, b in zip(attn_check(q, k, v, do, kv_len=good), (out, lse, *ops.attention_bwd(do, q, k, v, out, lse, 0.125, kv_len=bad))):
+        assert torch.equal(a, b)
+    q[1, 7, 0, 3] = math.nan
+    out, lse = ops.attention_fwd(q, k, v, 0.125)
+    assert out[1, 7, 0].isnan().all() and lse[1, 0, 7].isnan() and out.isnan().sum() == 64 and lse.isnan().sum() == 1
+    dq, dk, dv = ops.attention_bwd(do, q, k, v, out, lse, 0.125)
+    assert dq[1, 7, 0].isnan().all() and dk[1, :, 0].isnan().all() and not any(t[::2].isnan().any() for t in (dq, dk, dv))
+    assert not any(t[1, :, 1].isnan().any() for t in (dq, dk, dv))
+
+
 # ------------------------------------------------------------------------------------------------ layer norm
 def ln_ref(x, dy, gamma, beta, eps, dres=None):
     x, dy, gamma, beta = (t.double() for t in (x, dy, gamma, beta))
