@@ -384,7 +384,8 @@ __global__ __launch_bounds__(NW * 64) void embed_rows_kernel(const typename T::e
       if (accumulate) F32T::load4(d + c0 + lane * 4, f);
 #pragma unroll
       for (int k = 0; k < 4; ++k) f[k] = __builtin_fmaf(acc[k], scale, f[k]);
-      F32T::store4(d + c0 + lane * 4, f);
+      typedef __attribute__((ext_vector_type(4))) float f32v4;   // past the caches: written once, and most of the table is not read soon
+      __builtin_nontemporal_store(f32v4{f[0], f[1], f[2], f[3]}, reinterpret_cast<f32v4*>(d + c0 + lane * 4));
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
