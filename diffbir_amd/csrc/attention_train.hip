@@ -351,7 +351,6 @@ __global__ __launch_bounds__(256) void attn_bwd_join_kernel(const Args a) {
   if (WIDTH == 64 && c == 0) a.nd[(long long)bh * a.Lqp + row] -= d;
 }
 
-
 // ---------------------------------------------------------------------------------------------------------------- backward
 // f16: p and ds are operands of 11 bits between 2^-14 and 65504, and ds may be far below (4096 keys, a gradient of 1e-3: 1e-6) or, with
 // a loss scale, above.  Both are formed times 2^e, which the result is divided by: |ds| <= 2 max|do| max|v| must stay under 2^15,
@@ -687,8 +686,7 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_small_kernel(const Args a) {
   }
   for (int h = hk * grp; h < hk * grp + grp; ++h) {
     q_part<T, true>(a, lds, b, h, 0, 0, e);
-    __threadfence_block();   // its nl2 and nd, for the next part; the tiles in LDS are done with
-    __syncthreads();
+    tile_ready();   // its nl2 and nd are written, for the next part; the tiles in LDS are done with
   }
   kv_part<T, CAUSAL>(a, lds, b, hk, 0, 0, e);
 }
@@ -699,7 +697,7 @@ const char* bad_layout(const void* p, const long long* s, int B, int rows, int h
   if (!p || (reinterpret_cast<uintptr_t>(p) & 15)) return "must be 16-byte aligned and not NULL";
   const int n[3] = {B, rows, heads};
   for (int i = 0; i < 3; ++i)
-    if (n[i] > 1 && (s[i] < 0 || s[i] % 8 || (written && s[i] == 0))) return "needs strides that are multiples of 8 elements (an output: none of 0)";
+    if (n[i] > 1 && (s[i] < 0 || s[i] % 8 || (written && s[i] < HD))) return "needs strides that are multiples of 8 elements (an output: of at least 64)";
   if (rows > 1 && (s[1] < HD || s[1] >= (1 << 23))) return "needs rows at least 64 and less than 2^23 elements apart";
   return nullptr;
 }
@@ -717,7 +715,7 @@ int check_desc(const dbir_attn_desc* d, const char* name, bool bwd) {
   DBIR_CHECK_ARG(d->Lq <= (1 << 30) && d->Lk <= (1 << 30), "%s: more than 2^30 rows", name);
   DBIR_CHECK_ARG((long long)d->B * d->H <= 65535 && (long long)cdiv(d->Lq, 128) * d->B * d->H < (1 << 24) &&
                      (long long)cdiv(d->Lk, 128) * d->B * d->Hkv < (1 << 24), "%s: grid too large", name);
-  DBIR_CHECK_ARG(d->scale > 0.f && d->scale < INFINITY, "%s: scale must be positive and finite", name);
+  DBIR_CHECK_ARG(d->scale >= 1e-30f && d->scale <= 1e30f, "%s: scale must lie between 1e-30 and 1e30", name);
   DBIR_CHECK_ARG(d->lse, "%s: null lse", name);
   CHECK_LAYOUT(q, q_stride, Lq, H, false);
   CHECK_LAYOUT(k, k_stride, Lk, Hkv, false);

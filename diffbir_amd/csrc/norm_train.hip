@@ -30,6 +30,9 @@ struct H16T {
   static __device__ __forceinline__ void store(u16* p, float v) { *p = T::from_f32(v); }
   static __device__ __forceinline__ void unpack(const uint4& v, float* f) { unpack8<T>(v, f); }
   static __device__ __forceinline__ uint4 pack(const float* f) { return pack8<T>(f); }
+  static __device__ __forceinline__ void unpack(const uint2& v, float* f) {
+    f[0] = T::to_f32((u16)v.x); f[1] = T::to_f32((u16)(v.x >> 16)); f[2] = T::to_f32((u16)v.y); f[3] = T::to_f32((u16)(v.y >> 16));
+  }
 };
 typedef H16T<F16> F16T;
 typedef H16T<BF16> BF16T;
@@ -42,30 +45,36 @@ __device__ __forceinline__ float block_sum(float v, float* red) {   // 256 threa
   return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// Rows held in registers: LPR lanes a row, VPL vectors of V elements a lane (V = 16 bytes' worth, or 1 where the rows are not aligned for
+// Rows held in registers: LPR lanes a row, VPL vectors of V elements a lane (16 or 8 bytes, or one element where the rows are not aligned for
 // that), vector v = lane + LPR i.  A group goes through rows `step` apart, backwards with gamma and the column sums in its registers.
 // Every byte is read once: the bound is memory (figures at the host rule below).
-template <typename T, int V>
-__device__ __forceinline__ void load_vec(const typename T::elem* p, float* f) {
-  if constexpr (V == 1) f[0] = T::load(p);
-  else T::unpack(*reinterpret_cast<const uint4*>(p), f);
-}
-template <typename T, int V>
-__device__ __forceinline__ void store_vec(typename T::elem* p, const float* f) {
-  if constexpr (V == 1) T::store(p, f[0]);
-  else *reinterpret_cast<uint4*>(p) = T::pack(f);
-}
-// a vector as it lies in memory
+// V elements as they lie in memory: 16 bytes, 8 (four of 16 bits) or one element
 template <typename T, int V>
 struct Raw {
   typedef uint4 type;
   static __device__ __forceinline__ void unpack(const uint4& v, float* f) { T::unpack(v, f); }
+  static __device__ __forceinline__ uint4 pack(const float* f) { return T::pack(f); }
+};
+template <typename T>
+struct Raw<H16T<T>, 4> {
+  typedef uint2 type;
+  static __device__ __forceinline__ void unpack(const uint2& v, float* f) { H16T<T>::unpack(v, f); }
+  static __device__ __forceinline__ uint2 pack(const float* f) { return make_uint2(T::pack2(f[0], f[1]), T::pack2(f[2], f[3])); }
 };
 template <typename T>
 struct Raw<T, 1> {
   typedef typename T::elem type;
   static __device__ __forceinline__ void unpack(const type& v, float* f) { f[0] = T::load(&v); }
+  static __device__ __forceinline__ type pack(const float* f) {
+    type v;
+    T::store(&v, f[0]);
+    return v;
+  }
 };
+template <typename T, int V>
+__device__ __forceinline__ void load_vec(const typename T::elem* p, float* f) { Raw<T, V>::unpack(*reinterpret_cast<const typename Raw<T, V>::type*>(p), f); }
+template <typename T, int V>
+__device__ __forceinline__ void store_vec(typename T::elem* p, const float* f) { *reinterpret_cast<typename Raw<T, V>::type*>(p) = Raw<T, V>::pack(f); }
 // gamma / beta: 16 bytes at a time where rows are wide (they are aligned then)
 template <int V>
 __device__ __forceinline__ void load_f32(const float* p, int c, bool ok, float* f) {
@@ -85,40 +94,44 @@ __device__ __forceinline__ float row_sum(float v) {
   for (int o = (LPR > 64 ? 64 : LPR) / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
-// two sums over the lanes of a row; with four waves a row through `red`, whose halves are used in turn (one barrier a call)
+constexpr int threads_of(int lpr) { return lpr > 256 ? lpr : 256; }
+// two sums over the lanes of a row; with several waves a row through `red`, whose halves are used in turn (one barrier a call)
 template <int LPR>
-__device__ __forceinline__ void row_sum2(float& a, float& b, float (*red)[8], int& turn) {
+__device__ __forceinline__ void row_sum2(float& a, float& b, float (*red)[32], int& turn) {
   a = row_sum<LPR>(a);
   b = row_sum<LPR>(b);
-  if constexpr (LPR == 256) {
+  if constexpr (LPR > 64) {
     float* r = red[turn];
     turn ^= 1;
     if ((threadIdx.x & 63) == 0) {
       r[threadIdx.x >> 6] = a;
-      r[4 + (threadIdx.x >> 6)] = b;
+      r[16 + (threadIdx.x >> 6)] = b;
     }
     __syncthreads();
-    a = (r[0] + r[1]) + (r[2] + r[3]);
-    b = (r[4] + r[5]) + (r[6] + r[7]);
+    a = b = 0.f;
+#pragma unroll
+    for (int w = 0; w < LPR / 64; ++w) {
+      a += r[w];
+      b += r[16 + w];
+    }
   }
 }
 
 template <typename T, int V, int LPR, int VPL>
-__global__ __launch_bounds__(256) void ln_fwd_kernel(const typename T::elem* __restrict__ x, long long ldx, typename T::elem* __restrict__ y, long long ldy,
+__global__ __launch_bounds__(threads_of(LPR)) void ln_fwd_kernel(const typename T::elem* __restrict__ x, long long ldx, typename T::elem* __restrict__ y, long long ldy,
                                                      const float* __restrict__ gamma, const float* __restrict__ beta, float* __restrict__ stats, int rows,
                                                      int C, float eps) {
-  constexpr int GROUPS = 256 / LPR;
-  __shared__ float red[2][8];
+  constexpr int GROUPS = threads_of(LPR) / LPR;
+  __shared__ float red[2][32];
   const int l = threadIdx.x % LPR, nv = C / V, step = gridDim.x * GROUPS;
   int turn = 0;
-  for (int row = blockIdx.x * GROUPS + threadIdx.x / LPR; row < rows; row += step) {   // (LPR = 256: the same for the whole workgroup)
+  for (int row = blockIdx.x * GROUPS + threadIdx.x / LPR; row < rows; row += step) {   // (LPR >= 256: the same for the whole workgroup)
     const typename T::elem* xr = x + (long long)row * ldx;
     float f[VPL][V], s = 0.f, q = 0.f;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      if (l + LPR * i < nv) {
-        load_vec<T, V>(xr + (l + LPR * i) * V, f[i]);
-      } else {
+      load_vec<T, V>(xr + min(l + LPR * i, nv - 1) * V, f[i]);   // (lanes without a column read the last one and drop it)
+      if (l + LPR * i >= nv) {
 #pragma unroll
         for (int e = 0; e < V; ++e) f[i][e] = 0.f;
       }
@@ -139,27 +152,26 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const typename T::elem* __r
     row_sum2<LPR>(q, z, red, turn);
     const float rstd = 1.f / sqrtf(q / (float)C + eps);
 #pragma unroll
-    for (int i = 0; i < VPL; ++i)
-      if (l + LPR * i < nv) {
-        float g[V], b[V];   // (from the cache: held in registers they cost more waves than they save)
-        load_f32<V>(gamma, (l + LPR * i) * V, true, g);
-        load_f32<V>(beta, (l + LPR * i) * V, true, b);
+    for (int i = 0; i < VPL; ++i) {
+      float g[V], b[V];   // (from the cache: held in registers they cost more waves than they save)
+      load_f32<V>(gamma, min(l + LPR * i, nv - 1) * V, true, g);
+      load_f32<V>(beta, min(l + LPR * i, nv - 1) * V, true, b);
 #pragma unroll
-        for (int e = 0; e < V; ++e) f[i][e] = __builtin_fmaf(f[i][e] * rstd, g[e], b[e]);
-        store_vec<T, V>(y + (long long)row * ldy + (l + LPR * i) * V, f[i]);
-      }
+      for (int e = 0; e < V; ++e) f[i][e] = __builtin_fmaf(f[i][e] * rstd, g[e], b[e]);
+      if (l + LPR * i < nv) store_vec<T, V>(y + (long long)row * ldy + (l + LPR * i) * V, f[i]);
+    }
     if (l == 0) *reinterpret_cast<float2*>(stats + 2LL * row) = make_float2(mean, rstd);
   }
 }
 
 // dx, and this workgroup's sums of the columns: part[workgroup][0][c] = sum dy xh, [1][c] = sum dy
 template <typename T, int V, int LPR, int VPL>
-__global__ __launch_bounds__(256) void ln_bwd_kernel(const typename T::elem* __restrict__ dy, long long ldg, const typename T::elem* __restrict__ x,
+__global__ __launch_bounds__(threads_of(LPR)) void ln_bwd_kernel(const typename T::elem* __restrict__ dy, long long ldg, const typename T::elem* __restrict__ x,
                                                      long long ldx, const typename T::elem* __restrict__ dres, long long ldr,
                                                      typename T::elem* __restrict__ dx, long long ldd, const float* __restrict__ gamma,
                                                      const float* __restrict__ stats, float* __restrict__ part, int rows, int C) {
-  constexpr int GROUPS = 256 / LPR, WAVES = LPR == 256 ? 1 : 4;   // waves that hold the same columns
-  __shared__ float red[2][8];
+  constexpr int GROUPS = threads_of(LPR) / LPR, WAVES = LPR >= 256 ? 1 : 4;   // waves that hold the same columns
+  __shared__ float red[2][32];
   __shared__ float cols[WAVES > 1 ? 3 * 64 * V : 1];
   const int l = threadIdx.x % LPR, nv = C / V, step = gridDim.x * GROUPS;
   const float inv = 1.f / (float)C;
@@ -353,42 +365,59 @@ int any_chunks(int rows, int C) {   // partial rows: about 2048 workgroups over 
 struct Shape {
   int v, lpr, vpl;   // v = 0: too wide for registers
 };
-Shape shape_of(int dtype, int C, bool wide, bool fwd) {
-  const int v = wide ? (dtype == DBIR_F32 ? 4 : 8) : 1, nv = C / v;
-  if (wide && fwd && nv > 32 && nv <= 160) return nv <= 40 ? Shape{v, 8, 5} : nv <= 80 ? Shape{v, 16, 5} : Shape{v, 32, 5};   // (no column sums to hold)
-  if (!wide) return nv <= 256 ? Shape{1, 64, 4} : nv <= 2048 ? Shape{1, 256, 8} : nv <= 4096 ? Shape{1, 256, 16} : Shape{0, 0, 0};
+Shape shape_of(int C, int v, bool fwd) {   // v: elements of a vector
+  const int nv = C / v;
+  if (v == 1) return nv <= 256 ? Shape{1, 64, 4} : nv <= 2048 ? Shape{1, 256, 8} : nv <= 4096 ? Shape{1, 256, 16} : nv > 8192 ? Shape{0, 0, 0} :
+                     fwd ? Shape{1, 256, 32} : Shape{1, 1024, 8};
+  if (fwd && nv > 32 && nv <= 160) return nv <= 40 ? Shape{v, 8, 5} : nv <= 80 ? Shape{v, 16, 5} : Shape{v, 32, 5};   // (no column sums to hold)
   return nv <= 8 ? Shape{v, 8, 1} : nv <= 32 ? Shape{v, 32, 1} : nv <= 64 ? Shape{v, 32, 2} : nv <= 128 ? Shape{v, 64, 2} : nv <= 192 ? Shape{v, 64, 3} :
-         nv <= 320 ? Shape{v, 64, 5} : nv <= 512 ? Shape{v, 256, 2} : nv <= 1024 ? Shape{v, 256, 4} : Shape{0, 0, 0};
+         nv <= 320 ? Shape{v, 64, 5} : nv <= 512 ? Shape{v, 256, 2} : nv <= 1024 ? Shape{v, 256, 4} : nv <= 2048 ? Shape{v, 1024, 2} : Shape{0, 0, 0};
 }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-bool is_wide(int dtype, int C, const void* p, long long ld) {
-  const int v = dtype == DBIR_F32 ? 4 : 8;
-  return C % v == 0 && ld % v == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+// the widest vectors (8, 4 or 1 elements) that C and these rows allow
+int vector_of(int dtype, int C) { return dtype != DBIR_F32 && C % 8 == 0 ? 8 : C % 4 == 0 ? 4 : 1; }
+int vector_of(int dtype, int C, const void* p, long long ld) {
+  int v = vector_of(dtype, C);
+  const int size = dtype == DBIR_F32 ? 4 : 2;
+  while (v > 1 && (ld % v || reinterpret_cast<uintptr_t>(p) % (v * size))) v = v == 8 ? 4 : 1;
+  return v;
 }
-// workgroups of the backward pass = partial rows of the column sums: one row a group up to 512 workgroups (two a CU), then more rows a group
+// Workgroups of the backward pass = partial rows of the column sums: one row a group up to 512 (two a CU), then more rows a group (32768 x 320
+// f16: 25.1 us with 256, 19.1 with 512, 21.8 with 1024).  Narrow unaligned rows have too little in flight for that: up to 2048 while a group
+// keeps eight rows (65536 x 101 f16: 43.4 -> 33.0 us; for 16-byte rows it loses, 50000 x 520 bf16: 40.5 -> 56.2).
 int bwd_groups(int rows, const Shape& sh) {
-  const int n = cdiv(rows, 256 / sh.lpr);
-  return n < 512 ? n : 512;
+  const int n = cdiv(rows, threads_of(sh.lpr) / sh.lpr), most = sh.v > 1 || sh.lpr > 64 || n < 4096 ? 512 : n / 8 < 2048 ? n / 8 : 2048;
+  return n < most ? n : most;
 }
-int bwd_parts(int dtype, int rows, int C, bool wide) {
-  const Shape sh = shape_of(dtype, C, wide, false);
+int bwd_parts(int rows, int C, int v) {
+  const Shape sh = shape_of(C, v, false);
   return sh.v ? bwd_groups(rows, sh) : any_chunks(rows, C);
 }
 
-#define EACH_SHAPE(GO, T)                                                                              \
-  do {                                                                                                 \
-    if (sh.v > 1) {                                                                                    \
-      if (sh.lpr == 8) GO(T, T::wide, 8, 1);                                                           \
-      else if (sh.lpr == 32 && sh.vpl == 1) GO(T, T::wide, 32, 1);                                     \
-      else if (sh.lpr == 32) GO(T, T::wide, 32, 2);                                                    \
-      else if (sh.lpr == 64 && sh.vpl == 2) GO(T, T::wide, 64, 2);                                     \
-      else if (sh.lpr == 64 && sh.vpl == 3) GO(T, T::wide, 64, 3);                                     \
-      else if (sh.lpr == 64) GO(T, T::wide, 64, 5);                                                    \
-      else if (sh.vpl == 2) GO(T, T::wide, 256, 2);                                                    \
-      else GO(T, T::wide, 256, 4);                                                                     \
-    } else if (sh.lpr == 64) GO(T, 1, 64, 4);                                                          \
-    else if (sh.vpl == 8) GO(T, 1, 256, 8);                                                            \
-    else GO(T, 1, 256, 16);                                                                            \
+#define WIDE_SHAPES(GO, T, V)                                         \
+  do {                                                                \
+    if (sh.lpr == 8) GO(T, V, 8, 1);                                  \
+    else if (sh.lpr == 32 && sh.vpl == 1) GO(T, V, 32, 1);            \
+    else if (sh.lpr == 32) GO(T, V, 32, 2);                           \
+    else if (sh.lpr == 64 && sh.vpl == 2) GO(T, V, 64, 2);            \
+    else if (sh.lpr == 64 && sh.vpl == 3) GO(T, V, 64, 3);            \
+    else if (sh.lpr == 64) GO(T, V, 64, 5);                           \
+    else if (sh.lpr == 1024) GO(T, V, 1024, 2);                       \
+    else if (sh.vpl == 2) GO(T, V, 256, 2);                           \
+    else GO(T, V, 256, 4);                                            \
+  } while (0)
+#define FWD_SHAPES(GO, T, V)                                          \
+  do {                                                                \
+    if (sh.lpr == 8 && sh.vpl == 5) GO(T, V, 8, 5);                   \
+    else if (sh.lpr == 16) GO(T, V, 16, 5);                           \
+    else if (sh.lpr == 32 && sh.vpl == 5) GO(T, V, 32, 5);            \
+    else WIDE_SHAPES(GO, T, V);                                       \
+  } while (0)
+#define SINGLE_SHAPES(GO, T)                                          \
+  do {                                                                \
+    if (sh.lpr == 64) GO(T, 1, 64, 4);                                \
+    else if (sh.vpl == 8) GO(T, 1, 256, 8);                           \
+    else GO(T, 1, 256, 16);                                           \
   } while (0)
 
 template <typename T>
@@ -400,14 +429,14 @@ void launch_fwd(const Shape& sh, const void* x, long long ldx, void* y, long lon
                        eps);
     return;
   }
-  const int n = cdiv(rows, 256 / sh.lpr);
+  const int n = cdiv(rows, threads_of(sh.lpr) / sh.lpr);
   const dim3 grid((unsigned)(n < 2048 ? n : 2048));
 #define GO(TT, V, LPR, VPL) \
-  hipLaunchKernelGGL((ln_fwd_kernel<TT, V, LPR, VPL>), grid, dim3(256), 0, s, (const E*)x, ldx, (E*)y, ldy, gamma, beta, stats, rows, C, eps)
-  if (sh.v > 1 && sh.lpr == 8 && sh.vpl == 5) GO(T, T::wide, 8, 5);
-  else if (sh.v > 1 && sh.lpr == 16) GO(T, T::wide, 16, 5);
-  else if (sh.v > 1 && sh.lpr == 32 && sh.vpl == 5) GO(T, T::wide, 32, 5);
-  else EACH_SHAPE(GO, T);
+  hipLaunchKernelGGL((ln_fwd_kernel<TT, V, LPR, VPL>), grid, dim3(threads_of(LPR)), 0, s, (const E*)x, ldx, (E*)y, ldy, gamma, beta, stats, rows, C, eps)
+  if (sh.v == T::wide) FWD_SHAPES(GO, T, T::wide);
+  else if (sh.v == 4) FWD_SHAPES(GO, T, 4);
+  else if (sh.vpl == 32) GO(T, 1, 256, 32);
+  else SINGLE_SHAPES(GO, T);
 #undef GO
 }
 
@@ -423,9 +452,12 @@ void launch_bwd(const Shape& sh, int n, const void* dy, long long ldg, const voi
     return;
   }
 #define GO(TT, V, LPR, VPL)                                                                                                                            \
-  hipLaunchKernelGGL((ln_bwd_kernel<TT, V, LPR, VPL>), dim3((unsigned)n), dim3(256), 0, s, (const E*)dy, ldg, (const E*)x, ldx, (const E*)dres, ldr, (E*)dx, \
+  hipLaunchKernelGGL((ln_bwd_kernel<TT, V, LPR, VPL>), dim3((unsigned)n), dim3(threads_of(LPR)), 0, s, (const E*)dy, ldg, (const E*)x, ldx, (const E*)dres, ldr, (E*)dx, \
                      ldd, gamma, stats, ws, rows, C)
-  EACH_SHAPE(GO, T);
+  if (sh.v == T::wide) WIDE_SHAPES(GO, T, T::wide);
+  else if (sh.v == 4) WIDE_SHAPES(GO, T, 4);
+  else if (sh.lpr == 1024) GO(T, 1, 1024, 8);
+  else SINGLE_SHAPES(GO, T);
 #undef GO
 }
 
@@ -434,11 +466,10 @@ void launch_bwd(const Shape& sh, int n, const void* dy, long long ldg, const voi
 extern "C" int dbir_layernorm_bwd_ws(int rows, int C, long long* bytes) {
   DBIR_CHECK_ARG(rows > 0 && C > 0 && bytes, "dbir_layernorm_bwd_ws: bad arguments");
   int n = 0;   // whatever type and alignment the call has
-  for (int dtype = 0; dtype < 3; ++dtype)
-    for (int wide = 0; wide < 2; ++wide) {
-      const int m = bwd_parts(dtype, rows, C, wide && C % (dtype == DBIR_F32 ? 4 : 8) == 0);
-      n = m > n ? m : n;
-    }
+  for (int v = 8; v >= 1; v = v == 8 ? 4 : v == 4 ? 1 : 0) {
+    const int m = C % v ? 0 : bwd_parts(rows, C, v);
+    n = m > n ? m : n;
+  }
   *bytes = 8LL * C * n;
   return DBIR_OK;
 }
@@ -452,7 +483,8 @@ extern "C" int dbir_layernorm_fwd(int dtype, const void* x, long long ldx, void*
   DBIR_CHECK_ARG(dtype >= DBIR_F16 && dtype <= DBIR_F32, "dbir_layernorm_fwd: bad dtype %d", dtype);
   DBIR_CHECK_ARG((reinterpret_cast<uintptr_t>(stats) & 7) == 0, "dbir_layernorm_fwd: stats must be 8-byte aligned");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  const Shape sh = shape_of(dtype, C, is_wide(dtype, C, x, ldx) && is_wide(dtype, C, y, ldy) && aligned16(gamma) && aligned16(beta), true);
+  const int vx = vector_of(dtype, C, x, ldx), vy = vector_of(dtype, C, y, ldy);
+  const Shape sh = shape_of(C, aligned16(gamma) && aligned16(beta) ? (vx < vy ? vx : vy) : 1, true);
   if (dtype == DBIR_F16) launch_fwd<F16T>(sh, x, ldx, y, ldy, gamma, beta, stats, rows, C, eps, s);
   else if (dtype == DBIR_BF16) launch_fwd<BF16T>(sh, x, ldx, y, ldy, gamma, beta, stats, rows, C, eps, s);
   else launch_fwd<F32T>(sh, x, ldx, y, ldy, gamma, beta, stats, rows, C, eps, s);
@@ -468,9 +500,15 @@ extern "C" int dbir_layernorm_bwd(int dtype, const void* dy, long long ldg, cons
   DBIR_CHECK_ARG(dx != x && dx != dy && dx != dres, "dbir_layernorm_bwd: dx must not be an input");
   DBIR_CHECK_ARG(dtype >= DBIR_F16 && dtype <= DBIR_F32, "dbir_layernorm_bwd: bad dtype %d", dtype);
   DBIR_CHECK_ARG(((reinterpret_cast<uintptr_t>(stats) & 7) | (reinterpret_cast<uintptr_t>(ws) & 3)) == 0, "dbir_layernorm_bwd: stats must be 8-byte aligned");
-  const bool wide = aligned16(gamma) && is_wide(dtype, C, dy, ldg) && is_wide(dtype, C, x, ldx) && is_wide(dtype, C, dx, ldd) && (!dres || is_wide(dtype, C, dres, ldr));
-  const Shape sh = shape_of(dtype, C, wide, false);
-  const int n = bwd_parts(dtype, rows, C, wide);
+  int v = aligned16(gamma) ? vector_of(dtype, C) : 1;
+  const void* at[4] = {dy, x, dx, dres ? dres : x};
+  const long long lds[4] = {ldg, ldx, ldd, dres ? ldr : ldx};
+  for (int i = 0; i < 4; ++i) {
+    const int vi = vector_of(dtype, C, at[i], lds[i]);
+    v = vi < v ? vi : v;
+  }
+  const Shape sh = shape_of(C, v, false);
+  const int n = bwd_parts(rows, C, v);
   DBIR_CHECK_ARG(ws_bytes >= 8LL * C * n, "dbir_layernorm_bwd: the workspace must hold %lld bytes", 8LL * C * n);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   if (dtype == DBIR_F16) launch_bwd<F16T>(sh, n, dy, ldg, x, ldx, dres, ldr, dx, ldd, gamma, stats, ws, rows, C, s);

@@ -144,9 +144,9 @@ def good_desc():
 
 @pytest.mark.parametrize("change", [
     dict(dtype=2), dict(dtype=-1), dict(B=0), dict(H=0), dict(Hkv=0), dict(H=3, Hkv=2), dict(Lq=0), dict(Lk=0), dict(Lk=-1), dict(B=70000),
-    dict(scale=0.0), dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(q=None), dict(k=None), dict(v=None), dict(out=None),
+    dict(scale=0.0), dict(scale=1e-31), dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(q=None), dict(k=None), dict(v=None), dict(out=None),
     dict(lse=None), dict(q=(1 << 20) + 2), dict(q_stride=(0, 60, 64)), dict(k_stride=(0, 32, 64)), dict(v_stride=(0, 1 << 23, 64)),
-    dict(out_stride=(0, 64, 4)), dict(q_stride=(-64, 64, 64)), dict(k_stride=(8192, 128, 4)), dict(dq_stride=(0, 128, 64)), dict(dv_stride=(8192, 128, 0)), dict(dq=1 << 20), dict(dk=6 << 20),
+    dict(out_stride=(0, 64, 4)), dict(q_stride=(-64, 64, 64)), dict(k_stride=(8192, 128, 4)), dict(dq_stride=(0, 128, 64)), dict(dv_stride=(8192, 128, 0)), dict(dq_stride=(8192, 128, 8)), dict(dk_stride=(56, 128, 64)), dict(dq=1 << 20), dict(dk=6 << 20),
     dict(dv=2 << 20), dict(dq=8 << 20, dk=8 << 20), dict(dv=7 << 20), dict(dout=None), dict(dq=None), dict(dk=(1 << 20) + 8), dict(dv_stride=(0, 0, 64)),
     dict(ws=None), dict(ws_bytes=16), dict(ws=(1 << 20) + 4)])
 def test_attention_descriptor_refusals(lib, change):
@@ -155,7 +155,7 @@ def test_attention_descriptor_refusals(lib, change):
         setattr(d, n, (ctypes.c_longlong * 3)(*v) if isinstance(v, tuple) else v)
     assert lib.dbir_attention_bwd(ctypes.byref(d), None) == 1
     assert b"dbir_attention_bwd" in lib.dbir_last_error()
-    if not set(change) & {"dout", "dq", "dk", "dv", "dv_stride", "dq_stride", "ws", "ws_bytes"}:
+    if not set(change) & {"dout", "dq", "dk", "dv", "dv_stride", "dq_stride", "dk_stride", "ws", "ws_bytes"}:
         assert lib.dbir_attention_fwd(ctypes.byref(d), None) == 1
     assert lib.dbir_attention_fwd(None, None) == 1
 
