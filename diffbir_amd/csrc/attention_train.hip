@@ -51,8 +51,20 @@ __device__ __forceinline__ int xcd_range(int w, int n) {
   const int x = w & 7, i = w >> 3, per = n >> 3, rest = n & 7;
   return x * per + (x < rest ? x : rest) + i;
 }
-// The u-th head: the heads that share keys stay together, else the sequences alternate, so that each XCD has its part of the long ones in a padded
-// batch: 8 x 5 heads, lengths 128 to 4096, forward 175 -> 108 us, backward 512 -> 288.
+// The work of workgroup `wg` of heads x blocks x splits: the u-th head (of those of q, or of those of k) and the block `blk`, 0 the longest if CAUSAL.
+// Each XCD has a range of heads.  It goes through them one by one; with CAUSAL and heads that divide evenly over the XCDs through the longest blocks
+// of all its heads first (4 x 16 heads, 2048 rows: forward 66 -> 50 us, backward 189 -> 153), the heads turned by 3 a block so that the blocks of one do not meet on the same CUs.
+__device__ __forceinline__ void work_of(const Args& a, int heads, int blocks, int& u, int& blk, int& split) {
+  if (a.causal && (heads & 7) == 0) {
+    const int i = blockIdx.x >> 3, w = i / a.splits, mine = heads >> 3;
+    split = i % a.splits, blk = w / mine, u = (blockIdx.x & 7) * mine + (w % mine + 3 * blk) % mine;
+  } else {
+    const int i = xcd_range(blockIdx.x, gridDim.x), w = i / a.splits;
+    split = i % a.splits, blk = w % blocks, u = w / blocks;
+  }
+}
+// The u-th head of q: those that share keys stay together, else the sequences alternate, so that each XCD has its part of the long ones in a padded
+// batch (8 x 5 heads, lengths 128 to 4096: forward 175 -> 108 us, backward 512 -> 288).
 __device__ __forceinline__ void head_of(const Args& a, int u, int& b, int& h) {
   const int grp = a.H / a.Hkv, s = u / grp;
   b = s % a.B;
@@ -176,11 +188,12 @@ template <typename T>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char lds[4 * TILE_BYTES];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
-  const int nqb = (a.Lq + 127) >> 7, ws = xcd_range(blockIdx.x, gridDim.x), split = ws % a.splits, w = ws / a.splits;
-  int b, h;
-  head_of(a, w / nqb, b, h);
+  const int nqb = (a.Lq + 127) >> 7;
+  int u, blk, split, b, h;
+  work_of(a, a.B * a.H, nqb, u, blk, split);
+  head_of(a, u, b, h);
   const int bh = b * a.H + h, hk = h / (a.H / a.Hkv);
-  const int qb = a.causal ? nqb - 1 - w % nqb : w % nqb;   // (long rows first)
+  const int qb = a.causal ? nqb - 1 - blk : blk;   // (long rows first)
   const int nk = clamp_len(a.kv_len, b, a.Lk), nq = clamp_len(a.q_len, b, a.Lq), off = a.Lk - a.Lq;
   const int w0 = qb * 128 + wave * 32, row = w0 + (lane & 31);
   const bool q_ok = row < nq;
@@ -529,8 +542,10 @@ template <typename T, bool CAUSAL>
 __global__ __launch_bounds__(256, 2) void attn_bwd_kv_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char lds[KV_LDS];
   __shared__ float red[4];
-  const int nkb = (a.Lk + 127) >> 7, ws = xcd_range(blockIdx.x, gridDim.x), w = ws / a.splits, b = w / nkb % a.B, hk = w / nkb / a.B;
-  kv_part<T, CAUSAL>(a, lds, b, hk, (w % nkb) * 128, ws % a.splits, scale_exp<T>(a, b, hk, threadIdx.x, red));
+  int u, blk, split;
+  work_of(a, a.B * a.Hkv, (a.Lk + 127) >> 7, u, blk, split);
+  const int b = u % a.B, hk = u / a.B;
+  kv_part<T, CAUSAL>(a, lds, b, hk, blk * 128, split, scale_exp<T>(a, b, hk, threadIdx.x, red));
 }
 
 // dq: 128 queries a workgroup, 32 a wave; keys in tiles of 64, double buffered.  D = do . o comes from the ROUNDED o, and where one key has
@@ -675,10 +690,11 @@ template <typename T, bool EXACT>
 __global__ __launch_bounds__(256, EXACT ? 2 : 3) void attn_bwd_q_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char lds[4 * TILE_BYTES];
   __shared__ float red[4];
-  const int nqb = (a.Lq + 127) >> 7, ws = xcd_range(blockIdx.x, gridDim.x), w = ws / a.splits;
-  int b, h;
-  head_of(a, w / nqb, b, h);
-  q_part<T, EXACT>(a, lds, b, h, a.causal ? nqb - 1 - w % nqb : w % nqb, ws % a.splits, scale_exp<T>(a, b, h / (a.H / a.Hkv), threadIdx.x, red));
+  const int nqb = (a.Lq + 127) >> 7;
+  int u, blk, split, b, h;
+  work_of(a, a.B * a.H, nqb, u, blk, split);
+  head_of(a, u, b, h);
+  q_part<T, EXACT>(a, lds, b, h, a.causal ? nqb - 1 - blk : blk, split, scale_exp<T>(a, b, h / (a.H / a.Hkv), threadIdx.x, red));
 }
 
 // Up to 128 queries and keys: all of a key head in one workgroup and one launch.
@@ -786,7 +802,11 @@ Plan plan_of(int dtype, int B, int H, int Hkv, int Lq, int Lk) {
   p.exact = Lk <= 512;
   p.fwd = splits_of(bh * cdiv(Lq, 128), cdiv(Lk, TILE));
   p.q = p.exact ? 1 : p.fwd;   // (the correction needs all keys of a row)
-  p.kv = splits_of(bk * cdiv(Lk, 128), (long long)cdiv(Lq, TILE) * (H / Hkv));
+  // (a workgroup of dk and dv has the queries of all heads that share its keys: from 64 rounds on two splits pay below 1024 workgroups too,
+  // for the balance: 16 x 8 heads on 2, 2048 causal rows 300 -> 288 us, lengths 100 to 2048 217 -> 159; at 32 rounds 82 -> 86)
+  const long long groups = bk * cdiv(Lk, 128), rounds = (long long)cdiv(Lq, TILE) * (H / Hkv);
+  p.kv = splits_of(groups, rounds);
+  if (p.kv == 1 && groups < 1024 && rounds >= 64) p.kv = 2;
   p.lqp = ((long long)Lq + 63) / 64 * 64;
   p.rows_floats = (bh * p.lqp * 2 + (dtype == DBIR_F16 ? bh * (p.lqp / 64) + bk * ((Lk + 63) / 64) : 0) + 3) / 4 * 4;
   const long long nq = p.q > 1 && !p.small ? p.q * bh * Lq * (HD + 1) : 0, nk = p.kv > 1 && !p.small ? p.kv * bk * Lk * 128 : 0;
