@@ -111,7 +111,7 @@ def attn_check(q, k, v, do, scale=0.125, **kw):
     (1, 1, 1, 2, 2, False), (1, 1, 1, 32, 32, True), (2, 16, 16, 77, 77, True), (2, 5, 5, 256, 77, False), (1, 2, 1, 64, 64, False),
     (1, 3, 3, 65, 129, True), (2, 4, 2, 127, 128, True), (1, 8, 1, 129, 63, True), (3, 4, 2, 1, 300, False), (1, 2, 2, 300, 2, False),
     (1, 2, 2, 5, 1000, True), (1, 10, 5, 1, 2049, True), (2, 3, 1, 513, 511, False), (1, 1, 1, 1500, 1, False), (1, 20, 20, 16, 16, False),
-    (1, 2, 2, 200, 40, True)])
+    (1, 2, 2, 200, 40, True), (128, 22, 1, 129, 129, True), (128, 22, 1, 129, 130, False), (8, 3, 3, 300, 140, True)])
 def test_attention_train(B, H, Hkv, Lq, Lk, causal, dtype):
     q, k, v, do = attn_inputs(B, H, Hkv, Lq, Lk, dtype, 11)
     if Lk == 1:   # one key: its probability is 1 and no score has a gradient
