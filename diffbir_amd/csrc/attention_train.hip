@@ -14,6 +14,7 @@
 #include <math.h>
 
 #include <type_traits>
+#include <utility>
 
 #include "common.h"
 
@@ -724,8 +725,19 @@ const char* bad_layout(const void* p, const long long* s, int B, int rows, int h
   if (!p || (reinterpret_cast<uintptr_t>(p) & 15)) return "must be 16-byte aligned and not NULL";
   const int n[3] = {B, rows, heads};
   for (int i = 0; i < 3; ++i)
-    if (n[i] > 1 && (s[i] < 0 || s[i] % 8 || (written && s[i] < HD))) return "needs strides that are multiples of 8 elements (an output: of at least 64)";
+    if (n[i] > 1 && (s[i] < 0 || s[i] % 8)) return "needs strides that are multiples of 8 elements";
   if (rows > 1 && (s[1] < HD || s[1] >= (1 << 23))) return "needs rows at least 64 and less than 2^23 elements apart";
+  if (written) {   // no two elements in one place: in the order of the strides, each is at least what lies below it spans
+    int order[3] = {0, 1, 2};
+    for (int i = 0; i < 3; ++i)
+      for (int j = i + 1; j < 3; ++j)
+        if (s[order[j]] < s[order[i]]) std::swap(order[i], order[j]);
+    long long span = HD;
+    for (int i : order) {
+      if (n[i] > 1 && s[i] < span) return "is written to and must not overlap itself";
+      if (n[i] > 1) span += s[i] * (n[i] - 1);
+    }
+  }
   return nullptr;
 }
 #define CHECK_LAYOUT(P, S, ROWS, HEADS, WRITTEN)                                    \

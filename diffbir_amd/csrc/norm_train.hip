@@ -464,7 +464,7 @@ void launch_bwd(const Shape& sh, int n, const void* dy, long long ldg, const voi
 }  // namespace
 
 extern "C" int dbir_layernorm_bwd_ws(int rows, int C, long long* bytes) {
-  DBIR_CHECK_ARG(rows > 0 && C > 0 && bytes, "dbir_layernorm_bwd_ws: bad arguments");
+  DBIR_CHECK_ARG(rows > 0 && rows <= (1 << 30) && C > 0 && C <= (1 << 28) && bytes, "dbir_layernorm_bwd_ws: bad arguments");
   int n = 0;   // whatever type and alignment the call has
   for (int v = 8; v >= 1; v = v == 8 ? 4 : v == 4 ? 1 : 0) {
     const int m = C % v ? 0 : bwd_parts(rows, C, v);
@@ -477,7 +477,7 @@ extern "C" int dbir_layernorm_bwd_ws(int rows, int C, long long* bytes) {
 extern "C" int dbir_layernorm_fwd(int dtype, const void* x, long long ldx, void* y, long long ldy, const float* gamma, const float* beta,
                                   float* stats, int rows, int C, float eps, void* stream) {
   DBIR_CHECK_ARG(x && y && gamma && beta && stats, "dbir_layernorm_fwd: null pointer");
-  DBIR_CHECK_ARG(rows > 0 && rows <= (1 << 30) && C > 0 && ldx >= C && ldy >= C, "dbir_layernorm_fwd: bad rows / C / ld");
+  DBIR_CHECK_ARG(rows > 0 && rows <= (1 << 30) && C > 0 && C <= (1 << 28) && ldx >= C && ldy >= C, "dbir_layernorm_fwd: bad rows / C / ld");
   DBIR_CHECK_ARG(x != y, "dbir_layernorm_fwd: y must not be x");
   DBIR_CHECK_ARG(eps >= 0.f, "dbir_layernorm_fwd: eps must not be negative");
   DBIR_CHECK_ARG(dtype >= DBIR_F16 && dtype <= DBIR_F32, "dbir_layernorm_fwd: bad dtype %d", dtype);
@@ -496,7 +496,7 @@ extern "C" int dbir_layernorm_bwd(int dtype, const void* dy, long long ldg, cons
                                   void* dx, long long ldd, const float* gamma, const float* stats, float* dgamma, float* dbeta, int rows, int C,
                                   float* ws, long long ws_bytes, void* stream) {
   DBIR_CHECK_ARG(dy && x && dx && gamma && stats && dgamma && dbeta && ws, "dbir_layernorm_bwd: null pointer");
-  DBIR_CHECK_ARG(rows > 0 && rows <= (1 << 30) && C > 0 && ldg >= C && ldx >= C && ldd >= C && (!dres || ldr >= C), "dbir_layernorm_bwd: bad rows / C / ld");
+  DBIR_CHECK_ARG(rows > 0 && rows <= (1 << 30) && C > 0 && C <= (1 << 28) && ldg >= C && ldx >= C && ldd >= C && (!dres || ldr >= C), "dbir_layernorm_bwd: bad rows / C / ld");
   DBIR_CHECK_ARG(dx != x && dx != dy && dx != dres, "dbir_layernorm_bwd: dx must not be an input");
   DBIR_CHECK_ARG(dtype >= DBIR_F16 && dtype <= DBIR_F32, "dbir_layernorm_bwd: bad dtype %d", dtype);
   DBIR_CHECK_ARG(((reinterpret_cast<uintptr_t>(stats) & 7) | (reinterpret_cast<uintptr_t>(ws) & 3)) == 0, "dbir_layernorm_bwd: stats must be 8-byte aligned");

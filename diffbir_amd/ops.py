@@ -815,8 +815,8 @@ def layernorm_fwd(x: T, gamma: T, beta: T, eps: float = 1e-5, out: Optional[T] =
     if out.shape != shape or gamma.shape != (C,) or beta.shape != (C,) or not gamma.is_contiguous() or not beta.is_contiguous():
         raise ValueError("layernorm_fwd: out must have the shape of x, gamma and beta be contiguous of its last dimension")
     stats = torch.empty(shape[:-1] + (2,), dtype=torch.float32, device=x.device)
-    if stats.numel() >= 1 << 31 or C >= 1 << 31:
-        raise ValueError("layernorm_fwd: more than 2^30 rows or 2^31 columns")
+    if stats.numel() >= 1 << 31 or C > 1 << 28:
+        raise ValueError("layernorm_fwd: more than 2^30 rows or 2^28 columns")
     _train_call("dbir_layernorm_fwd", dev, dt, x.data_ptr(), _row_ld(x, "layernorm_fwd: x"), out.data_ptr(), _row_ld(out, "layernorm_fwd: out"),
                 gamma.data_ptr(), beta.data_ptr(), stats.data_ptr(), stats.numel() >> 1, C, eps)
     return out, stats

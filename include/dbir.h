@@ -287,7 +287,7 @@ int dbir_xf_tail(int dtype, const void* attn_out, long long ldo, const void* h, 
  *   those of batch, row and head in elements (multiples of 8; rows at least 64 and less than 2^23 apart; 16-byte aligned bases), so a slice of
  *   a wider buffer or a [B, H, L, 64] tensor serves as well (the stride of a dimension of one does not matter).  Outputs must not overlap
  *   inputs or each other.
- *   Outputs' strides are at least 64.  scale: 1e-30 .. 1e30.
+ *   An output must not overlap itself (rows read from an expanded tensor may).  scale: 1e-30 .. 1e30.
  *   lse f32 [B, H, Lq] dense: log of the sum of exp(scale q . k) over the visible keys, -infinity where a row sees none.
  *   causal: query i sees keys j <= i + Lk - Lq.  q_len / kv_len: int32 [B] on the device or NULL: rows of sample b at or behind its length are
  *   not read (they may hold anything); out, dq, dk, dv are zero and lse is -infinity there.  A row that sees no key: out and dq zero.
@@ -313,7 +313,7 @@ int dbir_attention_bwd(const dbir_attn_desc* d, void* stream);
 
 /* dbir_layernorm_fwd / dbir_layernorm_bwd (csrc/norm_train.hip): rows of C columns, dtype f16 / bf16 / f32 for x, y, dy, dres, dx (row
  *   strides ld*, any alignment), everything else f32.  stats [rows, 2]: mean and 1 / sqrt(variance + eps).
- *   Outputs must not overlap inputs.  dx = gradient of x (+ dres, the gradient that arrives past the norm, if not NULL); dgamma, dbeta [C] are written, not added to.
+ *   C up to 2^28.  Outputs must not overlap inputs.  dx = gradient of x (+ dres, the gradient that arrives past the norm, if not NULL); dgamma, dbeta [C] are written, not added to.
  *   ws: dbir_layernorm_bwd_ws bytes. */
 int dbir_layernorm_bwd_ws(int rows, int C, long long* bytes);
 int dbir_layernorm_fwd(int dtype, const void* x, long long ldx, void* y, long long ldy, const float* gamma, const float* beta,

@@ -146,7 +146,7 @@ def good_desc():
     dict(dtype=2), dict(dtype=-1), dict(B=0), dict(H=0), dict(Hkv=0), dict(H=3, Hkv=2), dict(Lq=0), dict(Lk=0), dict(Lk=-1), dict(B=70000),
     dict(scale=0.0), dict(scale=1e-31), dict(scale=-1.0), dict(scale=float("inf")), dict(scale=float("nan")), dict(q=None), dict(k=None), dict(v=None), dict(out=None),
     dict(lse=None), dict(q=(1 << 20) + 2), dict(q_stride=(0, 60, 64)), dict(k_stride=(0, 32, 64)), dict(v_stride=(0, 1 << 23, 64)),
-    dict(out_stride=(0, 64, 4)), dict(q_stride=(-64, 64, 64)), dict(k_stride=(8192, 128, 4)), dict(dq_stride=(0, 128, 64)), dict(dv_stride=(8192, 128, 0)), dict(dq_stride=(8192, 128, 8)), dict(dk_stride=(56, 128, 64)), dict(dq=1 << 20), dict(dk=6 << 20),
+    dict(out_stride=(0, 64, 4)), dict(q_stride=(-64, 64, 64)), dict(k_stride=(8192, 128, 4)), dict(dq_stride=(0, 128, 64)), dict(dv_stride=(8192, 128, 0)), dict(dq_stride=(8192, 128, 8)), dict(dk_stride=(56, 128, 64)), dict(dq_stride=(8192, 64, 64)), dict(dk_stride=(64, 128, 64)), dict(dv_stride=(8128, 128, 64)), dict(dq_stride=(4096, 128, 4096)), dict(dq=1 << 20), dict(dk=6 << 20),
     dict(dv=2 << 20), dict(dq=8 << 20, dk=8 << 20), dict(dv=7 << 20), dict(dout=None), dict(dq=None), dict(dk=(1 << 20) + 8), dict(dv_stride=(0, 0, 64)),
     dict(ws=None), dict(ws_bytes=16), dict(ws=(1 << 20) + 4)])
 def test_attention_descriptor_refusals(lib, change):
@@ -177,7 +177,7 @@ def test_packed_descriptor_is_the_struct():
 def test_norm_and_embedding_refusals(lib):
     p, r, t, big = 1 << 20, 2 << 20, 3 << 20, 1 << 30
     fwd = [0, p, 8, r, 8, p, p, p, 4, 8, 1e-5, None]
-    for i, v in [(0, 3), (0, -1), (1, None), (2, 7), (3, None), (3, p), (4, 7), (5, None), (7, None), (8, 0), (9, 0), (10, -1.0), (10, float("nan"))]:
+    for i, v in [(0, 3), (0, -1), (1, None), (2, 7), (3, None), (3, p), (4, 7), (5, None), (7, None), (8, 0), (9, 0), (8, (1 << 30) + 1), (10, -1.0), (10, float("nan"))]:
         a = list(fwd)
         a[i] = v
         assert lib.dbir_layernorm_fwd(*a) == 1, (i, v)
@@ -186,6 +186,11 @@ def test_norm_and_embedding_refusals(lib):
         a = list(bwd)
         a[i] = v
         assert lib.dbir_layernorm_bwd(*a) == 1, (i, v)
+    a = list(fwd)
+    a[2] = a[4] = a[9] = (1 << 28) + 1   # columns
+    assert lib.dbir_layernorm_fwd(*a) == 1
+    n = ctypes.c_longlong()
+    assert lib.dbir_layernorm_bwd_ws(4, (1 << 28) + 1, ctypes.byref(n)) == 1 and lib.dbir_layernorm_bwd_ws(4, 1 << 28, ctypes.byref(n)) == 0
     emb = [2, p, 8, p, None, 0, 2, r, 8, 1.0, 6, 3, 8, 5, None]
     for i, v in [(0, 3), (1, None), (2, 7), (3, None), (4, p), (6, 3), (7, None), (7, p), (8, 7), (10, 0), (11, 0), (12, 0), (13, 0), (10, 1 << 30)]:
         a = list(emb)
