@@ -177,6 +177,7 @@ __global__ void tile_accumulate_kernel(const float* __restrict__ tiles, const fl
                                        const int* __restrict__ coords, float* __restrict__ out, int T, int B, int C,
                                        int H, int W, int ts) {
   GRID_STRIDE(i, (long long)B * C * H * W) {
+#pragma clang fp contract(off)   // product and sum are rounded one by one, as in the sharded form: the two have to give the same bits
     const int xx = (int)(i % W);
     const int yy = (int)((i / W) % H);
     const long long bc = i / ((long long)W * H);
@@ -200,6 +201,7 @@ __global__ void tile_accumulate_partial_kernel(const float* __restrict__ tiles, 
                                                const int* __restrict__ coords, float* __restrict__ num, int T, int B,
                                                int C, int H, int W, int ts) {
   GRID_STRIDE(i, (long long)B * C * H * W) {
+#pragma clang fp contract(off)
     const int xx = (int)(i % W);
     const int yy = (int)((i / W) % H);
     const long long bc = i / ((long long)W * H);
