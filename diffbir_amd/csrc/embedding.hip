@@ -34,14 +34,18 @@ struct H16T {
 typedef H16T<F16> F16T;
 typedef H16T<BF16> BF16T;
 
-constexpr int RUN = 64;          // sorted positions of a piece that is summed ahead
-constexpr int RANK_MAX = 16384;  // up to here the sort is one launch that counts for every token how many go before it
+// Sorted positions of a piece that is summed ahead: 39424 positions of 1024 columns, 70 % one token, all sums 63 us (32: 70, 128: 67, without pieces 347).
+constexpr int RUN = 64;
+// Up to here the sort is one launch that counts for every token how many go before it: gradient of 4096 tokens in 49408 x 256 44 us (radix: 60), of 8192
+// 59.6 (71), of 16384 88.7 (90.2).
+constexpr int RANK_MAX = 16384;
 
 __device__ __forceinline__ uint32_t clamp_token(long long t, int vocab) { return (uint32_t)(t < 0 ? 0 : (t >= vocab ? vocab - 1 : t)); }
 
 // ------------------------------------------------------------------------------------------------------------- forward
 // lpr lanes (a power of two) a row, V elements a lane and step; a lane group takes R rows at once: their loads are in flight together, and
-// with positions they are rows of one position (rows `gap` = L apart), which is read once for all of them.
+// with positions they are rows of one position (rows `gap` = L apart), which is read once for all of them.  Bound by memory: 39424 rows of 1024,
+// f32 to bf16, 22 us (about 130 MB, 5.9 TB/s); up to a few hundred rows by the launch (4 us).
 template <typename TT, typename TO, int V, int R>
 __global__ __launch_bounds__(256) void embed_fwd_kernel(const typename TT::elem* __restrict__ table, long long ldt, const long long* __restrict__ tokens,
                                                         const float* __restrict__ pos, long long ldp, typename TO::elem* __restrict__ out, long long ldo,
@@ -98,7 +102,7 @@ __global__ __launch_bounds__(256) void embed_fwd_kernel(const typename TT::elem*
 // ------------------------------------------------------------------------------------------------------------- sort
 // Rank of each token among all: 64 tokens a workgroup, 16 waves that compare them with a sixteenth of every 4096 tokens each.  Of equal tokens the
 // earlier goes first: all that lie before the workgroup's count up to equality, all behind it only below it, and only among its own 64 places are
-// compared.  Two instructions a pair: n^2 / (64 lanes x 1024 SIMDs) of them take less than a radix sort's launches up to RANK_MAX.
+// compared.  154 tokens 2.5 us, 3003 7.4.  Two instructions a pair: n^2 / (64 lanes x 1024 SIMDs) of them take less than a radix sort's launches up to RANK_MAX.
 __global__ __launch_bounds__(1024) void embed_rank_kernel(const long long* __restrict__ tokens, int n, int vocab, uint32_t* __restrict__ skey,
                                                           int* __restrict__ spos) {
   __shared__ __attribute__((aligned(16))) uint32_t keys[4096];
@@ -139,6 +143,7 @@ __global__ __launch_bounds__(1024) void embed_rank_kernel(const long long* __res
 }
 
 // One pass of a stable radix sort over 8 bits: a wave counts / places one segment of `seg` items (a multiple of 64), at most 256 segments.
+// Bound by latency: 39424 tokens 3 us and 10.8 a pass (all loads of a segment ahead of its placing: 12.3 against 11.4 then).
 __global__ __launch_bounds__(256) void embed_count_kernel(const long long* __restrict__ tokens, const uint32_t* __restrict__ key, int n, int vocab,
                                                           int shift, int seg, int nseg, int* __restrict__ hist) {
   __shared__ int cnt[4][256];
@@ -341,6 +346,7 @@ __device__ __forceinline__ void join_waves(float* acc, float (*join)[256], int l
 // NW = 4: one row of the table a workgroup, its positions split over the waves (small tables); NW = 8: 64 rows, 8 a wave, most of them empty,
 // and runs of more than RUN positions split over the waves.  One block of 256 columns either way.  The first pos_rows * (blocks of columns)
 // workgroups make dpos[l], the waves a part of the batch each.  Blocks of columns are adjacent workgroups, so that a long run's all start early.
+// Bound by memory: the gradient of 49408 rows of 1024 is 202 MB, 37 us with 154 positions (5.5 TB/s), 53 with 39424 in bf16 (283 MB, 5.3 TB/s).
 template <typename T, int V, int NW>
 __global__ __launch_bounds__(NW * 64) void embed_rows_kernel(const typename T::elem* __restrict__ dy, long long ldg, const uint32_t* __restrict__ skey,
                                                              const int* __restrict__ spos, const float* __restrict__ part, float* __restrict__ dtable,
@@ -458,7 +464,9 @@ extern "C" int dbir_embedding_fwd(int table_dtype, const void* table, long long 
   int lg = 0;
   while (lg < 6 && (1 << lg) < nv) ++lg;
   const int gap = pos ? L : 1;
-  const int R = ((long long)n << lg) >= 64 * 8192 ? 4 : 1;   // one row a group while that gives fewer than eight waves a SIMD
+  // four rows a group where a row is at most two steps and one row a group is more than eight waves a SIMD (131072 rows of 320 in bf16 41.3 -> 27.9 us,
+  // 65536 of 256 13.8 -> 11.3; rows of 1024, 39424 with positions, f32 -> bf16: 33.7 -> 35.2)
+  const int R = nv <= 128 && ((long long)n << lg) >= 64 * 8192 ? 4 : 1;
   const long long sets = (long long)cdiv(n, (long long)gap * R) * gap;
   DBIR_CHECK_ARG((sets << lg) <= 0xffffff00LL, "dbir_embedding_fwd: too many tokens for one launch");
   const dim3 grid((unsigned)(((sets << lg) + 255) / 256));
