@@ -168,6 +168,13 @@ __global__ __launch_bounds__(threads_of(LPR)) void ln_fwd_kernel(const typename 
 // for the join; 60000 x 1024 f32 138 us (5.3); 4099 x 1283 bf16, element by element, 15.8 (2.7).  Memory bounds both where rows are many and aligned,
 // the number of loads in flight where they are not.
 //
+// A product that is not fused with what is added to it: a constant a = dy gamma leaves nothing behind a - mean(a), where fused the product's rounding
+// would be left, times rstd.
+__device__ __forceinline__ float rounded_product(float a, float b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+
 // dx, and this workgroup's sums of the columns: part[workgroup][0][c] = sum dy xh, [1][c] = sum dy
 template <typename T, int V, int LPR, int VPL>
 __global__ __launch_bounds__(threads_of(LPR)) void ln_bwd_kernel(const typename T::elem* __restrict__ dy, long long ldg, const typename T::elem* __restrict__ x,
@@ -222,7 +229,7 @@ __global__ __launch_bounds__(threads_of(LPR)) void ln_bwd_kernel(const typename 
         xh[i][e] = (xh[i][e] - st.x) * st.y;
         sg[i][e] = __builtin_fmaf(d[i][e], xh[i][e], sg[i][e]);
         sb[i][e] += d[i][e];
-        d[i][e] *= g[i][e];
+        d[i][e] = rounded_product(d[i][e], g[i][e]);
         s1 += d[i][e];
         s2 = __builtin_fmaf(d[i][e], xh[i][e], s2);   // (lanes without a column: d = 0)
       }
@@ -270,6 +277,79 @@ __global__ __launch_bounds__(threads_of(LPR)) void ln_bwd_kernel(const typename 
         for (int e = 0; e < V; ++e) out[which * C + (l + LPR * i) * V + e] = t[e];
       }
     }
+}
+
+// Few rows: one launch.  A workgroup a row for dx, its elements read again from the cache; and behind those a workgroup for 16 columns of dgamma
+// and dbeta, 16 threads a column, which read dy and x once more: the sums need the stats, not dx.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void ln_bwd_few_kernel(const typename T::elem* __restrict__ dy, long long ldg, const typename T::elem* __restrict__ x,
+                                                         long long ldx, const typename T::elem* __restrict__ dres, long long ldr,
+                                                         typename T::elem* __restrict__ dx, long long ldd, const float* __restrict__ gamma,
+                                                         const float* __restrict__ stats, float* __restrict__ dgamma, float* __restrict__ dbeta, int rows,
+                                                         int C) {
+  __shared__ float red[2][16][17];
+  const int tid = threadIdx.x;
+  if ((int)blockIdx.x < rows) {
+    const long long row = blockIdx.x;
+    const float2 st = *reinterpret_cast<const float2*>(stats + 2 * row);
+    float s1 = 0.f, s2 = 0.f;
+    auto terms = [&](int c, float* a, float* xh) {
+      float d[V], g[V];
+      load_vec<T, V>(dy + row * ldg + c, d);
+      load_vec<T, V>(x + row * ldx + c, xh);
+      load_f32<V>(gamma, c, true, g);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        xh[e] = (xh[e] - st.x) * st.y;
+        a[e] = rounded_product(d[e], g[e]);
+      }
+    };
+    for (int c = tid * V; c < C; c += 256 * V) {
+      float a[V], xh[V];
+      terms(c, a, xh);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        s1 += a[e];
+        s2 = __builtin_fmaf(a[e], xh[e], s2);
+      }
+    }
+    s1 = block_sum(s1, red[0][0]) / (float)C;
+    s2 = block_sum(s2, red[1][0]) / (float)C;
+    for (int c = tid * V; c < C; c += 256 * V) {
+      float a[V], xh[V], r[V];
+      terms(c, a, xh);
+      if (dres) load_vec<T, V>(dres + row * ldr + c, r);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        a[e] = st.y * (a[e] - __builtin_fmaf(xh[e], s2, s1));
+        if (dres) a[e] += r[e];
+      }
+      store_vec<T, V>(dx + row * ldd + c, a);
+    }
+    return;
+  }
+  const int lane = tid & 15, sl = tid >> 4, c = ((int)blockIdx.x - rows) * 16 + lane, col = min(c, C - 1);
+  float g = 0.f, b = 0.f;
+#pragma unroll 8
+  for (int row = sl; row < rows; row += 16) {
+    const float2 st = *reinterpret_cast<const float2*>(stats + 2 * row);
+    const float d = T::load(dy + row * ldg + col);
+    g = __builtin_fmaf(d, (T::load(x + row * ldx + col) - st.x) * st.y, g);
+    b += d;
+  }
+  red[0][sl][lane] = g;
+  red[1][sl][lane] = b;
+  __syncthreads();
+  if (sl == 0 && c < C) {
+    g = b = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      g += red[0][i][lane];
+      b += red[1][i][lane];
+    }
+    dgamma[c] = g;
+    dbeta[c] = b;
+  }
 }
 
 // Wider rows than registers hold: a workgroup a row, element by element, read again where it is needed again.
@@ -395,7 +475,11 @@ int bwd_groups(int rows, const Shape& sh) {
   const int n = cdiv(rows, threads_of(sh.lpr) / sh.lpr), most = sh.v > 1 || sh.lpr > 64 || n < 4096 ? 512 : n / 8 < 2048 ? n / 8 : 2048;
   return n < most ? n : most;
 }
+// One launch: 154 x 1024 f32 2.9 us (rows in registers and the join 7.2; a call with its host time 11.5 against 15.8), 512 x 4096 9.8 (18.3), 1024 x 1283
+// 10.9 (12.9); but 1024 x 4096 22.6 (18.8), 2048 x 320 13.2 (7.6).
+bool few_rows(int rows, int C) { return rows <= 1024 && (long long)rows * C <= 1 << 21; }
 int bwd_parts(int rows, int C, int v) {
+  if (few_rows(rows, C)) return 0;
   const Shape sh = shape_of(C, v, false);
   return sh.v ? bwd_groups(rows, sh) : any_chunks(rows, C);
 }
@@ -447,14 +531,26 @@ void launch_fwd(const Shape& sh, const void* x, long long ldx, void* y, long lon
 }
 
 template <typename T>
-void launch_bwd(const Shape& sh, int n, const void* dy, long long ldg, const void* x, long long ldx, const void* dres, long long ldr, void* dx, long long ldd,
-                const float* gamma, const float* stats, float* ws, int rows, int C, hipStream_t s) {
+void launch_bwd(int v, int n, const void* dy, long long ldg, const void* x, long long ldx, const void* dres, long long ldr, void* dx, long long ldd,
+                const float* gamma, const float* stats, float* ws, float* dgamma, float* dbeta, int rows, int C, hipStream_t s) {
   typedef typename T::elem E;
+  if (few_rows(rows, C)) {
+#define GO(V)                                                                                                                                        \
+  hipLaunchKernelGGL((ln_bwd_few_kernel<T, V>), dim3((unsigned)(rows + cdiv(C, 16))), dim3(256), 0, s, (const E*)dy, ldg, (const E*)x, ldx, (const E*)dres, ldr, \
+                     (E*)dx, ldd, gamma, stats, dgamma, dbeta, rows, C)
+    if (v == T::wide) GO(T::wide);
+    else if (v == 4) GO(4);
+    else GO(1);
+#undef GO
+    return;
+  }
+  const Shape sh = shape_of(C, v, false);
   if (!sh.v) {
     hipLaunchKernelGGL(ln_bwd_any_kernel<T>, dim3((unsigned)(rows < 65536 ? rows : 65536)), dim3(256), 0, s, (const E*)dy, ldg, (const E*)x, ldx,
                        (const E*)dres, ldr, (E*)dx, ldd, gamma, stats, rows, C);
     hipLaunchKernelGGL(ln_cols_any_kernel<T>, dim3((unsigned)cdiv(C, 256), (unsigned)n), dim3(256), 0, s, (const E*)dy, ldg, (const E*)x, ldx, stats, ws,
                        rows, C, cdiv(rows, n));
+    hipLaunchKernelGGL(ln_join_kernel, dim3((unsigned)cdiv(2 * C, 16)), dim3(256), 0, s, ws, n, C, dgamma, dbeta);
     return;
   }
 #define GO(TT, V, LPR, VPL)                                                                                                                            \
@@ -465,6 +561,7 @@ void launch_bwd(const Shape& sh, int n, const void* dy, long long ldg, const voi
   else if (sh.lpr == 1024) GO(T, 1, 1024, 8);
   else SINGLE_SHAPES(GO, T);
 #undef GO
+  hipLaunchKernelGGL(ln_join_kernel, dim3((unsigned)cdiv(2 * C, 16)), dim3(256), 0, s, ws, n, C, dgamma, dbeta);
 }
 
 }  // namespace
@@ -501,11 +598,11 @@ extern "C" int dbir_layernorm_fwd(int dtype, const void* x, long long ldx, void*
 extern "C" int dbir_layernorm_bwd(int dtype, const void* dy, long long ldg, const void* x, long long ldx, const void* dres, long long ldr,
                                   void* dx, long long ldd, const float* gamma, const float* stats, float* dgamma, float* dbeta, int rows, int C,
                                   float* ws, long long ws_bytes, void* stream) {
-  DBIR_CHECK_ARG(dy && x && dx && gamma && stats && dgamma && dbeta && ws, "dbir_layernorm_bwd: null pointer");
+  DBIR_CHECK_ARG(dy && x && dx && gamma && stats && dgamma && dbeta, "dbir_layernorm_bwd: null pointer");
   DBIR_CHECK_ARG(rows > 0 && rows <= (1 << 30) && C > 0 && C <= (1 << 28) && ldg >= C && ldx >= C && ldd >= C && (!dres || ldr >= C), "dbir_layernorm_bwd: bad rows / C / ld");
   DBIR_CHECK_ARG(dx != x && dx != dy && dx != dres, "dbir_layernorm_bwd: dx must not be an input");
   DBIR_CHECK_ARG(dtype >= DBIR_F16 && dtype <= DBIR_F32, "dbir_layernorm_bwd: bad dtype %d", dtype);
-  DBIR_CHECK_ARG(((reinterpret_cast<uintptr_t>(stats) & 7) | (reinterpret_cast<uintptr_t>(ws) & 3)) == 0, "dbir_layernorm_bwd: stats must be 8-byte aligned");
+  DBIR_CHECK_ARG((reinterpret_cast<uintptr_t>(stats) & 7) == 0, "dbir_layernorm_bwd: stats must be 8-byte aligned");
   int v = aligned16(gamma) ? vector_of(dtype, C) : 1;
   const void* at[4] = {dy, x, dx, dres ? dres : x};
   const long long lds[4] = {ldg, ldx, ldd, dres ? ldr : ldx};
@@ -513,14 +610,12 @@ extern "C" int dbir_layernorm_bwd(int dtype, const void* dy, long long ldg, cons
     const int vi = vector_of(dtype, C, at[i], lds[i]);
     v = vi < v ? vi : v;
   }
-  const Shape sh = shape_of(C, v, false);
   const int n = bwd_parts(rows, C, v);
-  DBIR_CHECK_ARG(ws_bytes >= 8LL * C * n, "dbir_layernorm_bwd: the workspace must hold %lld bytes", 8LL * C * n);
+  DBIR_CHECK_ARG(n == 0 || (ws && (reinterpret_cast<uintptr_t>(ws) & 3) == 0 && ws_bytes >= 8LL * C * n), "dbir_layernorm_bwd: the workspace must hold %lld bytes", 8LL * C * n);
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (dtype == DBIR_F16) launch_bwd<F16T>(sh, n, dy, ldg, x, ldx, dres, ldr, dx, ldd, gamma, stats, ws, rows, C, s);
-  else if (dtype == DBIR_BF16) launch_bwd<BF16T>(sh, n, dy, ldg, x, ldx, dres, ldr, dx, ldd, gamma, stats, ws, rows, C, s);
-  else launch_bwd<F32T>(sh, n, dy, ldg, x, ldx, dres, ldr, dx, ldd, gamma, stats, ws, rows, C, s);
-  hipLaunchKernelGGL(ln_join_kernel, dim3((unsigned)cdiv(2 * C, 16)), dim3(256), 0, s, ws, n, C, dgamma, dbeta);
+  if (dtype == DBIR_F16) launch_bwd<F16T>(v, n, dy, ldg, x, ldx, dres, ldr, dx, ldd, gamma, stats, ws, dgamma, dbeta, rows, C, s);
+  else if (dtype == DBIR_BF16) launch_bwd<BF16T>(v, n, dy, ldg, x, ldx, dres, ldr, dx, ldd, gamma, stats, ws, dgamma, dbeta, rows, C, s);
+  else launch_bwd<F32T>(v, n, dy, ldg, x, ldx, dres, ldr, dx, ldd, gamma, stats, ws, dgamma, dbeta, rows, C, s);
   DBIR_CHECK_LAUNCH("dbir_layernorm_bwd");
   return DBIR_OK;
 }

@@ -839,10 +839,11 @@ def layernorm_bwd(dy: T, x: T, gamma: T, stats: T, dres: Optional[T] = None, dx:
     M = stats.numel() >> 1
     dgamma, dbeta = torch.empty_like(gamma), torch.empty_like(gamma)
     nws = _ws_bytes("dbir_layernorm_bwd_ws", M, C)
-    ws = torch.empty(nws, dtype=torch.uint8, device=x.device)
+    ws = torch.empty(nws, dtype=torch.uint8, device=x.device) if nws else None
     _train_call("dbir_layernorm_bwd", dev, dt, dy.data_ptr(), _row_ld(dy, "layernorm_bwd: dy"), x.data_ptr(), _row_ld(x, "layernorm_bwd: x"),
                 None if dres is None else dres.data_ptr(), C if dres is None else _row_ld(dres, "layernorm_bwd: dres"), dx.data_ptr(),
-                _row_ld(dx, "layernorm_bwd: dx"), gamma.data_ptr(), stats.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), M, C, ws.data_ptr(), nws)
+                _row_ld(dx, "layernorm_bwd: dx"), gamma.data_ptr(), stats.data_ptr(), dgamma.data_ptr(), dbeta.data_ptr(), M, C,
+                None if ws is None else ws.data_ptr(), nws)
     return dx, dgamma, dbeta
 
 

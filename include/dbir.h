@@ -314,7 +314,7 @@ int dbir_attention_bwd(const dbir_attn_desc* d, void* stream);
 /* dbir_layernorm_fwd / dbir_layernorm_bwd (csrc/norm_train.hip): rows of C columns, dtype f16 / bf16 / f32 for x, y, dy, dres, dx (row
  *   strides ld*, any alignment), everything else f32.  stats [rows, 2]: mean and 1 / sqrt(variance + eps).
  *   C up to 2^28.  Outputs must not overlap inputs.  dx = gradient of x (+ dres, the gradient that arrives past the norm, if not NULL); dgamma, dbeta [C] are written, not added to.
- *   ws: dbir_layernorm_bwd_ws bytes. */
+ *   ws: dbir_layernorm_bwd_ws bytes (0 for few rows: may be NULL). */
 int dbir_layernorm_bwd_ws(int rows, int C, long long* bytes);
 int dbir_layernorm_fwd(int dtype, const void* x, long long ldx, void* y, long long ldy, const float* gamma, const float* beta,
                        float* stats, int rows, int C, float eps, void* stream);

@@ -181,7 +181,7 @@ def test_norm_and_embedding_refusals(lib):
         a = list(fwd)
         a[i] = v
         assert lib.dbir_layernorm_fwd(*a) == 1, (i, v)
-    bwd = [0, p, 8, r, 8, None, 0, t, 8, p, p, p, p, 4, 8, p, big, None]
+    bwd = [0, p, 8, r, 8, None, 0, t, 8, p, p, p, p, 4000, 8, p, big, None]
     for i, v in [(0, 3), (1, None), (2, 7), (4, 7), (5, p), (7, p), (7, r), (8, 7), (9, None), (10, None), (11, None), (12, None), (13, 0), (14, 0), (15, None), (16, 8)]:
         a = list(bwd)
         a[i] = v

@@ -294,7 +294,9 @@ def ln_inputs(shape, dtype, seed, res=True):
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 @pytest.mark.parametrize("rows,C", [(1, 64), (3, 3), (5, 8), (154, 1024), (1000, 320), (257, 640), (66, 1280), (33, 1283), (7, 100), (2, 8192),
-                                    (9, 8200), (1, 20000), (5, 8191), (3, 16384), (300, 1284), (70, 2052), (6000, 101), (4097, 40), (130, 2560), (61, 4096), (19, 5120), (300, 1032)])
+                                    (9, 8200), (1, 20000), (5, 8191), (3, 16384), (300, 1284), (70, 2052), (6000, 101), (4097, 40), (130, 2560), (61, 4096), (19, 5120), (300, 1032)] +
+                         [(1025, C) for C in (8, 40, 256, 320, 512, 999, 1000, 1024, 1284, 1536, 2049, 2052, 2560, 4096, 4097, 4100, 8191, 8192, 9001, 16384, 17000)] +
+                         [(1, 1), (1025, 1), (1024, 2048), (1024, 2049), (1, 300000), (7, 299593)])
 def test_layernorm_train(rows, C, dtype):
     x, dy, gamma, beta, dres = ln_inputs((rows, C), dtype, 31)
     y, stats = ops.layernorm_fwd(x, gamma, beta, eps=1e-5)
@@ -312,10 +314,11 @@ def test_layernorm_train(rows, C, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
-@pytest.mark.parametrize("off,ld", [(0, 336), (8, 336), (1, 321), (3, 1000)])
-def test_layernorm_train_strided_rows(off, ld, dtype):
+@pytest.mark.parametrize("rows", [50, 1100])
+@pytest.mark.parametrize("off,ld", [(0, 336), (8, 336), (4, 324), (1, 321), (3, 1000)])
+def test_layernorm_train_strided_rows(off, ld, rows, dtype):
     """Rows inside wider buffers, also at addresses that no wide load is aligned to; what lies between the rows stays."""
-    rows, C = 50, 320
+    C = 320
     x, dy, gamma, beta, dres = ln_inputs((rows, C), dtype, 32)
     wide = lambda t: torch.full((rows * ld + off,), 7.0, dtype=dtype, device=DEV)[off:].view(rows, ld)[:, :C].copy_(t)  # noqa: E731
     xs, dys, rs, ys, dxs = wide(x), wide(dy), wide(dres), wide(x), wide(x)
