@@ -447,8 +447,9 @@ __device__ __forceinline__ float scale_exp<F16>(const Args& a, int b, int hk, in
 // 40 heads of 4096 x 4096, f16: 387 us, 890 TF/s.  The time follows the number of matrix instructions (half of them left out: 225 us), not the exponentials
 // (7 %), the transposing reads (2 %) or the row reads (5 - 10 %); raising a wave's priority around them loses.
 constexpr int KV_LDS = 2 * (2 * TILE_BYTES + 512);
-template <typename T, bool CAUSAL>
-__device__ __forceinline__ void kv_part(const Args& a, char* lds, int b, int hk, int k0, int split, float e) {
+// LOCAL: the rows' nl2 and nd are in LDS already, [head of the group][tile][nl2 | nd][64].
+template <typename T, bool CAUSAL, bool LOCAL>
+__device__ __forceinline__ void kv_part(const Args& a, char* lds, const float* rows, int b, int hk, int k0, int split, float e) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
   const int bh = b * a.Hkv + hk, grp = a.H / a.Hkv;
   const int nk = clamp_len(a.kv_len, b, a.Lk), nq = clamp_len(a.q_len, b, a.Lq), off = a.Lk - a.Lq;
@@ -465,7 +466,7 @@ __device__ __forceinline__ void kv_part(const Args& a, char* lds, int b, int hk,
     char* p = lds + (it & 1) * (2 * TILE_BYTES + 512);
     stage_tile(p, a.q + b * a.qs[0] + h * a.qs[2], a.qs[1], q0, nq, wave, lane);
     stage_tile(p + TILE_BYTES, a.dout + b * a.gs[0] + h * a.gs[2], a.gs[1], q0, nq, wave, lane);
-    if (wave < 2) {
+    if (!LOCAL && wave < 2) {
       const float* st = (wave ? a.nd : a.nl2) + (long long)(b * a.H + h) * a.Lqp + q0;
       load_lds4(lds_at(p + 2 * TILE_BYTES + wave * 256), buffer_of(st, 256), lane * 4);
     }
@@ -473,9 +474,9 @@ __device__ __forceinline__ void kv_part(const Args& a, char* lds, int b, int hk,
   int it0, it1;
   split_range(nt * grp, split, a.splits, it0, it1);
   if (it0 < it1) stage(it0);
-  auto half = [&](auto masked, const char* qt, int q0, int sb) {
-    const char* gt = qt + TILE_BYTES;
-    const float* st = reinterpret_cast<const float*>(gt + TILE_BYTES);
+  auto half = [&](auto masked, int it, int q0, int sb) {
+    const char *qt = lds + (it & 1) * (2 * TILE_BYTES + 512), *gt = qt + TILE_BYTES;
+    const float* st = LOCAL ? rows + it / nt * 256 + (qt0 + it % nt) * 128 : reinterpret_cast<const float*>(gt + TILE_BYTES);
     f32x16 s = splat(e / c), dp;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
@@ -519,14 +520,14 @@ __device__ __forceinline__ void kv_part(const Args& a, char* lds, int b, int hk,
       if (it + 1 < it1) stage(it + 1);
       if (k0 + wave * 32 >= nk) continue;
 #pragma unroll 1
-      for (int sb = 0; sb < 2; ++sb) half(std::true_type(), lds + (it & 1) * (2 * TILE_BYTES + 512), (qt0 + q) * TILE, sb);
+      for (int sb = 0; sb < 2; ++sb) half(std::true_type(), it, (qt0 + q) * TILE, sb);
     }
     for (; it < it1 && q < nt; ++it, ++q) {
       tile_ready();
       if (it + 1 < it1) stage(it + 1);
       if (k0 + wave * 32 >= nk) continue;
 #pragma unroll 1   // (two in flight do not fit the registers)
-      for (int sb = 0; sb < 2; ++sb) half(std::false_type(), lds + (it & 1) * (2 * TILE_BYTES + 512), 0, sb);
+      for (int sb = 0; sb < 2; ++sb) half(std::false_type(), it, 0, sb);
     }
     q = 0;
   }
@@ -551,7 +552,7 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_kv_kernel(const Args a) {
   int u, blk, split;
   work_of(a, a.B * a.Hkv, (a.Lk + 127) >> 7, u, blk, split);
   const int b = u % a.B, hk = u / a.B;
-  kv_part<T, CAUSAL>(a, lds, b, hk, blk * 128, split, scale_exp<T>(a, b, hk, threadIdx.x, red));
+  kv_part<T, CAUSAL, false>(a, lds, nullptr, b, hk, blk * 128, split, scale_exp<T>(a, b, hk, threadIdx.x, red));
 }
 
 // dq: 128 queries a workgroup, 32 a wave; keys in tiles of 64, double buffered.  D = do . o comes from the ROUNDED o, and where one key has
@@ -560,8 +561,8 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_kv_kernel(const Args a) {
 // subtracts delta times that; else rows of up to two tiles are gone through once more with the corrected D.
 // 40 heads of 4096 x 4096, f16: 286 us, 900 TF/s, at three waves a SIMD (two: 344).  EXACT, 160 heads of 256 x 256, bf16: 16.9 us where the plain one took 15.5; the
 // error of dq against 64 bits falls from 0.0025 to 0.0024, at 2 keys from 0.037 to 0.002.
-template <typename T, bool EXACT>
-__device__ __forceinline__ void q_part(const Args& a, char* lds, int b, int h, int qb, int split, float e) {
+template <typename T, bool EXACT, bool LOCAL>
+__device__ __forceinline__ void q_part(const Args& a, char* lds, float* rows, int b, int h, int qb, int split, float e) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
   const int bh = b * a.H + h, hk = h / (a.H / a.Hkv);
   const int nk = clamp_len(a.kv_len, b, a.Lk), nq = clamp_len(a.q_len, b, a.Lq), off = a.Lk - a.Lq;
@@ -593,9 +594,10 @@ __device__ __forceinline__ void q_part(const Args& a, char* lds, int b, int h, i
     nd += __shfl_xor(nd, 32, 64);
     if (nl2 == -INFINITY) nd = 0.f;
   }
-  float* const to_nd = a.nd + (long long)bh * a.Lqp + row;
+  float* const to_nl2 = LOCAL ? rows + (row >> 6) * 128 + (row & 63) : a.nl2 + (long long)bh * a.Lqp + row;
+  float* const to_nd = LOCAL ? to_nl2 + 64 : a.nd + (long long)bh * a.Lqp + row;
   if (hi == 0 && split == 0 && row < a.Lqp) {
-    a.nl2[(long long)bh * a.Lqp + row] = nl2;
+    *to_nl2 = nl2;
     *to_nd = nd;
   }
   nl2 += e;
@@ -702,7 +704,7 @@ __global__ __launch_bounds__(256, EXACT ? 2 : 3) void attn_bwd_q_kernel(const Ar
   int u, blk, split, b, h;
   work_of(a, a.B * a.H, nqb, u, blk, split);
   head_of(a, u, b, h);
-  q_part<T, EXACT>(a, lds, b, h, a.causal ? nqb - 1 - blk : blk, split, scale_exp<T>(a, b, h / (a.H / a.Hkv), threadIdx.x, red));
+  q_part<T, EXACT, false>(a, lds, nullptr, b, h, a.causal ? nqb - 1 - blk : blk, split, scale_exp<T>(a, b, h / (a.H / a.Hkv), threadIdx.x, red));
 }
 
 // Up to 128 queries and keys: all of a key head in one workgroup and one launch (32 heads of 77 x 77, f16: 15.7 us, latency; as three launches 19.3, and
@@ -710,6 +712,7 @@ __global__ __launch_bounds__(256, EXACT ? 2 : 3) void attn_bwd_q_kernel(const Ar
 template <typename T, bool CAUSAL>
 __global__ __launch_bounds__(256, 2) void attn_bwd_small_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char lds[KV_LDS];
+  __shared__ __attribute__((aligned(16))) float rows[4 * 256];   // up to four heads
   __shared__ float red[4];
   const int tid = threadIdx.x, b = blockIdx.x / a.Hkv, hk = blockIdx.x % a.Hkv, grp = a.H / a.Hkv;
   float e = 0.f;
@@ -721,10 +724,10 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_small_kernel(const Args a) {
     e = exponent_for(sqrtf(x) * sqrtf(block_max(norm2_part<T>(a.v + b * a.vs[0] + hk * a.vs[2], a.vs[1], 0, clamp_len(a.kv_len, b, a.Lk), tid), red, tid)));
   }
   for (int h = hk * grp; h < hk * grp + grp; ++h) {
-    q_part<T, true>(a, lds, b, h, 0, 0, e);
-    tile_ready();   // its nl2 and nd are written, for the next part; the tiles in LDS are done with
+    q_part<T, true, true>(a, lds, rows + (h - hk * grp) * 256, b, h, 0, 0, e);
+    tile_ready();   // its nl2 and nd are written, for the other part; the tiles in LDS are done with
   }
-  kv_part<T, CAUSAL>(a, lds, b, hk, 0, 0, e);
+  kv_part<T, CAUSAL, true>(a, lds, rows, b, hk, 0, 0, e);
 }
 
 // ---------------------------------------------------------------------------------------------------------------- host
@@ -829,7 +832,7 @@ Plan plan_of(int dtype, int B, int H, int Hkv, int Lq, int Lk) {
   p.kv = splits_of(groups, rounds);
   if (p.kv == 1 && groups < 1024 && rounds >= 64) p.kv = 2;
   p.lqp = ((long long)Lq + 63) / 64 * 64;
-  p.rows_floats = (bh * p.lqp * 2 + (dtype == DBIR_F16 ? bh * (p.lqp / 64) + bk * ((Lk + 63) / 64) : 0) + 3) / 4 * 4;
+  p.rows_floats = p.small ? 0 : (bh * p.lqp * 2 + (dtype == DBIR_F16 ? bh * (p.lqp / 64) + bk * ((Lk + 63) / 64) : 0) + 3) / 4 * 4;
   const long long nq = p.q > 1 && !p.small ? p.q * bh * Lq * (HD + 1) : 0, nk = p.kv > 1 && !p.small ? p.kv * bk * Lk * 128 : 0;
   p.part_floats = nq > nk ? nq : nk;
   return p;
@@ -911,7 +914,7 @@ extern "C" int dbir_attention_bwd(const dbir_attn_desc* d, void* stream) {
   if (int rc = check_desc(d, name, true)) return rc;
   const Plan p = plan_of(d->dtype, d->B, d->H, d->Hkv, d->Lq, d->Lk);
   const long long need = (p.rows_floats + p.part_floats) * 4, bh = (long long)d->B * d->H;
-  DBIR_CHECK_ARG(d->ws && d->ws_bytes >= need && (reinterpret_cast<uintptr_t>(d->ws) & 15) == 0,
+  DBIR_CHECK_ARG(!need || (d->ws && d->ws_bytes >= need && (reinterpret_cast<uintptr_t>(d->ws) & 15) == 0),
                  "%s: the workspace must hold %lld bytes, 16-byte aligned", name, need);
   Args a = to_args(d);
   a.nl2 = reinterpret_cast<float*>(d->ws);

@@ -164,10 +164,6 @@ __global__ __launch_bounds__(threads_of(LPR)) void ln_fwd_kernel(const typename 
   }
 }
 
-// Forward above, 32768 x 320 f16: 11.3 us (3.7 TB/s); 60000 x 1024 f32 98 us (5.0).  Backward, 32768 x 320 f16 with a residual: 18.8 us (4.5 TB/s), and 3.8
-// for the join; 60000 x 1024 f32 138 us (5.3); 4099 x 1283 bf16, element by element, 15.8 (2.7).  Memory bounds both where rows are many and aligned,
-// the number of loads in flight where they are not.
-//
 // A product that is not fused with what is added to it: a constant a = dy gamma leaves nothing behind a - mean(a), where fused the product's rounding
 // would be left, times rstd.
 __device__ __forceinline__ float rounded_product(float a, float b) {
@@ -175,6 +171,9 @@ __device__ __forceinline__ float rounded_product(float a, float b) {
   return a * b;
 }
 
+// Forward (above), 32768 x 320 f16: 11.3 us (3.7 TB/s); 60000 x 1024 f32 98 us (5.0).  Backward, 32768 x 320 f16 with a residual: 18.8 us (4.5 TB/s), and 3.8
+// for the join; 60000 x 1024 f32 138 us (5.3); 4099 x 1283 bf16, element by element, 15.8 (2.7).  Memory bounds both where rows are many and aligned,
+// the number of loads in flight where they are not.
 // dx, and this workgroup's sums of the columns: part[workgroup][0][c] = sum dy xh, [1][c] = sum dy
 template <typename T, int V, int LPR, int VPL>
 __global__ __launch_bounds__(threads_of(LPR)) void ln_bwd_kernel(const typename T::elem* __restrict__ dy, long long ldg, const typename T::elem* __restrict__ x,

@@ -795,10 +795,10 @@ def attention_bwd(dout: T, q: T, k: T, v: T, out: T, lse: T, scale: float, causa
         raise ValueError("attention_bwd: the head dimension must have unit stride")
     lens = _attn_lens("attention_bwd", B, q_len, kv_len)
     nws = _ws_bytes("dbir_attention_bwd_ws", _dt(q), B, H, ks[2], Lq, ks[1])
-    ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
+    ws = torch.empty(nws, dtype=torch.uint8, device=q.device) if nws else None
     _train_call("dbir_attention_bwd", dev, _ATTN_PACK(
         _dt(q), B, H, ks[2], Lq, ks[1], bool(causal), scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), *lens,
-        dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), nws, *[n for x in st for n in x[:3]]))
+        dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr() if nws else 0, nws, *[n for x in st for n in x[:3]]))
     return dq, dk, dv
 
 

@@ -292,7 +292,7 @@ int dbir_xf_tail(int dtype, const void* attn_out, long long ldo, const void* h, 
  *   causal: query i sees keys j <= i + Lk - Lq.  q_len / kv_len: int32 [B] on the device or NULL: rows of sample b at or behind its length are
  *   not read (they may hold anything); out, dq, dk, dv are zero and lse is -infinity there.  A row that sees no key: out and dq zero.
  *   The backward pass takes out and lse of the forward pass.  ws: dbir_attention_bwd_ws bytes (forward: dbir_attention_fwd_ws), 16-byte
- *   aligned. */
+ *   aligned (0 bytes for few rows: may be NULL). */
 typedef struct {
   int dtype, B, H, Hkv, Lq, Lk, causal;
   float scale;

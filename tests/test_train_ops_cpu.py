@@ -148,7 +148,7 @@ def good_desc():
     dict(lse=None), dict(q=(1 << 20) + 2), dict(q_stride=(0, 60, 64)), dict(k_stride=(0, 32, 64)), dict(v_stride=(0, 1 << 23, 64)),
     dict(out_stride=(0, 64, 4)), dict(q_stride=(-64, 64, 64)), dict(k_stride=(8192, 128, 4)), dict(dq_stride=(0, 128, 64)), dict(dv_stride=(8192, 128, 0)), dict(dq_stride=(8192, 128, 8)), dict(dk_stride=(56, 128, 64)), dict(dq_stride=(8192, 64, 64)), dict(dk_stride=(64, 128, 64)), dict(dv_stride=(8128, 128, 64)), dict(dq_stride=(4096, 128, 4096)), dict(dq=1 << 20), dict(dk=6 << 20),
     dict(dv=2 << 20), dict(dq=8 << 20, dk=8 << 20), dict(dv=7 << 20), dict(dout=None), dict(dq=None), dict(dk=(1 << 20) + 8), dict(dv_stride=(0, 0, 64)),
-    dict(ws=None), dict(ws_bytes=16), dict(ws=(1 << 20) + 4)])
+    dict(ws=None, Lk=129, B=1), dict(ws_bytes=16, Lk=129, B=1), dict(ws=(1 << 20) + 4, Lk=129, B=1)])
 def test_attention_descriptor_refusals(lib, change):
     d = good_desc()
     for n, v in change.items():
