@@ -707,8 +707,8 @@ __global__ __launch_bounds__(256, EXACT ? 2 : 3) void attn_bwd_q_kernel(const Ar
   q_part<T, EXACT, false>(a, lds, nullptr, b, h, a.causal ? nqb - 1 - blk : blk, split, scale_exp<T>(a, b, h / (a.H / a.Hkv), threadIdx.x, red));
 }
 
-// Up to 128 queries and keys: all of a key head in one workgroup and one launch (32 heads of 77 x 77, f16: 15.7 us, latency; as three launches 19.3, and
-// 5 us more of the host's time).
+// Up to 128 queries and keys: all of a key head in one workgroup and one launch (32 heads of 77 x 77, f16: 14.7 us, latency; as three launches 19.3, and
+// 5 us more of the host's time).  The rows' nl2 and nd stay in LDS (through memory 15.7).
 template <typename T, bool CAUSAL>
 __global__ __launch_bounds__(256, 2) void attn_bwd_small_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char lds[KV_LDS];
