@@ -557,10 +557,12 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_kv_kernel(const Args a) {
 
 // dq: 128 queries a workgroup, 32 a wave; keys in tiles of 64, double buffered.  D = do . o comes from the ROUNDED o, and where one key has
 // most of a row, dp - D is far below D.  The exact D makes sum_j ds_ij zero, so the sum of the ds that are formed with the rounded one is its error,
-// delta: it corrects D for the dk kernel.  For dq, EXACT (up to 512 keys, where the error shows) also sums p_ij k_j, a third more products, and
-// subtracts delta times that; else rows of up to two tiles are gone through once more with the corrected D.
-// 40 heads of 4096 x 4096, f16: 286 us, 900 TF/s, at three waves a SIMD (two: 344).  EXACT, 160 heads of 256 x 256, bf16: 16.9 us where the plain one took 15.5; the
-// error of dq against 64 bits falls from 0.0025 to 0.0024, at 2 keys from 0.037 to 0.002.
+// delta: it corrects D for the dk kernel.  For dq, EXACT (up to 512 keys, where the error shows) also sums p_ij k_j and
+// subtracts delta times that, and takes what the rounding of ds to 16 bits left as a product of its own: two thirds more products, and dq is as exact as its
+// own rounding.  Else p and ds are rounded once, as in the dk kernel, which makes the error that of two roundings (f16 0.0003, bf16 0.0024 where the
+// result's own is 0.0002 and 0.0017), and rows of up to two tiles are gone through once more with the corrected D.
+// 40 heads of 4096 x 4096, f16: 286 us, 900 TF/s, at three waves a SIMD (two: 344).  EXACT, 160 heads of 256 x 256, bf16: 17.5 us (without
+// the rest of ds 16.0, without the sum of p k too 15.5); error of dq against 64 bits 0.0017, 0.0024, 0.0025, and at 2 keys 0.037 without either.
 template <typename T, bool EXACT, bool LOCAL>
 __device__ __forceinline__ void q_part(const Args& a, char* lds, float* rows, int b, int h, int qb, int split, float e) {
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), hi = lane >> 5;
@@ -639,13 +641,23 @@ __device__ __forceinline__ void q_part(const Args& a, char* lds, float* rows, in
 #pragma unroll
     for (int hf = 0; hf < 2; ++hf) {
       const typename T::vec8 df = pack_frag<T>(dp, hf);
-      typename T::vec8 pf;
-      if constexpr (EXACT) pf = pack_frag<T>(s, hf);
+      typename T::vec8 pf, lf;
+      if constexpr (EXACT) {
+        pf = pack_frag<T>(s, hf);
+        float x[8];
+        unpack8<T>(__builtin_bit_cast(uint4, df), x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dp[8 * hf + i] -= x[i];
+        lf = pack_frag<T>(dp, hf);   // what the rounding of ds left
+      }
 #pragma unroll
       for (int d = 0; d < 2; ++d) {
         const typename T::vec8 kc = cols_frag<T>(kt, kb * 32 + hf * 16, d * 32, lane);
         acc[d] = T::mfma32(kc, df, acc[d]);
-        if constexpr (EXACT) accp[d] = T::mfma32(kc, pf, accp[d]);
+        if constexpr (EXACT) {
+          acc[d] = T::mfma32(kc, lf, acc[d]);
+          accp[d] = T::mfma32(kc, pf, accp[d]);
+        }
       }
     }
   };
@@ -707,8 +719,8 @@ __global__ __launch_bounds__(256, EXACT ? 2 : 3) void attn_bwd_q_kernel(const Ar
   q_part<T, EXACT, false>(a, lds, nullptr, b, h, a.causal ? nqb - 1 - blk : blk, split, scale_exp<T>(a, b, h / (a.H / a.Hkv), threadIdx.x, red));
 }
 
-// Up to 128 queries and keys: all of a key head in one workgroup and one launch (32 heads of 77 x 77, f16: 14.7 us, latency; as three launches 19.3, and
-// 5 us more of the host's time).  The rows' nl2 and nd stay in LDS (through memory 15.7).
+// Up to 128 queries and keys: all of a key head in one workgroup and one launch (32 heads of 77 x 77, f16: 15.1 us, latency; as three launches 19.3, and
+// 5 us more of the host's time).  The rows' nl2 and nd stay in LDS (through memory a microsecond more).
 template <typename T, bool CAUSAL>
 __global__ __launch_bounds__(256, 2) void attn_bwd_small_kernel(const Args a) {
   __shared__ __attribute__((aligned(16))) char lds[KV_LDS];
